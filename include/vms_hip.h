@@ -499,6 +499,54 @@ int vms_param_prep(const vms_prep_params *p, void *stream);
 int vms_sum_slices(const void *src, int src_dtype, int n_slices, int64_t n, int64_t slice_stride, void *dst, int dst_dtype, void *stream);
 int vms_sizeof_prep_params(void);
 
+/* ---- gated delta rule ------------------------------------------------------------------------------------
+ * Per batch entry and head, state S (dk, dv), a_t = exp(g_t):
+ *   S' = a_t S_{t-1};  u_t = beta_t (v_t - S'^T k_t);  S_t = S' + k_t u_t^T;  out_t = scale S_t^T q_t
+ * q, k (batch, seqlen, heads_k, dk), v, out (batch, seqlen, heads, dv) in dtype, unit stride along dk / dv; head h reads q / k head
+ * h / (heads / heads_k).  g, beta (batch, seqlen, heads) in gate_dtype: dtype or VMS_F32.  initial_state, final_state
+ * (batch, heads, dk, dv) fp32 contiguous, optional.  seq_lens (batch) int32 on the device, optional: tokens behind an entry's length
+ * (clamped to 0 .. seqlen) are padding: they leave the state alone and their out is 0.  reverse: right to left over the valid tokens.
+ * 1 <= dk <= 128, 1 <= dv <= 4096.  workspace: vms_gated_delta_workspace_bytes(), 16-byte aligned; with for_backward it holds
+ * what the backward of the same call reads, and goes to vms_gated_delta_bwd unchanged. */
+typedef struct {
+    int32_t batch, seqlen, heads, heads_k, dk, dv;
+    int32_t dtype, gate_dtype;
+    int32_t reverse, for_backward;
+    float scale;
+    int32_t reserved;
+    const void *q, *k, *v, *g, *beta;
+    const float *initial_state;
+    const int32_t *seq_lens;
+    void *out;
+    float *final_state;
+    int64_t q_batch_stride, q_seq_stride, q_head_stride, k_batch_stride, k_seq_stride, k_head_stride;
+    int64_t v_batch_stride, v_seq_stride, v_head_stride, out_batch_stride, out_seq_stride, out_head_stride;
+    int64_t g_batch_stride, g_seq_stride, g_head_stride, beta_batch_stride, beta_seq_stride, beta_head_stride;
+    void *workspace;
+    int64_t workspace_bytes;
+} vms_gated_delta_params;
+
+/* backward.  f: the forward's block with for_backward set and its workspace (out, final_state and initial_state are not read).  dout in dtype
+ * (batch, seqlen, heads, dv) with its strides; dfinal_state fp32 optional.  Written whole, contiguous: dq, dk (batch, seqlen, heads_k, dk),
+ * dv (batch, seqlen, heads, dv) in dtype, dg, dbeta (batch, seqlen, heads) in gate_dtype, dinitial_state fp32 optional; zeros on padding. */
+typedef struct {
+    vms_gated_delta_params f;
+    const void *dout;
+    const float *dfinal_state;
+    void *dq, *dk, *dv, *dg, *dbeta;
+    float *dinitial_state;
+    int64_t dout_batch_stride, dout_seq_stride, dout_head_stride;
+    void *workspace;                  /* vms_gated_delta_bwd_workspace_bytes(), 16-byte aligned: scratch of this call alone */
+    int64_t workspace_bytes;
+} vms_gated_delta_bwd_params;
+
+int vms_gated_delta_fwd(const vms_gated_delta_params *p, void *stream);
+int vms_gated_delta_bwd(const vms_gated_delta_bwd_params *p, void *stream);
+int64_t vms_gated_delta_workspace_bytes(const vms_gated_delta_params *p);
+int64_t vms_gated_delta_bwd_workspace_bytes(const vms_gated_delta_params *p);
+int vms_sizeof_gated_delta_params(void);
+int vms_sizeof_gated_delta_bwd_params(void);
+
 int vms_abi_version(void);
 const char *vms_last_error(void);       /* thread-local, valid until the next failing call */
 /* thread-local: the kernel family the last successful launch call of this thread enqueued, e.g. "scan_fwd_pair",

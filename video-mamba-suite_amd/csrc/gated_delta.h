@@ -1,0 +1,249 @@
+// gated_delta.h -- what the gated delta rule's kernels share (gated_delta_fwd.hip, gated_delta_bwd.hip): the chunk's
+// algebra, operand precision, fragment layouts and the workspace they pass from kernel to kernel.
+//
+// Per batch entry and head, S (dk x dv), a_t = exp(g_t):
+//   S' = a_t S_{t-1};  e_t = v_t - S'^T k_t;  u_t = beta_t e_t;  S_t = S' + k_t u_t^T;  o_t = scale S_t^T q_t
+// over 64 tokens at once (G = cumulative sum of g inside the chunk, gam = exp(G), del = exp(G_63 - G), L_ij = exp(G_i - G_j)):
+//   N_ij = L_ij k_i.k_j (i > j);  T = (I + diag(beta) N)^-1;  M_ij = scale L_ij q_i.k_j (i >= j)
+//   U = T beta (V - gam K S0);  O = scale gam Q S0 + M U;  S1 = gam_63 S0 + K^T (del U)
+// T, M and the gates depend on no state: one parallel launch makes them for every chunk; what is left for the sequential walk
+// over the chunks is four products per chunk.
+//
+// Precision.  Everything runs on the bf16 matrix cores with fp32 accumulators.  An operand is the sum of 1 .. 3 bf16 planes
+// (8 bits of the significand each), so that
+//   inputs are exact:             bf16 1 plane, fp16 2, fp32 3                                             (NX)
+//   the state's recurrence is carried with 2 planes (3 for fp32 inputs): the state's error per chunk is ~2^-18 (2^-24) and does
+//     not grow to the 2^-9 of one plane, since final states are fp32 and errors in S live on over chunks    (NS)
+//   what only enters outputs of the inputs' type is held in that type's precision: 1 plane for bf16, 2, 3     (NO)
+#pragma once
+#include "vms_common.h"
+
+namespace vms {
+namespace gd {
+
+constexpr int C = 64;   // tokens of a chunk
+
+using bf16x8 = vec_t<bf16_t, 8>;
+using bf16x4 = vec_t<bf16_t, 4>;
+using f32x4 = vec_t<float, 4>;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+template <typename T> struct Prec;
+template <> struct Prec<bf16_t> { static constexpr int NX = 1, NS = 2, NO = 1; };
+template <> struct Prec<f16_t> { static constexpr int NX = 2, NS = 2, NO = 2; };
+template <> struct Prec<float> { static constexpr int NX = 3, NS = 3, NO = 3; };
+
+// An operand of v_mfma_f32_16x16x32_bf16: lane = 16 p + n holds row (A) / column (B) n and 8 of the 32 contracted indices.
+// Two index orders are in use (any order is right as long as both operands share it):
+//   natural   element e of quarter p = index 8 p + e          (16-byte reads of a row)
+//   paired    e < 4: 4 p + e, else 16 + 4 p + (e - 4)          (the accumulators of two 16-row tiles ARE the operand:
+//                                                               a product's result enters the next product without moving)
+template <int N> struct Frag { bf16x8 p[N]; };
+
+template <int KEEP, int NA, int NB>
+__device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB>& b) {
+#pragma unroll
+    for (int s = KEEP - 1; s >= 0; --s)   // the smallest products first
+#pragma unroll
+        for (int i = 0; i <= s; ++i)
+            if (i < NA && s - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], acc, 0, 0, 0);
+}
+
+// x -> N bf16 planes whose sum is x up to 2^-(8 N + 1) (round to nearest each)
+template <int N>
+__device__ __forceinline__ void split(float (&x)[8], Frag<N>& f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            f.p[i][e] = static_cast<bf16_t>(x[e]);
+            if (i + 1 < N) x[e] -= static_cast<float>(f.p[i][e]);
+        }
+}
+template <int N>
+__device__ __forceinline__ Frag<N> frag_of(const f32x4& a, const f32x4& b) {   // two 16-row tiles, paired order
+    float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    Frag<N> f;
+    split<N>(x, f);
+    return f;
+}
+
+// 8 elements as they stand in memory
+template <typename T> struct Raw8 { T v[8]; };
+// columns c .. c+7 of a row of n (`ok` = the row exists), zeros outside; rows have any alignment
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* row, int c, int n, bool ok) {
+    Raw8<T> r;
+    if (ok && c + 8 <= n) {
+        __builtin_memcpy(&r, row + c, sizeof(r));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.v[e] = ok && c + e < n ? row[c + e] : static_cast<T>(0.f);
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ Frag<Prec<T>::NX> planes_of(const Raw8<T>& r) {
+    Frag<Prec<T>::NX> f;
+    if constexpr (Prec<T>::NX == 1) {
+        __builtin_memcpy(&f.p[0], &r, 16);
+    } else {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(r.v[e]);
+        split<Prec<T>::NX>(x, f);
+    }
+    return f;
+}
+
+// B operand that copies columns 16 half .. 16 half + 15 of a paired-order operand out of a product: D = A I.  Turns an operand
+// whose lanes hold a column (4 consecutive rows in a register each) into one whose lanes hold a row: 8-byte stores instead of 2-byte ones.
+__device__ __forceinline__ bf16x8 unit_frag(int half, int n, int p) {
+    bf16x8 f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = static_cast<bf16_t>((e >> 2) == half && 4 * p + (e & 3) == n ? 1.f : 0.f);
+    return f;
+}
+
+// ---- a (64 tokens x KP) tile of q or k in LDS: NX planes, rows of 2 KP + 16 bytes (16 rows of one quarter fall on all banks), the
+// columns of every 32 in paired order (position 8 p + 4 half + r of column 16 half + 4 p + r), so that one 16-byte read is an operand
+template <int KP> constexpr int tile_row() { return 2 * KP + 16; }
+template <int KP> constexpr int tile_bytes() { return C * tile_row<KP>(); }
+template <int KP, int NX>
+__device__ __forceinline__ void tile_put(char* tile, int row, int c, const Frag<NX>& f) {   // columns c .. c+7, c % 8 == 0
+    const int pos = (c & ~31) + 8 * ((c & 15) >> 2) + 4 * ((c & 31) >> 4);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+        char* d = tile + i * tile_bytes<KP>() + row * tile_row<KP>() + 2 * pos;
+        reinterpret_cast<bf16x4*>(d)[0] = __builtin_shufflevector(f.p[i], f.p[i], 0, 1, 2, 3);
+        reinterpret_cast<bf16x4*>(d + 16)[0] = __builtin_shufflevector(f.p[i], f.p[i], 4, 5, 6, 7);
+    }
+}
+// lane: token 16 rt + n, columns of block kb in paired order
+template <int KP, int NX>
+__device__ __forceinline__ Frag<NX> tile_rows(const char* tile, int rt, int kb, int n, int p) {
+    Frag<NX> f;
+#pragma unroll
+    for (int i = 0; i < NX; ++i)
+        f.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * tile_bytes<KP>() + (16 * rt + n) * tile_row<KP>() + 2 * (32 * kb + 8 * p));
+    return f;
+}
+__device__ __forceinline__ bf16x4 read_tr(const char* at) {   // 4 x 16 elements transposed among 16 lanes
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at));
+}
+__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// lane: column 16 m + n, tokens of block tb (32) in paired order.  ds_read_b64_tr_b16: lane i of 16 names row i / 4, column group i % 4
+template <int KP, int NX>
+__device__ __forceinline__ Frag<NX> tile_cols(const char* tile, int m, int tb, int n, int p) {
+    Frag<NX> f;
+    const char* at = tile + (32 * tb + 4 * p + (n >> 2)) * tile_row<KP>() + 2 * (32 * (m >> 1) + 8 * (n & 3) + 4 * (m & 1));
+#pragma unroll
+    for (int i = 0; i < NX; ++i)
+        f.p[i] = join(read_tr(at + i * tile_bytes<KP>()), read_tr(at + i * tile_bytes<KP>() + 16 * tile_row<KP>()));
+    return f;
+}
+
+// ---- lower triangular 64 x 64 matrices (T, M): the six 16 x 32 operands that hold something, in operand order (1 KB each, lane by lane)
+constexpr int kTri = 6 * 1024;   // bytes of one plane
+__device__ __host__ constexpr int tri(int rt, int kb) { return rt < 2 ? rt : 2 + 2 * (rt - 2) + kb; }
+template <int N>
+__device__ __forceinline__ Frag<N> tri_rows(const char* m, int rt, int kb, int lane) {   // lane: row 16 rt + n, columns of block kb
+    Frag<N> f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(m + i * kTri + 1024 * tri(rt, kb) + 16 * lane);
+    return f;
+}
+template <int N>
+__device__ __forceinline__ Frag<N> tri_cols(const char* m, int ct, int ib, int n, int p) {   // lane: column 16 ct + n, rows of block ib
+    Frag<N> f;
+    const int at = 16 * (16 * (n & 3) + 4 * p + (n >> 2)) + 8 * (ct & 1);
+    const int kb = ct >> 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        f.p[i] = join(read_tr(m + i * kTri + 1024 * tri(2 * ib, kb) + at), read_tr(m + i * kTri + 1024 * tri(2 * ib + 1, kb) + at));
+    return f;
+}
+
+// ---- what a chunk leaves in the workspace; slot = (batch entry * heads + head) * chunks + chunk
+struct Gates { float gam[C], bet[C], del[C]; double G[C]; };
+struct Layout {
+    int64_t tri, gates, S0, U;                      // byte offsets of the arrays in the forward's workspace
+    int64_t dS, Y;                                  // ... in the backward's own
+    int64_t tri_slot, s_slot, u_slot;               // bytes per chunk (T and M; S0 / dS; U / Y)
+    int64_t bytes, bwd_bytes;
+    int chunks, vpad;
+};
+__host__ __device__ __forceinline__ int ceil_to(int a, int b) { return (a + b - 1) / b * b; }
+__host__ __device__ __forceinline__ int pad_k(int dk) { return dk <= 64 ? 64 : 128; }
+__host__ inline Layout layout(const vms_gated_delta_params& p) {
+    Layout l{};
+    const int ns = p.dtype == VMS_F32 ? 3 : 2, no = p.dtype == VMS_F32 ? 3 : p.dtype == VMS_F16 ? 2 : 1;
+    l.chunks = (p.seqlen + C - 1) / C;
+    l.vpad = ceil_to(p.dv, 32);
+    const int64_t slots = (int64_t)p.batch * p.heads * l.chunks;
+    l.tri_slot = (int64_t)2 * ns * kTri;              // the planes of T, then those of M
+    l.s_slot = (int64_t)no * pad_k(p.dk) * l.vpad * 2;
+    l.u_slot = (int64_t)no * C * l.vpad * 2;
+    int64_t at = 0;
+    auto take = [&](int64_t n) { int64_t o = at; at += (n + 255) / 256 * 256; return o; };
+    l.tri = take(slots * l.tri_slot);
+    l.gates = take(slots * (int64_t)sizeof(Gates));
+    if (p.for_backward) {
+        l.S0 = take(slots * l.s_slot);
+        l.U = take(slots * l.u_slot);
+    }
+    l.bytes = at;
+    at = 0;
+    l.dS = take(slots * l.s_slot);
+    l.Y = take(slots * l.u_slot);
+    l.bwd_bytes = at;
+    return l;
+}
+
+// position in memory of the i-th token of the walk (valid for i < len); rows >= len are padding and stay where they are
+__device__ __forceinline__ int token(int i, int len, int reverse) { return reverse ? len - 1 - i : i; }
+__device__ __forceinline__ int length_of(const vms_gated_delta_params& p, int b) {
+    if (!p.seq_lens) return p.seqlen;
+    const int n = p.seq_lens[b];
+    return n < 0 ? 0 : n > p.seqlen ? p.seqlen : n;
+}
+// workgroup -> (batch * heads + head, slice): the slices of one head share q, k, T and M, so they go to one XCD's L2 (workgroups
+// are dealt to the 8 XCDs in turn)
+__device__ __forceinline__ void pair_of(int id, int pairs, int slices, int& pair, int& slice) {
+    if (pairs % 8 == 0) {
+        const int in = id >> 3;
+        slice = in % slices;
+        pair = (in / slices) * 8 + (id & 7);
+    } else {
+        slice = id % slices;
+        pair = id / slices;
+    }
+}
+
+__device__ __forceinline__ float ld_gate(const void* p, int64_t i, int dt) {
+    if (dt == VMS_F32) return static_cast<const float*>(p)[i];
+    if (dt == VMS_F16) return static_cast<float>(static_cast<const f16_t*>(p)[i]);
+    return static_cast<float>(static_cast<const bf16_t*>(p)[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int c, int n, const f32x4& v) {   // columns c .. c+3 of a row of n
+    if (c + 4 <= n) {
+        T o[4] = {static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+        __builtin_memcpy(row + c, o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < n) row[c + e] = static_cast<T>(v[e]);
+    }
+}
+__device__ __forceinline__ void store_planes4(char* at, const f32x4& v) {   // an exact bf16 plane that went through unit_frag
+    bf16x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<bf16_t>(v[e]);
+    *reinterpret_cast<bf16x4*>(at) = o;
+}
+
+int validate(const vms_gated_delta_params& p);   // gated_delta_fwd.hip
+
+}  // namespace gd
+}  // namespace vms

@@ -113,6 +113,25 @@ class StateUpdateParams(ctypes.Structure):
     )
 
 
+class GatedDeltaParams(ctypes.Structure):
+    _fields_ = (
+        [(n, _i32) for n in ("batch", "seqlen", "heads", "heads_k", "dk", "dv", "dtype", "gate_dtype", "reverse", "for_backward")]
+        + [("scale", ctypes.c_float), ("reserved", _i32)]
+        + [(n, _vp) for n in ("q", "k", "v", "g", "beta", "initial_state", "seq_lens", "out", "final_state")]
+        + [(f"{t}_{d}_stride", _i64) for t in ("q", "k", "v", "out", "g", "beta") for d in ("batch", "seq", "head")]
+        + [("workspace", _vp), ("workspace_bytes", _i64)]
+    )
+
+
+class GatedDeltaBwdParams(ctypes.Structure):
+    _fields_ = (
+        [("f", GatedDeltaParams)]
+        + [(n, _vp) for n in ("dout", "dfinal_state", "dq", "dk", "dv", "dg", "dbeta", "dinitial_state")]
+        + [(n, _i64) for n in ("dout_batch_stride", "dout_seq_stride", "dout_head_stride")]
+        + [("workspace", _vp), ("workspace_bytes", _i64)]
+    )
+
+
 class ProjApplyParams(ctypes.Structure):
     _fields_ = (
         [(n, _i32) for n in ("batch", "rows", "k", "seqlen", "dtype", "accumulate", "tiles_per_wg", "reserved")]
@@ -182,6 +201,8 @@ EXPORTS = (
     "vms_selective_scan_bwd_dual", "vms_scan_bwd_dual_fused",
     "vms_proj_kred", "vms_sizeof_proj_kred_params",
     "vms_conv_xproj_dual", "vms_sizeof_conv_xproj_dual_params", "vms_layer_norm_bwd_finish", "vms_sum_slices",
+    "vms_gated_delta_fwd", "vms_gated_delta_bwd", "vms_gated_delta_workspace_bytes", "vms_gated_delta_bwd_workspace_bytes",
+    "vms_sizeof_gated_delta_params", "vms_sizeof_gated_delta_bwd_params",
 )
 
 ABI_VERSION = 11   # include/vms_hip.h VMS_ABI_VERSION: checked against libvms_hip.so and against the compiled binding
@@ -361,7 +382,8 @@ def lib():
                          ("norm", NormParams), ("norm_bwd", NormBwdParams), ("state_update", StateUpdateParams),
                          ("proj_apply", ProjApplyParams), ("proj_wgrad", ProjWgradParams),
                          ("proj_conv_bwd", ProjConvBwdParams), ("prep", PrepParams), ("conv_fwd_dual", ConvFwdDualParams),
-                         ("proj_kred", ProjKredParams), ("conv_xproj_dual", ConvXprojDualParams)):
+                         ("proj_kred", ProjKredParams), ("conv_xproj_dual", ConvXprojDualParams),
+                         ("gated_delta", GatedDeltaParams), ("gated_delta_bwd", GatedDeltaBwdParams)):
             n = getattr(L, f"vms_sizeof_{name}_params")()
             if n != ctypes.sizeof(st):
                 raise ImportError(f"ABI mismatch: {name} params are {n} bytes in the library, "
@@ -371,6 +393,8 @@ def lib():
         for fn in EXPORTS[11:14]:
             getattr(L, fn).restype = ctypes.c_int64
         L.vms_scan_x_pitch.restype = ctypes.c_int64
+        for fn in ("vms_gated_delta_workspace_bytes", "vms_gated_delta_bwd_workspace_bytes"):
+            getattr(L, fn).restype = ctypes.c_int64
         L.vms_scan_x_pitch.argtypes = [ctypes.c_void_p, ctypes.c_int32]
         _lib = L
     return _lib
@@ -996,6 +1020,46 @@ def state_update(state, x, dt, A, B, C, D, z, dt_bias, out, dt_softplus):
     P.B_batch_stride, P.B_n_stride = B.stride()
     P.C_batch_stride, P.C_n_stride = C.stride()
     _call("vms_selective_state_update", P, x)
+
+
+# ---- gated delta rule (csrc/gated_delta_fwd.hip, gated_delta_bwd.hip) ----------------------------------------
+def _fill_gated_delta(P, q, k, v, g, beta, scale, seq_lens, reverse, for_backward):
+    P.batch, P.seqlen, P.heads, P.dv = v.shape
+    P.heads_k, P.dk = k.shape[2:]
+    P.dtype, P.gate_dtype = dtype_code(v), dtype_code(g)
+    P.reverse, P.for_backward, P.scale = int(bool(reverse)), int(bool(for_backward)), float(scale)
+    P.q, P.k, P.v, P.g, P.beta, P.seq_lens = _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(seq_lens)
+    P.q_batch_stride, P.q_seq_stride, P.q_head_stride = q.stride()[:3]
+    P.k_batch_stride, P.k_seq_stride, P.k_head_stride = k.stride()[:3]
+    P.v_batch_stride, P.v_seq_stride, P.v_head_stride = v.stride()[:3]
+    P.g_batch_stride, P.g_seq_stride, P.g_head_stride = g.stride()
+    P.beta_batch_stride, P.beta_seq_stride, P.beta_head_stride = beta.stride()
+
+
+def gated_delta_fwd(q, k, v, g, beta, scale, initial_state, seq_lens, reverse, out, final_state, for_backward):
+    """q, k, v, out: unit last stride; initial_state / final_state: contiguous fp32.  -> the workspace, which gated_delta_bwd of the same
+    call reads (for_backward)"""
+    P = GatedDeltaParams()
+    _fill_gated_delta(P, q, k, v, g, beta, scale, seq_lens, reverse, for_backward)
+    P.initial_state, P.final_state, P.out = _ptr(initial_state), _ptr(final_state), _ptr(out)
+    P.out_batch_stride, P.out_seq_stride, P.out_head_stride = out.stride()[:3]
+    ws = torch.empty(lib().vms_gated_delta_workspace_bytes(ctypes.byref(P)), dtype=torch.uint8, device=v.device)
+    P.workspace, P.workspace_bytes = _ptr(ws), ws.numel()
+    _call("vms_gated_delta_fwd", P, v)
+    return ws
+
+
+def gated_delta_bwd(q, k, v, g, beta, scale, seq_lens, reverse, ws, dout, dfinal_state, dq, dk, dv, dg, dbeta, dinitial_state):
+    """dq .. dbeta, dinitial_state: contiguous, written whole"""
+    Q = GatedDeltaBwdParams()
+    _fill_gated_delta(Q.f, q, k, v, g, beta, scale, seq_lens, reverse, True)
+    Q.f.workspace, Q.f.workspace_bytes = _ptr(ws), ws.numel()
+    Q.dout, Q.dfinal_state, Q.dinitial_state = _ptr(dout), _ptr(dfinal_state), _ptr(dinitial_state)
+    Q.dq, Q.dk, Q.dv, Q.dg, Q.dbeta = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(dbeta)
+    Q.dout_batch_stride, Q.dout_seq_stride, Q.dout_head_stride = dout.stride()[:3]
+    own = torch.empty(lib().vms_gated_delta_bwd_workspace_bytes(ctypes.byref(Q.f)), dtype=torch.uint8, device=v.device)
+    Q.workspace, Q.workspace_bytes = _ptr(own), own.numel()
+    _call("vms_gated_delta_bwd", Q, v)
 
 
 class PrepPlan:
