@@ -547,6 +547,61 @@ int64_t vms_gated_delta_bwd_workspace_bytes(const vms_gated_delta_params *p);
 int vms_sizeof_gated_delta_params(void);
 int vms_sizeof_gated_delta_bwd_params(void);
 
+/* one token: state (batch, heads, dk, dv) in / out in state_dtype, (dk, dv) contiguous; q, k (batch, heads_k, dk), v, out (batch, heads, dv) in
+ * dtype, unit last stride; g, beta (batch, heads) in gate_dtype (dtype or VMS_F32).  The arithmetic is fp32; a 16-bit state is rounded as
+ * it is stored, out is computed before that rounding. */
+typedef struct {
+    int32_t batch, heads, heads_k, dk, dv;
+    int32_t state_dtype, dtype, gate_dtype;
+    float scale;
+    int32_t reserved;
+    void *state;
+    const void *q, *k, *v, *g, *beta;
+    void *out;
+    int64_t state_batch_stride, state_head_stride, q_batch_stride, q_head_stride, k_batch_stride, k_head_stride;
+    int64_t v_batch_stride, v_head_stride, out_batch_stride, out_head_stride, g_batch_stride, g_head_stride, beta_batch_stride, beta_head_stride;
+} vms_gated_delta_step_params;
+
+int vms_gated_delta_state_update(const vms_gated_delta_step_params *p, void *stream);
+int vms_sizeof_gated_delta_step_params(void);
+
+/* ---- norm after a block, gate, scaled residual add, norm before the next block -----------------------------
+ * h = norm(x; post_weight, post_bias);  residual_out = residual_scale * residual + gate * h;  y = norm(residual_out; pre_weight, pre_bias)
+ * x, y (rows, cols) in x_dtype; residual, residual_out in res_dtype (x_dtype or VMS_F32), residual may be NULL (zeros); unit column strides.
+ * weights, biases (cols) fp32, biases may be NULL.  gate in gate_dtype, may be NULL: (rows / rows_per_gate, cols), row i of the problem reads gate
+ * row i / rows_per_gate (rows: one for all; 1: one each).  y is the norm of the sum before its rounding to res_dtype.  stats (rows, 4) fp32,
+ * 16-byte aligned: mean and 1 / deviation of both norms, for the backward (may be NULL).  cols <= 8192. */
+typedef struct {
+    int32_t rows, cols;
+    int32_t x_dtype, res_dtype, gate_dtype, is_rms;
+    float eps, residual_scale;
+    int64_t rows_per_gate;
+    const void *x, *residual, *gate;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias;
+    void *y, *residual_out;
+    float *stats;
+    int64_t x_row_stride, residual_row_stride, gate_row_stride, y_row_stride, residual_out_row_stride;
+} vms_sandwich_norm_params;
+
+/* backward.  f: the forward's block (y, residual_out are not read), stats required.  dy in x_dtype, dresidual_out in res_dtype: either may
+ * be NULL (zero).  dx in x_dtype, dresidual in res_dtype (may be NULL).  dgate (required with gate) contiguous in gate_dtype; dpost_weight, dpre_weight
+ * fp32 (cols), dpost_bias, dpre_bias may be NULL.  Everything is written whole. */
+typedef struct {
+    vms_sandwich_norm_params f;
+    const void *dy, *dresidual_out;
+    void *dx, *dresidual, *dgate;
+    float *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+    int64_t dy_row_stride, dresidual_out_row_stride, dx_row_stride, dresidual_row_stride;
+    void *workspace;                  /* vms_sandwich_norm_bwd_workspace_bytes(&f) */
+    int64_t workspace_bytes;
+} vms_sandwich_norm_bwd_params;
+
+int vms_sandwich_norm_fwd(const vms_sandwich_norm_params *p, void *stream);
+int vms_sandwich_norm_bwd(const vms_sandwich_norm_bwd_params *p, void *stream);
+int64_t vms_sandwich_norm_bwd_workspace_bytes(const vms_sandwich_norm_params *p);
+int vms_sizeof_sandwich_norm_params(void);
+int vms_sizeof_sandwich_norm_bwd_params(void);
+
 int vms_abi_version(void);
 const char *vms_last_error(void);       /* thread-local, valid until the next failing call */
 /* thread-local: the kernel family the last successful launch call of this thread enqueued, e.g. "scan_fwd_pair",

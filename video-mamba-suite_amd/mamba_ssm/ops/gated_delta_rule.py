@@ -32,6 +32,9 @@ def _check_inputs(q, k, v, g, beta, lead):
     _check(g.dtype == beta.dtype and g.dtype in (v.dtype, torch.float32), "g and beta must have one dtype: fp32 or that of v")
     for t in (q, k, g, beta):
         _check(t.device == v.device, "all tensors must be on one device")
+
+
+def _check_gpu(v):
     _check(v.is_cuda, "tensors must be on a GPU (no CPU path in this library)")
 
 
@@ -83,6 +86,8 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
     if seq_lens is not None:
         _check(tuple(seq_lens.shape) == (batch,) and seq_lens.device == v.device and seq_lens.dtype in (torch.int32, torch.int64),
                "seq_lens must be int32 or int64 (batch,) on the device of v")
+    _check_gpu(v)
+    if seq_lens is not None:
         # clamped before the narrowing: a 64-bit length must not wrap
         seq_lens = seq_lens.clamp(0, seqlen).to(torch.int32).contiguous() if seq_lens.dtype == torch.int64 else seq_lens.contiguous()
     scale = dk ** -0.5 if scale is None else float(scale)
@@ -117,3 +122,45 @@ def gated_delta_rule_ref(q, k, v, g, beta, scale=None, initial_state=None, retur
         finals.append(S)
     out = torch.stack(outs).to(v.dtype)
     return (out, torch.stack(finals).to(state_dtype)) if return_final_state else out
+
+
+def _separate_states(state):
+    """(batch, heads) states that each stand for themselves: (dk, dv) contiguous, none on top of another"""
+    batch, heads, dk, dv = state.shape
+    if not (dv == 1 or state.stride(3) == 1) or not (dk == 1 or state.stride(2) == dv):
+        return False
+    least = dk * dv
+    for stride, n in sorted((state.stride(i), state.shape[i]) for i in (0, 1) if state.shape[i] > 1):
+        if stride < least:
+            return False
+        least = stride * n
+    return True
+
+
+def gated_delta_state_update(state, q, k, v, g, beta, scale=None):
+    """One token.  state (batch, heads, dk, dv) [in/out], fp32, fp16 or bf16, each (dk, dv) contiguous; q, k (batch, heads_k, dk), v (batch, heads, dv),
+    one dtype; g, beta (batch, heads), that dtype or fp32; scale: default dk ** -0.5 -> out (batch, heads, dv).  The arithmetic is fp32; a
+    16-bit state is rounded as it is stored, out is computed before that rounding.  Not differentiable."""
+    _check_inputs(q, k, v, g, beta, 1)
+    _check(state.dim() == 4 and tuple(state.shape) == (*v.shape[:2], k.shape[-1], v.shape[-1]), "state must be (batch, heads, dk, dv)")
+    _check(state.dtype in (torch.float32, torch.float16, torch.bfloat16) and state.device == v.device, "state must be fp32, fp16 or bf16 on the device of v")
+    _check(_separate_states(state), "the (dk, dv) states must be contiguous and must not overlap: they are updated in place")
+    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in (state, q, k, v, g, beta))),
+           "the single-token step has no gradient: call it under torch.no_grad(), or gated_delta_rule_fn")
+    _check_gpu(v)
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if v.numel():
+        _k.gated_delta_step(state, _unit_last(q), _unit_last(k), _unit_last(v), g, beta, k.shape[-1] ** -0.5 if scale is None else scale, out)
+    return out
+
+
+def gated_delta_state_update_ref(state, q, k, v, g, beta, scale=None):
+    """The same in plain PyTorch (fp32, or fp64 for fp64 inputs); runs anywhere."""
+    acc = torch.float64 if v.dtype == torch.float64 else torch.float32
+    rep = v.shape[1] // k.shape[1]
+    q, k = (t.to(acc).repeat_interleave(rep, 1) for t in (q, k))
+    S = state.to(acc) * g.to(acc).exp()[..., None, None]
+    u = beta.to(acc)[..., None] * (v.to(acc) - (S * k[..., None]).sum(-2))
+    S = S + k[..., None] * u[..., None, :]
+    state.copy_(S)
+    return ((k.shape[-1] ** -0.5 if scale is None else scale) * (S * q[..., None]).sum(-2)).to(v.dtype)

@@ -132,6 +132,33 @@ class GatedDeltaBwdParams(ctypes.Structure):
     )
 
 
+class GatedDeltaStepParams(ctypes.Structure):
+    _fields_ = (
+        [(n, _i32) for n in ("batch", "heads", "heads_k", "dk", "dv", "state_dtype", "dtype", "gate_dtype")]
+        + [("scale", ctypes.c_float), ("reserved", _i32)]
+        + [(n, _vp) for n in ("state", "q", "k", "v", "g", "beta", "out")]
+        + [(f"{t}_{d}_stride", _i64) for t in ("state", "q", "k", "v", "out", "g", "beta") for d in ("batch", "head")]
+    )
+
+
+class SandwichNormParams(ctypes.Structure):
+    _fields_ = (
+        [(n, _i32) for n in ("rows", "cols", "x_dtype", "res_dtype", "gate_dtype", "is_rms")]
+        + [("eps", ctypes.c_float), ("residual_scale", ctypes.c_float), ("rows_per_gate", _i64)]
+        + [(n, _vp) for n in ("x", "residual", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "y", "residual_out", "stats")]
+        + [(f"{t}_row_stride", _i64) for t in ("x", "residual", "gate", "y", "residual_out")]
+    )
+
+
+class SandwichNormBwdParams(ctypes.Structure):
+    _fields_ = (
+        [("f", SandwichNormParams)]
+        + [(n, _vp) for n in ("dy", "dresidual_out", "dx", "dresidual", "dgate", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias")]
+        + [(f"{t}_row_stride", _i64) for t in ("dy", "dresidual_out", "dx", "dresidual")]
+        + [("workspace", _vp), ("workspace_bytes", _i64)]
+    )
+
+
 class ProjApplyParams(ctypes.Structure):
     _fields_ = (
         [(n, _i32) for n in ("batch", "rows", "k", "seqlen", "dtype", "accumulate", "tiles_per_wg", "reserved")]
@@ -203,6 +230,9 @@ EXPORTS = (
     "vms_conv_xproj_dual", "vms_sizeof_conv_xproj_dual_params", "vms_layer_norm_bwd_finish", "vms_sum_slices",
     "vms_gated_delta_fwd", "vms_gated_delta_bwd", "vms_gated_delta_workspace_bytes", "vms_gated_delta_bwd_workspace_bytes",
     "vms_sizeof_gated_delta_params", "vms_sizeof_gated_delta_bwd_params",
+    "vms_gated_delta_state_update", "vms_sizeof_gated_delta_step_params",
+    "vms_sandwich_norm_fwd", "vms_sandwich_norm_bwd", "vms_sandwich_norm_bwd_workspace_bytes",
+    "vms_sizeof_sandwich_norm_params", "vms_sizeof_sandwich_norm_bwd_params",
 )
 
 ABI_VERSION = 11   # include/vms_hip.h VMS_ABI_VERSION: checked against libvms_hip.so and against the compiled binding
@@ -383,7 +413,9 @@ def lib():
                          ("proj_apply", ProjApplyParams), ("proj_wgrad", ProjWgradParams),
                          ("proj_conv_bwd", ProjConvBwdParams), ("prep", PrepParams), ("conv_fwd_dual", ConvFwdDualParams),
                          ("proj_kred", ProjKredParams), ("conv_xproj_dual", ConvXprojDualParams),
-                         ("gated_delta", GatedDeltaParams), ("gated_delta_bwd", GatedDeltaBwdParams)):
+                         ("gated_delta", GatedDeltaParams), ("gated_delta_bwd", GatedDeltaBwdParams),
+                         ("gated_delta_step", GatedDeltaStepParams), ("sandwich_norm", SandwichNormParams),
+                         ("sandwich_norm_bwd", SandwichNormBwdParams)):
             n = getattr(L, f"vms_sizeof_{name}_params")()
             if n != ctypes.sizeof(st):
                 raise ImportError(f"ABI mismatch: {name} params are {n} bytes in the library, "
@@ -393,7 +425,7 @@ def lib():
         for fn in EXPORTS[11:14]:
             getattr(L, fn).restype = ctypes.c_int64
         L.vms_scan_x_pitch.restype = ctypes.c_int64
-        for fn in ("vms_gated_delta_workspace_bytes", "vms_gated_delta_bwd_workspace_bytes"):
+        for fn in ("vms_gated_delta_workspace_bytes", "vms_gated_delta_bwd_workspace_bytes", "vms_sandwich_norm_bwd_workspace_bytes"):
             getattr(L, fn).restype = ctypes.c_int64
         L.vms_scan_x_pitch.argtypes = [ctypes.c_void_p, ctypes.c_int32]
         _lib = L
@@ -1060,6 +1092,62 @@ def gated_delta_bwd(q, k, v, g, beta, scale, seq_lens, reverse, ws, dout, dfinal
     own = torch.empty(lib().vms_gated_delta_bwd_workspace_bytes(ctypes.byref(Q.f)), dtype=torch.uint8, device=v.device)
     Q.workspace, Q.workspace_bytes = _ptr(own), own.numel()
     _call("vms_gated_delta_bwd", Q, v)
+
+
+def gated_delta_step(state, q, k, v, g, beta, scale, out):
+    P = GatedDeltaStepParams()
+    P.batch, P.heads, P.dk, P.dv = state.shape
+    P.heads_k = k.shape[1]
+    P.state_dtype, P.dtype, P.gate_dtype, P.scale = dtype_code(state), dtype_code(v), dtype_code(g), float(scale)
+    P.state, P.q, P.k, P.v, P.g, P.beta, P.out = _ptr(state), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(out)
+    P.state_batch_stride, P.state_head_stride = state.stride()[:2]
+    P.q_batch_stride, P.q_head_stride = q.stride()[:2]
+    P.k_batch_stride, P.k_head_stride = k.stride()[:2]
+    P.v_batch_stride, P.v_head_stride = v.stride()[:2]
+    P.out_batch_stride, P.out_head_stride = out.stride()[:2]
+    P.g_batch_stride, P.g_head_stride = g.stride()
+    P.beta_batch_stride, P.beta_head_stride = beta.stride()
+    _call("vms_gated_delta_state_update", P, v)
+
+
+# ---- norm after a block + gate + residual + norm before the next (csrc/sandwich_norm.hip) ---------------------
+def _fill_sandwich(P, x, residual, gate, rows_per_gate, post_w, post_b, pre_w, pre_b, res_dtype, residual_scale, eps, is_rms, stats):
+    P.rows, P.cols = x.shape
+    P.x_dtype, P.res_dtype, P.is_rms = dtype_code(x), _DTYPE[res_dtype], int(bool(is_rms))
+    P.eps, P.residual_scale = float(eps), float(residual_scale)
+    P.x, P.residual, P.gate = _ptr(x), _ptr(residual), _ptr(gate)
+    P.post_weight, P.post_bias, P.pre_weight, P.pre_bias, P.stats = _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(stats)
+    P.x_row_stride = x.stride(0)
+    if residual is not None:
+        P.residual_row_stride = residual.stride(0)
+    if gate is not None:
+        P.gate_dtype, P.rows_per_gate, P.gate_row_stride = dtype_code(gate), int(rows_per_gate), gate.stride(0)
+
+
+def sandwich_norm_fwd(x, residual, gate, rows_per_gate, post_w, post_b, pre_w, pre_b, y, residual_out, stats, residual_scale, eps, is_rms):
+    """x, residual, gate, y, residual_out: 2-D, unit column stride; weights / biases: contiguous fp32 (cols); stats: fp32 (rows, 4) or None"""
+    P = SandwichNormParams()
+    _fill_sandwich(P, x, residual, gate, rows_per_gate, post_w, post_b, pre_w, pre_b, residual_out.dtype, residual_scale, eps, is_rms, stats)
+    P.y, P.residual_out, P.y_row_stride, P.residual_out_row_stride = _ptr(y), _ptr(residual_out), y.stride(0), residual_out.stride(0)
+    _call("vms_sandwich_norm_fwd", P, x)
+
+
+def sandwich_norm_bwd(x, residual, gate, rows_per_gate, post_w, post_b, pre_w, pre_b, stats, res_dtype, residual_scale, eps, is_rms,
+                      dy, dres_out, dx, dres, dgate, dpost_w, dpost_b, dpre_w, dpre_b):
+    Q = SandwichNormBwdParams()
+    _fill_sandwich(Q.f, x, residual, gate, rows_per_gate, post_w, post_b, pre_w, pre_b, res_dtype, residual_scale, eps, is_rms, stats)
+    Q.dy, Q.dresidual_out, Q.dx, Q.dresidual, Q.dgate = _ptr(dy), _ptr(dres_out), _ptr(dx), _ptr(dres), _ptr(dgate)
+    Q.dpost_weight, Q.dpost_bias, Q.dpre_weight, Q.dpre_bias = _ptr(dpost_w), _ptr(dpost_b), _ptr(dpre_w), _ptr(dpre_b)
+    Q.dx_row_stride = dx.stride(0)
+    if dy is not None:
+        Q.dy_row_stride = dy.stride(0)
+    if dres_out is not None:
+        Q.dresidual_out_row_stride = dres_out.stride(0)
+    if dres is not None:
+        Q.dresidual_row_stride = dres.stride(0)
+    ws = torch.empty(lib().vms_sandwich_norm_bwd_workspace_bytes(ctypes.byref(Q.f)), dtype=torch.uint8, device=x.device)
+    Q.workspace, Q.workspace_bytes = _ptr(ws), ws.numel()
+    _call("vms_sandwich_norm_bwd", Q, x)
 
 
 class PrepPlan:
