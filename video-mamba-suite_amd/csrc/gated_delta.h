@@ -68,17 +68,33 @@ __device__ __forceinline__ Frag<N> frag_of(const f32x4& a, const f32x4& b) {   /
     return f;
 }
 
-// 8 elements as they stand in memory
+// 8 elements of a row as they stand in memory: columns c .. c+7 of a row of n, any alignment.  WHOLE: n % 8 == 0, one 16- or 32-byte load;
+// otherwise element by element.  Never a branch: what lies outside is read from a place that exists and becomes zero in clear(), when it is
+// used.  (Behind a branch the loads of the next chunk meet the other side's values in a register copy, which waits for them at once: a chunk of
+// the walk took 5.7 us.)
 template <typename T> struct Raw8 { T v[8]; };
-// columns c .. c+7 of a row of n (`ok` = the row exists), zeros outside; rows have any alignment
-template <typename T>
-__device__ __forceinline__ Raw8<T> load_raw8(const T* row, int c, int n, bool ok) {
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* row, int c, int n) {
     Raw8<T> r;
-    if (ok && c + 8 <= n) {
-        __builtin_memcpy(&r, row + c, sizeof(r));
+    if constexpr (WHOLE) {
+        __builtin_memcpy(&r, row + (c < n ? c : 0), sizeof(r));
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r.v[e] = ok && c + e < n ? row[c + e] : static_cast<T>(0.f);
+        for (int e = 0; e < 8; ++e) r.v[e] = row[c + e < n ? c + e : 0];
+    }
+    return r;
+}
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Raw8<T> clear(Raw8<T> r, int c, int n, bool ok) {   // ok: the row exists
+    if constexpr (WHOLE) {
+        unsigned w[sizeof(r) / 4];
+        __builtin_memcpy(w, &r, sizeof(r));
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(r) / 4); ++i) w[i] = ok && c < n ? w[i] : 0u;
+        __builtin_memcpy(&r, w, sizeof(r));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.v[e] = ok && c + e < n ? r.v[e] : static_cast<T>(0.f);
     }
     return r;
 }
@@ -105,28 +121,13 @@ __device__ __forceinline__ bf16x8 unit_frag(int half, int n, int p) {
     return f;
 }
 
-// ---- a (64 tokens x KP) tile of q or k in LDS: NX planes, rows of 2 KP + 16 bytes (16 rows of one quarter fall on all banks), the
-// columns of every 32 in paired order (position 8 p + 4 half + r of column 16 half + 4 p + r), so that one 16-byte read is an operand
-template <int KP> constexpr int tile_row() { return 2 * KP + 16; }
+// ---- a (64 tokens x KP) tile of q or k in LDS: NX planes, rows of 2 KP + 32 bytes (the 16 rows a transposing read touches start 8 banks apart)
+template <int KP> constexpr int tile_row() { return 2 * KP + 32; }
 template <int KP> constexpr int tile_bytes() { return C * tile_row<KP>(); }
 template <int KP, int NX>
-__device__ __forceinline__ void tile_put(char* tile, int row, int c, const Frag<NX>& f) {   // columns c .. c+7, c % 8 == 0
-    const int pos = (c & ~31) + 8 * ((c & 15) >> 2) + 4 * ((c & 31) >> 4);
+__device__ __forceinline__ void tile_put(char* tile, int row, int c, const Frag<NX>& f) {   // columns c .. c+7
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-        char* d = tile + i * tile_bytes<KP>() + row * tile_row<KP>() + 2 * pos;
-        reinterpret_cast<bf16x4*>(d)[0] = __builtin_shufflevector(f.p[i], f.p[i], 0, 1, 2, 3);
-        reinterpret_cast<bf16x4*>(d + 16)[0] = __builtin_shufflevector(f.p[i], f.p[i], 4, 5, 6, 7);
-    }
-}
-// lane: token 16 rt + n, columns of block kb in paired order
-template <int KP, int NX>
-__device__ __forceinline__ Frag<NX> tile_rows(const char* tile, int rt, int kb, int n, int p) {
-    Frag<NX> f;
-#pragma unroll
-    for (int i = 0; i < NX; ++i)
-        f.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * tile_bytes<KP>() + (16 * rt + n) * tile_row<KP>() + 2 * (32 * kb + 8 * p));
-    return f;
+    for (int i = 0; i < NX; ++i) *reinterpret_cast<bf16x8*>(tile + i * tile_bytes<KP>() + row * tile_row<KP>() + 2 * c) = f.p[i];
 }
 __device__ __forceinline__ bf16x4 read_tr(const char* at) {   // 4 x 16 elements transposed among 16 lanes
     return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at));
@@ -136,12 +137,40 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_sh
 template <int KP, int NX>
 __device__ __forceinline__ Frag<NX> tile_cols(const char* tile, int m, int tb, int n, int p) {
     Frag<NX> f;
-    const char* at = tile + (32 * tb + 4 * p + (n >> 2)) * tile_row<KP>() + 2 * (32 * (m >> 1) + 8 * (n & 3) + 4 * (m & 1));
+    const char* at = tile + (32 * tb + 4 * p + (n >> 2)) * tile_row<KP>() + 2 * (16 * m + 4 * (n & 3));
 #pragma unroll
     for (int i = 0; i < NX; ++i)
         f.p[i] = join(read_tr(at + i * tile_bytes<KP>()), read_tr(at + i * tile_bytes<KP>() + 16 * tile_row<KP>()));
     return f;
 }
+
+// ---- what the waves of a walk hand each other: N planes of a matrix by columns, CT x 16 columns (lane n) x `len` rows of the matrix, 4 consecutive
+// ones (a register quadruple) written at a time, 8 (an operand) read.  Rows of 2 len + 16 bytes: 16 lanes of a quarter fall on all banks.
+template <int N, int CT, int LEN>
+struct Exchange {
+    static constexpr int kRow = 2 * LEN + 16, kPlane = CT * 16 * kRow, kBytes = N * kPlane;
+    char* base;
+    __device__ __forceinline__ void put(int j, int n, int at, const f32x4& v) const {
+        float x[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            bf16x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h[e] = static_cast<bf16_t>(x[e]);
+                if (i + 1 < N) x[e] -= static_cast<float>(h[e]);
+            }
+            *reinterpret_cast<bf16x4*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at) = h;
+        }
+    }
+    __device__ __forceinline__ Frag<N> get(int j, int n, int at) const {
+        Frag<N> f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at);
+        return f;
+    }
+};
+__device__ __forceinline__ int paired(int tile, int p) { return 32 * (tile >> 1) + 8 * p + 4 * (tile & 1); }   // where rows 16 tile + 4 p .. + 3 stand
 
 // ---- lower triangular 64 x 64 matrices (T, M): the six 16 x 32 operands that hold something, in operand order (1 KB each, lane by lane)
 constexpr int kTri = 6 * 1024;   // bytes of one plane
@@ -153,14 +182,13 @@ __device__ __forceinline__ Frag<N> tri_rows(const char* m, int rt, int kb, int l
     for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(m + i * kTri + 1024 * tri(rt, kb) + 16 * lane);
     return f;
 }
+// their transposes, for the backward: lane = column 16 ct + n, rows of block ib (those with ib >= ct / 2)
+__device__ __host__ constexpr int tri_t(int ct, int ib) { return ct < 2 ? 2 * ct + ib : 4 + (ct - 2); }
 template <int N>
-__device__ __forceinline__ Frag<N> tri_cols(const char* m, int ct, int ib, int n, int p) {   // lane: column 16 ct + n, rows of block ib
+__device__ __forceinline__ Frag<N> tri_cols(const char* m, int ct, int ib, int lane) {
     Frag<N> f;
-    const int at = 16 * (16 * (n & 3) + 4 * p + (n >> 2)) + 8 * (ct & 1);
-    const int kb = ct >> 1;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        f.p[i] = join(read_tr(m + i * kTri + 1024 * tri(2 * ib, kb) + at), read_tr(m + i * kTri + 1024 * tri(2 * ib + 1, kb) + at));
+    for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(m + i * kTri + 1024 * tri_t(ct, ib) + 16 * lane);
     return f;
 }
 
@@ -181,7 +209,7 @@ __host__ inline Layout layout(const vms_gated_delta_params& p) {
     l.chunks = (p.seqlen + C - 1) / C;
     l.vpad = ceil_to(p.dv, 32);
     const int64_t slots = (int64_t)p.batch * p.heads * l.chunks;
-    l.tri_slot = (int64_t)2 * ns * kTri;              // the planes of T, then those of M
+    l.tri_slot = (int64_t)(p.for_backward ? 4 : 2) * ns * kTri;   // the planes of T, those of M, and of their transposes
     l.s_slot = (int64_t)no * pad_k(p.dk) * l.vpad * 2;
     l.u_slot = (int64_t)no * C * l.vpad * 2;
     int64_t at = 0;
@@ -241,6 +269,26 @@ __device__ __forceinline__ void store_planes4(char* at, const f32x4& v) {   // a
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = static_cast<bf16_t>(v[e]);
     *reinterpret_cast<bf16x4*>(at) = o;
+}
+
+inline int allow_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
+    if (bytes <= 65536) return VMS_OK;
+    const hipError_t e = once.run([&] { return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+    if (e != hipSuccess) { set_error("hipFuncSetAttribute: %s", hipGetErrorString(e)); return VMS_ERR_LAUNCH; }
+    return VMS_OK;
+}
+// one 16 x 16 accumulator tile (rows row0 + 4 p + r, column col0 + n) into NO planes of (rows, vpad): through unit_frag, so that a lane
+// stores 4 consecutive columns of one row
+template <int NO>
+__device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int row0, int col0, const f32x4& v, int n, int p) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const Frag<NO> f = frag_of<NO>(v, zero);
+    if (col0 < vpad) {
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+            store_planes4(base + 2 * (((int64_t)i * rows + row0 + n) * vpad + col0 + 4 * p),
+                          __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, p), zero, 0, 0, 0));
+    }
 }
 
 int validate(const vms_gated_delta_params& p);   // gated_delta_fwd.hip

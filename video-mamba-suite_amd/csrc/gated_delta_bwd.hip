@@ -23,29 +23,27 @@ struct BwdArgs {   // what the kernels need of vms_gated_delta_bwd_params (one k
 };
 
 // ---- the walk over the chunks, from the end ------------------------------------------------------------------
-template <typename T, int KP, int NW, int CT>
-__global__ __launch_bounds__(NW * 64, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
+// Split among the four waves as the forward's walk: wave w has token tile w of dU and Y and dk / 4 rows of dS.  Three exchanges per chunk: dS, dU, Y;
+// dO of the next chunk is handed over while dS is updated, Q and K go through LDS for their transposes.
+template <typename T, int KP, int CT, bool WHOLE>
+__global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
-    constexpr int NT = NW * 64, KB = KP / 32, DT = KP / 16;
-    constexpr int TB = tile_bytes<KP>();
-    constexpr int PK = C * KP / 8 / NT;
-    constexpr int PT = (768 * NS + NT - 1) / NT;
+    constexpr int KB = KP / 32, DW = KP / 64;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char* const Ks = lds;
-    char* const Qs = Ks + NX * TB;
-    char* const Ts = Qs + NX * TB;
-    char* const Ms = Ts + NS * kTri;
-    float* const gs = reinterpret_cast<float*>(Ms + NS * kTri);   // gam, bet, del
+    char* const Qs = Ks + NX * tile_bytes<KP>();
+    const Exchange<NS, CT, KP> Sx{Qs + NX * tile_bytes<KP>()};
+    const Exchange<NX, CT, C> Ox{Sx.base + Sx.kBytes};                                                                 // dO
+    const Exchange<NS, CT, C> Gx{Ox.base + Ox.kBytes}, Ux{Gx.base + Gx.kBytes}, Yx{Ux.base + Ux.kBytes};   // scale gam dO, dU, -beta gam Y
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
     int pair, slice;
     pair_of(blockIdx.x, p.batch * p.heads, slices, pair, slice);
     const int b = pair / p.heads, h = pair % p.heads, hk = h / (p.heads / p.heads_k);
     const int len = length_of(p, b), nc = (len + C - 1) / C;
-    const int col0 = (slice * NW + w) * CT * 16;
-    const bool active = col0 < l.vpad;
+    const int col0 = slice * CT * 16;
     const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
     const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
     const T* const dob = static_cast<const T*>(a.q.dout) + (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride;
@@ -55,207 +53,194 @@ __global__ __launch_bounds__(NW * 64, 1) void gd_bwd_scan_kernel(const BwdArgs a
     char* const wb = static_cast<char*>(a.q.workspace);
     const int64_t slot0 = (int64_t)pair * l.chunks;
 
-    Raw8<T> kr[PK], qr[PK];
-    bf16x8 tr[PT];
-    float gr = 0.f;
-    T vr[CT][4][4];
-    auto fetch = [&](int c) __attribute__((always_inline)) {
+    Raw8<T> kr[KB], qr[KB];   // token 16 w + n
+    Frag<NS> tf[2], mf[2];    // columns 16 w + n of T, M (row blocks 0, 1; tiles 2 and 3 have no block 0)
+    T vr[CT][4], vn[CT][4];   // dO at tokens 16 w + 4 q4 + r, column n: this chunk's, the next one's
+    f32x4 ga, be, de;
+    float glast;
+    auto fetch_qk = [&](int c) __attribute__((always_inline)) {
+        const int at = c * C + 16 * w + n;
+        const int64_t t = at < len ? token(at, len, p.reverse) : 0;
 #pragma unroll
-        for (int i = 0; i < PK; ++i) {
-            const int id = tid + i * NT, row = id / (KP / 8), cc = 8 * (id % (KP / 8)), at = c * C + row;
-            const bool ok = at < len;
-            const int64_t t = ok ? token(at, len, p.reverse) : 0;
-            kr[i] = load_raw8<T>(kb_ + t * p.k_seq_stride, cc, p.dk, ok);
-            qr[i] = load_raw8<T>(qb + t * p.q_seq_stride, cc, p.dk, ok);
-        }
-        const bf16x8* const t8 = reinterpret_cast<const bf16x8*>(ws + l.tri + (slot0 + c) * l.tri_slot);
-#pragma unroll
-        for (int i = 0; i < PT; ++i)
-            if (tid + i * NT < 768 * NS) tr[i] = t8[tid + i * NT];
-        const float* const g = reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c);
-        if (tid < 3 * C) gr = g[tid];
-        if (active) {
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = c * C + 16 * rt + 4 * q4 + r;
-                    const bool ok = at < len;
-                    const T* const row = dob + (ok ? (int64_t)token(at, len, p.reverse) * a.q.dout_seq_stride : 0);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) vr[j][rt][r] = ok && col0 + 16 * j + n < p.dv ? row[col0 + 16 * j + n] : static_cast<T>(0.f);
-                }
+        for (int kb = 0; kb < KB; ++kb) {
+            kr[kb] = load_raw8<WHOLE, T>(kb_ + t * p.k_seq_stride, 32 * kb + 8 * q4, p.dk);
+            qr[kb] = load_raw8<WHOLE, T>(qb + t * p.q_seq_stride, 32 * kb + 8 * q4, p.dk);
         }
     };
-    auto stage = [&]() __attribute__((always_inline)) {
+    auto fetch_do = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PK; ++i) {
-            const int id = tid + i * NT, row = id / (KP / 8), cc = 8 * (id % (KP / 8));
-            tile_put<KP, NX>(Ks, row, cc, planes_of<T>(kr[i]));
-            tile_put<KP, NX>(Qs, row, cc, planes_of<T>(qr[i]));
+        for (int r = 0; r < 4; ++r) {
+            const int at = c * C + 16 * w + 4 * q4 + r;
+            const T* const row = dob + (at < len ? (int64_t)token(at, len, p.reverse) * a.q.dout_seq_stride : 0);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) vn[j][r] = row[col0 + 16 * j + n < p.dv ? col0 + 16 * j + n : 0];
         }
+    };
+    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // first: 2 NS T, 3 NS M (their transposes)
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;
+        f[0] = tri_cols<NS>(at, w, w >= 2 ? 1 : 0, lane);
+        f[1] = tri_cols<NS>(at, w, 1, lane);
+    };
+    auto fetch_gates = [&](int c) __attribute__((always_inline)) {
+        const Gates* const g = reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c;
+        ga = *reinterpret_cast<const f32x4*>(&g->gam[16 * w + 4 * q4]);
+        be = *reinterpret_cast<const f32x4*>(&g->bet[16 * w + 4 * q4]);
+        de = *reinterpret_cast<const f32x4*>(&g->del[16 * w + 4 * q4]);
+        glast = g->gam[C - 1];
+    };
+    auto out_grad = [&](int c, int j, int r, const T (&v)[CT][4]) __attribute__((always_inline)) {
+        return c * C + 16 * w + 4 * q4 + r < len && col0 + 16 * j + n < p.dv ? static_cast<float>(v[j][r]) : 0.f;
+    };
+    auto hand_do = [&](int c) __attribute__((always_inline)) {   // vn -> Ox
 #pragma unroll
-        for (int i = 0; i < PT; ++i)
-            if (tid + i * NT < 768 * NS) reinterpret_cast<bf16x8*>(Ts)[tid + i * NT] = tr[i];
-        if (tid < 3 * C) gs[tid] = gr;
+        for (int j = 0; j < CT; ++j) {
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = out_grad(c, j, r, vn);
+            Ox.put(j, n, paired(w, q4), x);
+        }
     };
 
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 dS[DT][CT];
+    f32x4 dS[DW][CT];
     const int64_t sbase = (int64_t)pair * p.dk * p.dv;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DW; ++d)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
+                dS[d][j][r] = a.q.dfinal_state && row < p.dk && col < p.dv ? a.q.dfinal_state[sbase + (int64_t)row * p.dv + col] : 0.f;
+            }
+            Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
+        }
+    if (nc > 0) {
+        fetch_do(nc - 1);
+        fetch_qk(nc - 1);
+        fetch_tri(nc - 1, 2 * NS, tf);
+        fetch_tri(nc - 1, 3 * NS, mf);
+        fetch_gates(nc - 1);
+        hand_do(nc - 1);
+    }
+    for (int c = nc - 1; c >= 0; --c) {
+        const int next = c > 0 ? c - 1 : 0;   // the first chunk again rather than a branch
+        const int64_t slot = slot0 + c;
+        const bool ok_n = c * C + 16 * w + n < len;
 #pragma unroll
         for (int j = 0; j < CT; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * d + 4 * q4 + r, col = col0 + 16 * j + n;
-                dS[d][j][r] = a.q.dfinal_state && row < p.dk && col < p.dv ? a.q.dfinal_state[sbase + (int64_t)row * p.dv + col] : 0.f;
-            }
-    if (nc > 0) {
-        fetch(nc - 1);
-        stage();
-    }
-    for (int c = nc - 1; c >= 0; --c) {
+            for (int r = 0; r < 4; ++r) vr[j][r] = vn[j][r];
+        fetch_do(next);
+        __syncthreads();   // dS and dO are there; the tiles of K and Q are no longer read
+        // ---- dU = del K dS1 + M^T dO
+        f32x4 dU[CT];
+#pragma unroll
+        for (int j = 0; j < CT; ++j) dU[j] = zero;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const Frag<NX> kf = planes_of<T>(clear<WHOLE, T>(kr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
+            const Frag<NX> qf = planes_of<T>(clear<WHOLE, T>(qr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
+            tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
+            tile_put<KP, NX>(Qs, 16 * w + n, 32 * kb + 8 * q4, qf);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) mma<NS>(dU[j], kf, Sx.get(j, n, 32 * kb + 8 * q4));
+        }
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            dU[j] *= de;
+            mma<NS>(dU[j], mf[1], Ox.get(j, n, 32 + 8 * q4));
+        }
+        if (w < 2)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) mma<NS>(dU[j], mf[0], Ox.get(j, n, 8 * q4));
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            Ux.put(j, n, paired(w, q4), dU[j]);
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = p.scale * ga[r] * out_grad(c, j, r, vr);
+            Gx.put(j, n, paired(w, q4), x);
+        }
+        fetch_qk(next);
+        fetch_tri(next, 3 * NS, mf);
+#pragma unroll
+        for (int d = 0; d < DW; ++d)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) store_rows<NO>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0 + 16 * j, dS[d][j], n, q4);
         __syncthreads();
-        f32x4 D[4][CT];   // dO
+        // ---- Y = T^T dU, dV = beta Y
+        f32x4 Y[CT];
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt)
+        for (int j = 0; j < CT; ++j) {
+            Y[j] = zero;
+            mma<NS>(Y[j], tf[1], Ux.get(j, n, 32 + 8 * q4));
+        }
+        if (w < 2)
 #pragma unroll
-            for (int j = 0; j < CT; ++j)
+            for (int j = 0; j < CT; ++j) mma<NS>(Y[j], tf[0], Ux.get(j, n, 8 * q4));
+        f32x4 V[CT];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) D[rt][j][r] = static_cast<float>(vr[j][rt][r]);
-        if (c > 0) fetch(c - 1);
-        if (active) {
-            const int64_t slot = slot0 + c;
-            f32x4 dU[4][CT], Y[4][CT];
+        for (int j = 0; j < CT; ++j) {
+            V[j] = be * Y[j];
+            f32x4 x;
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
+            for (int r = 0; r < 4; ++r) x[r] = -ga[r] * V[j][r];
+            Yx.put(j, n, paired(w, q4), x);
+        }
+        const float gl = glast;
+        fetch_tri(next, 2 * NS, tf);
+        fetch_gates(next);
+        __syncthreads();
+        // ---- dS0 = gam dS1 + Q^T (scale gam dO) - K^T (beta gam Y)
 #pragma unroll
-                for (int j = 0; j < CT; ++j) { dU[rt][j] = zero; Y[rt][j] = zero; }
+        for (int d = 0; d < DW; ++d)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                Frag<NS> sf[CT];
+            for (int j = 0; j < CT; ++j) dS[d][j] *= gl;
 #pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    sf[j] = frag_of<NS>(dS[2 * kb][j], dS[2 * kb + 1][j]);
-                    if (col0 + 16 * j < l.vpad)
+        for (int tb = 0; tb < 2; ++tb) {
+            Frag<NS> gf[CT], yf[CT];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
+            for (int j = 0; j < CT; ++j) { gf[j] = Gx.get(j, n, 32 * tb + 8 * q4); yf[j] = Yx.get(j, n, 32 * tb + 8 * q4); }
 #pragma unroll
-                            for (int i = 0; i < NO; ++i) {
-                                const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf[j].p[i], unit_frag(half, n, q4), zero, 0, 0, 0);
-                                store_planes4(wb + l.dS + slot * l.s_slot + 2 * (((int64_t)i * KP + 32 * kb + 16 * half + n) * l.vpad + col0 + 16 * j + 4 * q4), x);
-                            }
-                }
-#pragma unroll
-                for (int rt = 0; rt < 4; ++rt) {
-                    const Frag<NX> kf = tile_rows<KP, NX>(Ks, rt, kb, n, q4);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) mma<NS>(dU[rt][j], kf, sf[j]);
-                }
-            }
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
-                const f32x4 de = *reinterpret_cast<const f32x4*>(&gs[2 * C + 16 * rt + 4 * q4]);
-#pragma unroll
-                for (int j = 0; j < CT; ++j) dU[rt][j] *= de;
-            }
-#pragma unroll
-            for (int ib = 0; ib < 2; ++ib) {
-                Frag<NX> df[CT];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) df[j] = frag_of<NX>(D[2 * ib][j], D[2 * ib + 1][j]);
-#pragma unroll
-                for (int ct = 0; ct < 2 * ib + 2; ++ct) {
-                    const Frag<NS> mf = tri_cols<NS>(Ms, ct, ib, n, q4);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) mma<NS>(dU[ct][j], mf, df[j]);
-                }
-            }
-#pragma unroll
-            for (int ib = 0; ib < 2; ++ib) {
-                Frag<NS> uf[CT];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) uf[j] = frag_of<NS>(dU[2 * ib][j], dU[2 * ib + 1][j]);
-#pragma unroll
-                for (int ct = 0; ct < 2 * ib + 2; ++ct) {
-                    const Frag<NS> tf = tri_cols<NS>(Ts, ct, ib, n, q4);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) mma<NS>(Y[ct][j], tf, uf[j]);
-                }
-            }
-            const float glast = gs[C - 1];
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int j = 0; j < CT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) dS[d][j][r] *= glast;
-#pragma unroll
-            for (int ib = 0; ib < 2; ++ib) {
-                const f32x4 g0 = *reinterpret_cast<const f32x4*>(&gs[32 * ib + 4 * q4]), g1 = *reinterpret_cast<const f32x4*>(&gs[32 * ib + 16 + 4 * q4]);
-                const f32x4 b0 = *reinterpret_cast<const f32x4*>(&gs[C + 32 * ib + 4 * q4]), b1 = *reinterpret_cast<const f32x4*>(&gs[C + 32 * ib + 16 + 4 * q4]);
-                Frag<NS> qf[CT], yf[CT];
+            for (int d = 0; d < DW; ++d) {
+                const Frag<NX> qc = tile_cols<KP, NX>(Qs, DW * w + d, tb, n, q4), kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
 #pragma unroll
                 for (int j = 0; j < CT; ++j) {
-                    f32x4 x0, x1, y0, y1;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        x0[r] = p.scale * g0[r] * D[2 * ib][j][r];
-                        x1[r] = p.scale * g1[r] * D[2 * ib + 1][j][r];
-                        y0[r] = b0[r] * Y[2 * ib][j][r];
-                        y1[r] = b1[r] * Y[2 * ib + 1][j][r];
-                    }
-                    qf[j] = frag_of<NS>(x0, x1);
-                    if (col0 + 16 * j < l.vpad) {   // Y for gd_grad, dV = beta Y
-                        const Frag<NO> yo = frag_of<NO>(Y[2 * ib][j], Y[2 * ib + 1][j]), vo = frag_of<NO>(y0, y1);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const bf16x8 one = unit_frag(half, n, q4);
-                            f32x4 dv = zero;
-#pragma unroll
-                            for (int i = NO - 1; i >= 0; --i) {
-                                const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yo.p[i], one, zero, 0, 0, 0);
-                                store_planes4(wb + l.Y + slot * l.u_slot + 2 * (((int64_t)i * C + 32 * ib + 16 * half + n) * l.vpad + col0 + 16 * j + 4 * q4), x);
-                                dv = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo.p[i], one, dv, 0, 0, 0);
-                            }
-                            const int at = c * C + 32 * ib + 16 * half + n;
-                            if (at < len) store4<T>(dvb + (int64_t)token(at, len, p.reverse) * dv_seq, col0 + 16 * j + 4 * q4, p.dv, dv);
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) { y0[r] *= -g0[r]; y1[r] *= -g1[r]; }
-                    yf[j] = frag_of<NS>(y0, y1);
-                }
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const Frag<NX> qc = tile_cols<KP, NX>(Qs, d, ib, n, q4), kc = tile_cols<KP, NX>(Ks, d, ib, n, q4);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) {
-                        mma<NS>(dS[d][j], qc, qf[j]);
-                        mma<NS>(dS[d][j], kc, yf[j]);
-                    }
+                    mma<NS>(dS[d][j], qc, gf[j]);
+                    mma<NS>(dS[d][j], kc, yf[j]);
                 }
             }
         }
-        __syncthreads();
-        if (c > 0) stage();
-    }
-    if (active && a.q.dinitial_state) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DW; ++d)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
+        hand_do(next);
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            store_rows<NO>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0 + 16 * j, Y[j], n, q4);
+            const Frag<NO> f = frag_of<NO>(V[j], zero);
+            f32x4 dv = zero;
+#pragma unroll
+            for (int i = NO - 1; i >= 0; --i) dv = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv, 0, 0, 0);
+            if (ok_n) store4<T>(dvb + (int64_t)token(c * C + 16 * w + n, len, p.reverse) * dv_seq, col0 + 16 * j + 4 * q4, p.dv, dv);
+        }
+    }
+    if (a.q.dinitial_state) {
+#pragma unroll
+        for (int d = 0; d < DW; ++d)
 #pragma unroll
             for (int j = 0; j < CT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * d + 4 * q4 + r, col = col0 + 16 * j + n;
+                    const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
                     if (row < p.dk && col < p.dv) a.q.dinitial_state[sbase + (int64_t)row * p.dv + col] = dS[d][j][r];
                 }
     }
-    const int c0 = slice * NW * CT * 16, cn = (p.dv - c0) < NW * CT * 16 ? (p.dv - c0) : NW * CT * 16;
-    for (int t = len + w; t < p.seqlen; t += NW)
-        for (int cc = lane; cc < cn; cc += 64) dvb[(int64_t)t * dv_seq + c0 + cc] = static_cast<T>(0.f);
+    const int cn = p.dv - col0 < CT * 16 ? p.dv - col0 : CT * 16;
+    for (int t = len + w; t < p.seqlen; t += 4)
+        for (int cc = lane; cc < cn; cc += 64) dvb[(int64_t)t * dv_seq + col0 + cc] = static_cast<T>(0.f);
 }
 
 // ---- dq, dk, dg, dbeta of one chunk --------------------------------------------------------------------------
@@ -270,7 +255,7 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
 }
 __device__ __forceinline__ float L_of(double d) { return fast_exp2((float)(d * 1.4426950408889634)); }
 
-template <typename T, int KP>
+template <typename T, int KP, bool WHOLE>   // WHOLE: dk % 8 == 0 and dv % 8 == 0
 __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO, DT = KP / 16, TB = tile_bytes<KP>();
     constexpr int PK = C * KP / 8 / 256;
@@ -315,8 +300,8 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
         const int id = tid + i * 256, row = id / (KP / 8), cc = 8 * (id % (KP / 8)), at = c * C + row;
         const bool ok = at < len;
         const int64_t t = ok ? token(at, len, p.reverse) : 0;
-        tile_put<KP, NX>(Ks, row, cc, planes_of<T>(load_raw8<T>(kb_ + t * p.k_seq_stride, cc, p.dk, ok)));
-        tile_put<KP, NX>(Qs, row, cc, planes_of<T>(load_raw8<T>(qb + t * p.q_seq_stride, cc, p.dk, ok)));
+        tile_put<KP, NX>(Ks, row, cc, planes_of<T>(clear<WHOLE, T>(load_raw8<WHOLE, T>(kb_ + t * p.k_seq_stride, cc, p.dk), cc, p.dk, ok)));
+        tile_put<KP, NX>(Qs, row, cc, planes_of<T>(clear<WHOLE, T>(load_raw8<WHOLE, T>(qb + t * p.q_seq_stride, cc, p.dk), cc, p.dk, ok)));
     }
     const char* const ws = static_cast<const char*>(p.workspace);
     const char* const wb = static_cast<const char*>(a.q.workspace);
@@ -351,7 +336,8 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
         auto out_rows = [&](int tok, int vblk) __attribute__((always_inline)) {
             const int at = c * C + tok;
             const bool ok = at < len;
-            return planes_of<T>(load_raw8<T>(dob + (ok ? (int64_t)token(at, len, p.reverse) * a.q.dout_seq_stride : 0), 32 * vblk + 8 * q4, p.dv, ok));
+            const int cc = 32 * vblk + 8 * q4;
+            return planes_of<T>(clear<WHOLE, T>(load_raw8<WHOLE, T>(dob + (ok ? (int64_t)token(at, len, p.reverse) * a.q.dout_seq_stride : 0), cc, p.dv), cc, p.dv, ok));
         };
         // [j][i]: rows = another tile's tokens, columns (lanes) = this wave's tokens
         f32x4 dm[4], zl[4];   // this wave's tokens as i, tiles j <= w: dO_i.U_j, Y_i.U_j
@@ -366,7 +352,8 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
             const Frag<NO> yi = planes(Yw, C, own, vk), ui = planes(Uw, C, own, vk);
             const Frag<NX> oi = out_rows(own, vk);
             {
-                const Raw8<T> v = load_raw8<T>(vb + (ok_own ? (int64_t)token(at_own, len, p.reverse) * p.v_seq_stride : 0), 32 * vk + 8 * q4, p.dv, ok_own);
+                const int cc = 32 * vk + 8 * q4;
+                const Raw8<T> v = clear<WHOLE, T>(load_raw8<WHOLE, T>(vb + (ok_own ? (int64_t)token(at_own, len, p.reverse) * p.v_seq_stride : 0), cc, p.dv), cc, p.dv, ok_own);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float y = 0.f;
@@ -415,7 +402,7 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
                 f32x4 v = zero;
 #pragma unroll
                 for (int i = NX - 1; i >= 0; --i) {
-                    const bf16x4 t4 = *reinterpret_cast<const bf16x4*>(tile + i * TB + own * tile_row<KP>() + 2 * (32 * (d >> 1) + 8 * q4 + 4 * (d & 1)));
+                    const bf16x4 t4 = *reinterpret_cast<const bf16x4*>(tile + i * TB + own * tile_row<KP>() + 2 * (16 * d + 4 * q4));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += static_cast<float>(t4[e]);
                 }
@@ -510,33 +497,33 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
-static int allow_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
-    if (bytes <= 65536) return VMS_OK;
-    const hipError_t e = once.run([&] { return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
-    if (e != hipSuccess) { set_error("hipFuncSetAttribute: %s", hipGetErrorString(e)); return VMS_ERR_LAUNCH; }
-    return VMS_OK;
-}
-template <typename T, int KP, int NW, int CT>
+template <typename T, int KP, int CT, bool WHOLE>
 static int bwd_scan_launch(const BwdArgs& a, hipStream_t s) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int lds = 2 * NX * tile_bytes<KP>() + 2 * NS * kTri + 3 * C * 4;
-    static_assert(NW * 64 >= 3 * C && lds <= 163840, "a thread per gate; 160 KB of LDS");
+    constexpr int lds = 2 * NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + Exchange<NX, CT, C>::kBytes + 3 * Exchange<NS, CT, C>::kBytes;
+    static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, KP, NW, CT>), lds)) return rc;
-    const int slices = (a.l.vpad + NW * CT * 16 - 1) / (NW * CT * 16);
-    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, NW, CT>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(NW * 64), lds, s, a, slices);
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, KP, CT, WHOLE>), lds)) return rc;
+    const int slices = (a.l.vpad + CT * 16 - 1) / (CT * 16);
+    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, CT, WHOLE>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(256), lds, s, a, slices);
+    VMS_LAUNCH_CHECK();
+    return VMS_OK;
+}
+template <typename T, int KP, bool WHOLE>
+static int grad_launch(const BwdArgs& a, hipStream_t s) {
+    constexpr int lds = 2 * Prec<T>::NX * tile_bytes<KP>() + (int)sizeof(Gates) + (C + 4) * 4;
+    static PerDeviceOnce once;
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_grad_kernel<T, KP, WHOLE>), lds)) return rc;
+    hipLaunchKernelGGL((gd_grad_kernel<T, KP, WHOLE>), dim3(a.l.chunks, a.q.f.heads_k, a.q.f.batch), dim3(256), lds, s, a);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
 template <typename T, int KP>
 static int bwd_launch(const BwdArgs& a, hipStream_t s) {
-    if (int rc = bwd_scan_launch<T, KP, 4, 1>(a, s)) return rc;
-    constexpr int lds = 2 * Prec<T>::NX * tile_bytes<KP>() + (int)sizeof(Gates) + (C + 4) * 4;
-    static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_grad_kernel<T, KP>), lds)) return rc;
-    hipLaunchKernelGGL((gd_grad_kernel<T, KP>), dim3(a.l.chunks, a.q.f.heads_k, a.q.f.batch), dim3(256), lds, s, a);
-    VMS_LAUNCH_CHECK();
-    return VMS_OK;
+    constexpr int kCT = sizeof(T) == 4 ? 1 : 2;   // column tiles of a workgroup: fp32's six planes of K and Q leave LDS for one
+    const bool whole = a.q.f.dk % 8 == 0;
+    if (int rc = whole ? bwd_scan_launch<T, KP, kCT, true>(a, s) : bwd_scan_launch<T, KP, kCT, false>(a, s)) return rc;
+    return whole && a.q.f.dv % 8 == 0 ? grad_launch<T, KP, true>(a, s) : grad_launch<T, KP, false>(a, s);
 }
 template <typename T>
 static int bwd_type(const BwdArgs& a, hipStream_t s) {

@@ -1,9 +1,9 @@
 // gated_delta_fwd.hip -- gated delta rule, forward (vms_gated_delta_fwd): the algebra and the layouts are in gated_delta.h.
 //
 //   gd_prep   one wave per (chunk, head): the gates, T (triangular inverse in fp32), M.
-//   gd_scan   the walk over the chunks.  The columns of S (and of V, U, O) never meet: a wave owns 16 CT of them for the whole
-//             sequence, S in its accumulators, and shares only the operands K, Q, T, M of a chunk with the other waves of its
-//             workgroup through LDS.
+//   gd_scan   the walk over the chunks.  The columns of S (and of V, U, O) never meet: a workgroup owns 16 CT of them for the whole
+//             sequence.  Its four waves split the chunk's 64 tokens and S's dk rows: wave w computes token tile w of K S0, U and O
+//             and dk / 4 rows of S, which stay in its accumulators.
 #include "gated_delta.h"
 
 namespace vms {
@@ -18,7 +18,7 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __bui
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
-template <typename T, int KP>
+template <typename T, int KP, bool WHOLE>   // WHOLE: dk % 8 == 0
 __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_params p, const Layout l) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
     constexpr int AR = 68;   // row pitch of As, floats
@@ -61,26 +61,48 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 
     const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
     const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
-    auto rows = [&](const T* base, int64_t stride, int rt, int kb) {
+    auto rows = [&](const T* base, int64_t stride, int rt, int kb) __attribute__((always_inline)) {
         const int i = c * C + 16 * rt + n;
         const bool ok = i < len;
-        return planes_of<T>(load_raw8<T>(base + (ok ? (int64_t)token(i, len, p.reverse) * stride : 0), 32 * kb + 8 * q4, p.dk, ok));
+        const T* const row = base + (ok ? (int64_t)token(i, len, p.reverse) * stride : 0);
+        return load_raw8<WHOLE, T>(row, 32 * kb + 8 * q4, p.dk);
     };
+    auto as_frag = [&](const Raw8<T>& r, int rt, int kb) __attribute__((always_inline)) {
+        return planes_of<T>(clear<WHOLE, T>(r, 32 * kb + 8 * q4, p.dk, c * C + 16 * rt + n < len));
+    };
+    Raw8<T> kraw[4][KP / 32];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+        for (int kb = 0; kb < KP / 32; ++kb) kraw[rt][kb] = rows(kb_, p.k_seq_stride, rt, kb);
     char* const tw = ws + l.tri + slot * l.tri_slot;
     char* const mw = tw + NS * kTri;
+    char* const ttw = mw + NS * kTri;   // transposes (for_backward)
+    char* const mtw = ttw + NS * kTri;
+    auto put4 = [&](char* at, const f32x4& v) __attribute__((always_inline)) {   // half an operand, NS planes
+        float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+        Frag<NS> f;
+        split<NS>(x, f);
+#pragma unroll
+        for (int i2 = 0; i2 < NS; ++i2) *reinterpret_cast<bf16x4*>(at + i2 * kTri) = __builtin_shufflevector(f.p[i2], f.p[i2], 0, 1, 2, 3);
+    };
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
-        f32x4 kk[4], qk[4];
+        f32x4 kk[4], qk[4], kq[4];   // kq: Q K^T once more, lanes along j: the transpose of M
 #pragma unroll
-        for (int ct = 0; ct < 4; ++ct) { kk[ct] = f32x4{0.f, 0.f, 0.f, 0.f}; qk[ct] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+        for (int ct = 0; ct < 4; ++ct) { kk[ct] = f32x4{0.f, 0.f, 0.f, 0.f}; qk[ct] = kk[ct]; kq[ct] = kk[ct]; }
+        Raw8<T> qraw[KP / 32];
+#pragma unroll
+        for (int kb = 0; kb < KP / 32; ++kb) qraw[kb] = rows(qb, p.q_seq_stride, rt, kb);
 #pragma unroll
         for (int kb = 0; kb < KP / 32; ++kb) {
-            const Frag<NX> qi = rows(qb, p.q_seq_stride, rt, kb), ki = rows(kb_, p.k_seq_stride, rt, kb);
+            const Frag<NX> qi = as_frag(qraw[kb], rt, kb), ki = as_frag(kraw[rt][kb], rt, kb);
 #pragma unroll
             for (int ct = 0; ct <= rt; ++ct) {   // [j][i]: lane i, 4 consecutive j
-                const Frag<NX> kj = ct == rt ? ki : rows(kb_, p.k_seq_stride, ct, kb);
+                const Frag<NX> kj = ct == rt ? ki : as_frag(kraw[ct][kb], ct, kb);
                 mma<NS>(kk[ct], kj, ki);
                 mma<NS>(qk[ct], kj, qi);
+                if (p.for_backward) mma<NS>(kq[ct], qi, kj);
             }
         }
         const int i = 16 * rt + n;
@@ -97,7 +119,17 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
                 qk[ct][r] = j <= i ? p.scale * L * qk[ct][r] : 0.f;
             }
             *reinterpret_cast<f32x4*>(&As[i * AR + 16 * ct + 4 * q4]) = a;
+            if (p.for_backward) {
+                const int j = 16 * ct + n;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i2 = 16 * rt + 4 * q4 + r;
+                    kq[ct][r] = j <= i2 ? p.scale * fast_exp2((float)((Gs[i2] - Gs[j]) * 1.4426950408889634)) * kq[ct][r] : 0.f;
+                }
+                put4(mtw + 1024 * tri_t(ct, rt >> 1) + 16 * lane + 8 * (rt & 1), kq[ct]);
+            }
         }
+        if (p.for_backward && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
 #pragma unroll
         for (int kb = 0; kb <= rt / 2; ++kb) {
             const Frag<NS> f = frag_of<NS>(qk[2 * kb], qk[2 * kb + 1]);
@@ -186,30 +218,36 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 #pragma unroll
             for (int i2 = 0; i2 < NS; ++i2) *reinterpret_cast<bf16x8*>(tw + i2 * kTri + 1024 * tri(rt, kb) + 16 * lane) = f.p[i2];
         }
+    if (p.for_backward) {
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+            for (int ib = ct / 2; ib < 2; ++ib)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) put4(ttw + 1024 * tri_t(ct, ib) + 16 * lane + 8 * half, 2 * ib + half >= ct ? b_of(2 * ib + half, ct) : zero);
+    }
 }
 
 // ---- the walk over the chunks --------------------------------------------------------------------------------
-template <typename T, int KP, int NW, int CT>
-__global__ __launch_bounds__(NW * 64, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
+// What bounds it is the chain of one chunk (K S0 -> R -> U -> S1), not a rate: a head is 16 .. 64 tokens of work per step on one CU.  A wave with
+// a whole chunk of 16 columns to itself (no exchange, every wave reading all of K, Q, T, M from LDS) took 5.4 us per chunk at dk = 128,
+// four waves on one chunk take 1.5: three barriers, but a quarter of the products in a row and each operand of K, Q, T, M read once, straight
+// from memory into the registers of the one wave that uses it.  K alone also goes through LDS, for its transpose.
+template <typename T, int KP, int CT, bool WHOLE, bool TRAIN>
+__global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
-    constexpr int NT = NW * 64, KB = KP / 32, DT = KP / 16;
-    constexpr int TB = tile_bytes<KP>();
-    constexpr int PK = C * KP / 8 / NT;                       // 8-element pieces of a k / q tile per thread
-    constexpr int PT = (768 * NS + NT - 1) / NT;              // 16-byte pieces of T and M per thread
+    constexpr int KB = KP / 32, DW = KP / 64;   // 32-column blocks of k; 16-row tiles of S per wave
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char* const Ks = lds;
-    char* const Qs = Ks + NX * TB;
-    char* const Ts = Qs + NX * TB;
-    char* const Ms = Ts + NS * kTri;
-    float* const gs = reinterpret_cast<float*>(Ms + NS * kTri);   // gam, bet, del
+    const Exchange<NS, CT, KP> Sx{Ks + NX * tile_bytes<KP>()};
+    const Exchange<NS, CT, C> Rx{Sx.base + Sx.kBytes}, Ux{Rx.base + Rx.kBytes}, Dx{Ux.base + Ux.kBytes};   // R, U, del U
 
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
     int pair, slice;
     pair_of(blockIdx.x, p.batch * p.heads, slices, pair, slice);
     const int b = pair / p.heads, h = pair % p.heads, hk = h / (p.heads / p.heads_k);
     const int len = length_of(p, b), nc = (len + C - 1) / C;
-    const int col0 = (slice * NW + w) * CT * 16;
-    const bool active = col0 < l.vpad;   // uniform in the wave
+    const int col0 = slice * CT * 16;
     const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
     const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
     const T* const vb = static_cast<const T*>(p.v) + (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride;
@@ -217,204 +255,176 @@ __global__ __launch_bounds__(NW * 64, 1) void gd_scan_kernel(const vms_gated_del
     char* const ws = static_cast<char*>(p.workspace);
     const int64_t slot0 = (int64_t)pair * l.chunks;
 
-    Raw8<T> kr[PK], qr[PK];
-    bf16x8 tr[PT];
-    float gr = 0.f;
-    T vr[CT][4][4];
-    auto fetch = [&](int c) __attribute__((always_inline)) {
+    Raw8<T> kr[KB], qr[KB];   // token 16 w + n
+    Frag<NS> tf[2], mf[2];    // rows 16 w + n of T, M (blocks 0, 1; tiles 0 and 1 have no block 1)
+    T vr[CT][4];              // tokens 16 w + 4 q4 + r, column n
+    f32x4 ga, be, de;         // gates of those tokens
+    float gn, glast;          // gam of token 16 w + n, of the last one
+    auto fetch_qkv = [&](int c) __attribute__((always_inline)) {
+        const int at = c * C + 16 * w + n;
+        const int64_t t = at < len ? token(at, len, p.reverse) : 0;
 #pragma unroll
-        for (int i = 0; i < PK; ++i) {
-            const int id = tid + i * NT, row = id / (KP / 8), cc = 8 * (id % (KP / 8)), at = c * C + row;
-            const bool ok = at < len;
-            const int64_t t = ok ? token(at, len, p.reverse) : 0;
-            kr[i] = load_raw8<T>(kb_ + t * p.k_seq_stride, cc, p.dk, ok);
-            qr[i] = load_raw8<T>(qb + t * p.q_seq_stride, cc, p.dk, ok);
+        for (int kb = 0; kb < KB; ++kb) {
+            kr[kb] = load_raw8<WHOLE, T>(kb_ + t * p.k_seq_stride, 32 * kb + 8 * q4, p.dk);
+            qr[kb] = load_raw8<WHOLE, T>(qb + t * p.q_seq_stride, 32 * kb + 8 * q4, p.dk);
         }
-        const bf16x8* const t8 = reinterpret_cast<const bf16x8*>(ws + l.tri + (slot0 + c) * l.tri_slot);
 #pragma unroll
-        for (int i = 0; i < PT; ++i)
-            if (tid + i * NT < 768 * NS) tr[i] = t8[tid + i * NT];
-        const float* const g = reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c);
-        if (tid < 3 * C) gr = g[tid];
-        if (active) {
+        for (int r = 0; r < 4; ++r) {
+            const int at2 = c * C + 16 * w + 4 * q4 + r;
+            const T* const row = vb + (at2 < len ? (int64_t)token(at2, len, p.reverse) * p.v_seq_stride : 0);
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = c * C + 16 * rt + 4 * q4 + r;
-                    const bool ok = at < len;
-                    const T* const row = vb + (ok ? (int64_t)token(at, len, p.reverse) * p.v_seq_stride : 0);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) vr[j][rt][r] = ok && col0 + 16 * j + n < p.dv ? row[col0 + 16 * j + n] : static_cast<T>(0.f);
-                }
+            for (int j = 0; j < CT; ++j) vr[j][r] = row[col0 + 16 * j + n < p.dv ? col0 + 16 * j + n : 0];
         }
     };
-    auto stage = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < PK; ++i) {
-            const int id = tid + i * NT, row = id / (KP / 8), cc = 8 * (id % (KP / 8));
-            tile_put<KP, NX>(Ks, row, cc, planes_of<T>(kr[i]));
-            tile_put<KP, NX>(Qs, row, cc, planes_of<T>(qr[i]));
-        }
-#pragma unroll
-        for (int i = 0; i < PT; ++i)
-            if (tid + i * NT < 768 * NS) reinterpret_cast<bf16x8*>(Ts)[tid + i * NT] = tr[i];
-        if (tid < 3 * C) gs[tid] = gr;
+    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // first: 0 T, NS M
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;
+        f[0] = tri_rows<NS>(at, w, 0, lane);
+        f[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
+    };
+    auto fetch_gates = [&](int c) __attribute__((always_inline)) {
+        const Gates* const g = reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c;
+        ga = *reinterpret_cast<const f32x4*>(&g->gam[16 * w + 4 * q4]);
+        be = *reinterpret_cast<const f32x4*>(&g->bet[16 * w + 4 * q4]);
+        de = *reinterpret_cast<const f32x4*>(&g->del[16 * w + 4 * q4]);
+        gn = g->gam[16 * w + n];
+        glast = g->gam[C - 1];
     };
 
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 S[DT][CT];
+    f32x4 S[DW][CT];   // rows 16 (DW w + d) + 4 q4 + r, column n
     const int64_t sbase = (int64_t)pair * p.dk * p.dv;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DW; ++d)
 #pragma unroll
-        for (int j = 0; j < CT; ++j)
+        for (int j = 0; j < CT; ++j) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * d + 4 * q4 + r, col = col0 + 16 * j + n;
+                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
                 S[d][j][r] = p.initial_state && row < p.dk && col < p.dv ? p.initial_state[sbase + (int64_t)row * p.dv + col] : 0.f;
             }
-
+            Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
+        }
     if (nc > 0) {
-        fetch(0);
-        stage();
+        fetch_qkv(0);
+        fetch_tri(0, 0, tf);
+        fetch_tri(0, NS, mf);
+        fetch_gates(0);
     }
     for (int c = 0; c < nc; ++c) {
-        __syncthreads();
-        f32x4 R[4][CT];   // V of this chunk: its registers are the next chunk's from the fetch on
+        const int next = c + 1 < nc ? c + 1 : c;   // the last chunk again rather than a branch
+        const int64_t slot = slot0 + c;
+        const bool ok_n = c * C + 16 * w + n < len;
+        __syncthreads();   // S is there; K's tile is no longer read
+        // ---- P = K S0, O = S0^T Q^T, R
+        f32x4 P[CT], O[CT];
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt)
+        for (int j = 0; j < CT; ++j) { P[j] = zero; O[j] = zero; }
 #pragma unroll
-            for (int j = 0; j < CT; ++j)
+        for (int kb = 0; kb < KB; ++kb) {
+            const Frag<NX> kf = planes_of<T>(clear<WHOLE, T>(kr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
+            const Frag<NX> qf = planes_of<T>(clear<WHOLE, T>(qr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
+            tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) R[rt][j][r] = static_cast<float>(vr[j][rt][r]);
-        if (c + 1 < nc) fetch(c + 1);
-        if (active) {
-            f32x4 P[4][CT], O[4][CT];
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-                for (int j = 0; j < CT; ++j) { P[rt][j] = zero; O[rt][j] = zero; }
-            const int64_t slot = slot0 + c;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                Frag<NS> sf[CT];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) sf[j] = frag_of<NS>(S[2 * kb][j], S[2 * kb + 1][j]);
-                if (p.for_backward) {   // S0 by rows (dk): 4 consecutive columns per lane
-#pragma unroll
-                    for (int j = 0; j < CT; ++j)
-                        if (col0 + 16 * j < l.vpad)
-#pragma unroll
-                            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                                for (int i = 0; i < NO; ++i) {
-                                    const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf[j].p[i], unit_frag(half, n, q4), zero, 0, 0, 0);
-                                    store_planes4(ws + l.S0 + slot * l.s_slot + 2 * (((int64_t)i * KP + 32 * kb + 16 * half + n) * l.vpad + col0 + 16 * j + 4 * q4), x);
-                                }
-                }
-#pragma unroll
-                for (int rt = 0; rt < 4; ++rt) {
-                    const Frag<NX> kf = tile_rows<KP, NX>(Ks, rt, kb, n, q4), qf = tile_rows<KP, NX>(Qs, rt, kb, n, q4);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) {
-                        mma<NS>(P[rt][j], kf, sf[j]);    // [token][v]
-                        mma<NO>(O[rt][j], sf[j], qf);    // [v][token]: the lanes of a store hold 4 consecutive v
-                    }
-                }
-            }
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
-                const f32x4 ga = *reinterpret_cast<const f32x4*>(&gs[16 * rt + 4 * q4]), be = *reinterpret_cast<const f32x4*>(&gs[C + 16 * rt + 4 * q4]);
-                const float sg = p.scale * gs[16 * rt + n];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) R[rt][j][r] = be[r] * fmaf(-ga[r], P[rt][j][r], R[rt][j][r]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) O[rt][j][r] *= sg;
-                }
-            }
-            f32x4 U[4][CT];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                Frag<NS> rf[CT];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) rf[j] = frag_of<NS>(R[2 * kb][j], R[2 * kb + 1][j]);
-#pragma unroll
-                for (int rt = 2 * kb; rt < 4; ++rt) {
-                    const Frag<NS> tf = tri_rows<NS>(Ts, rt, kb, lane);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) {
-                        if (kb == 0) U[rt][j] = zero;
-                        mma<NS>(U[rt][j], tf, rf[j]);
-                    }
-                }
-            }
-            const float glast = gs[C - 1];
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int j = 0; j < CT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[d][j][r] *= glast;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                Frag<NS> uf[CT];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    const Frag<NS> of = frag_of<NS>(U[2 * kb][j], U[2 * kb + 1][j]);
-#pragma unroll
-                    for (int rt = 2 * kb; rt < 4; ++rt) mma<NS>(O[rt][j], of, tri_rows<NS>(Ms, rt, kb, lane));
-                    if (p.for_backward && col0 + 16 * j < l.vpad) {
-#pragma unroll
-                        for (int half = 0; half < 2; ++half)
-#pragma unroll
-                            for (int i = 0; i < NO; ++i) {
-                                const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(of.p[i], unit_frag(half, n, q4), zero, 0, 0, 0);
-                                store_planes4(ws + l.U + slot * l.u_slot + 2 * (((int64_t)i * C + 32 * kb + 16 * half + n) * l.vpad + col0 + 16 * j + 4 * q4), x);
-                            }
-                    }
-                    f32x4 a = U[2 * kb][j], a2 = U[2 * kb + 1][j];
-                    a *= *reinterpret_cast<const f32x4*>(&gs[2 * C + 32 * kb + 4 * q4]);
-                    a2 *= *reinterpret_cast<const f32x4*>(&gs[2 * C + 32 * kb + 16 + 4 * q4]);
-                    uf[j] = frag_of<NS>(a, a2);
-                }
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const Frag<NX> kf = tile_cols<KP, NX>(Ks, d, kb, n, q4);
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) mma<NS>(S[d][j], kf, uf[j]);
-                }
-            }
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
-                const int at = c * C + 16 * rt + n;
-                if (at < len) {
-                    T* const row = ob + (int64_t)token(at, len, p.reverse) * p.out_seq_stride;
-#pragma unroll
-                    for (int j = 0; j < CT; ++j) store4<T>(row, col0 + 16 * j + 4 * q4, p.dv, O[rt][j]);
-                }
+            for (int j = 0; j < CT; ++j) {
+                const Frag<NS> sf = Sx.get(j, n, 32 * kb + 8 * q4);
+                mma<NS>(P[j], kf, sf);    // [token][v]
+                mma<NO>(O[j], sf, qf);    // [v][token]: the lanes of a store hold 4 consecutive v
             }
         }
-        __syncthreads();
-        if (c + 1 < nc) stage();
-    }
-    if (active && p.final_state) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int j = 0; j < CT; ++j) {
+            f32x4 R;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float v = c * C + 16 * w + 4 * q4 + r < len && col0 + 16 * j + n < p.dv ? static_cast<float>(vr[j][r]) : 0.f;
+                R[r] = be[r] * fmaf(-ga[r], P[j][r], v);
+            }
+            Rx.put(j, n, paired(w, q4), R);
+        }
+        fetch_qkv(next);
+        if constexpr (TRAIN) {   // S0 by rows: 4 consecutive columns per lane
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) store_rows<NO>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0 + 16 * j, S[d][j], n, q4);
+        }
+        __syncthreads();
+        // ---- U = T R
+        f32x4 U[CT];
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            U[j] = zero;
+            mma<NS>(U[j], tf[0], Rx.get(j, n, 8 * q4));
+        }
+        if (w >= 2)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) mma<NS>(U[j], tf[1], Rx.get(j, n, 32 + 8 * q4));
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            f32x4 x = U[j] * de;
+            Dx.put(j, n, paired(w, q4), x);
+            Ux.put(j, n, paired(w, q4), U[j]);
+        }
+        fetch_tri(next, 0, tf);
+        __syncthreads();
+        // ---- S1 = gam S0 + K^T (del U)
+#pragma unroll
+        for (int d = 0; d < DW; ++d)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) S[d][j] *= glast;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            Frag<NS> uf[CT];
+#pragma unroll
+            for (int j = 0; j < CT; ++j) uf[j] = Dx.get(j, n, 32 * tb + 8 * q4);
+#pragma unroll
+            for (int d = 0; d < DW; ++d) {
+                const Frag<NX> kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
+#pragma unroll
+                for (int j = 0; j < CT; ++j) mma<NS>(S[d][j], kc, uf[j]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DW; ++d)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
+        // ---- O += M U
+        const float sg = p.scale * gn;
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            O[j] *= sg;
+            mma<NS>(O[j], Ux.get(j, n, 8 * q4), mf[0]);
+        }
+        if (w >= 2)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) mma<NS>(O[j], Ux.get(j, n, 32 + 8 * q4), mf[1]);
+        if (ok_n) {
+            T* const row = ob + (int64_t)token(c * C + 16 * w + n, len, p.reverse) * p.out_seq_stride;
+#pragma unroll
+            for (int j = 0; j < CT; ++j) store4<T>(row, col0 + 16 * j + 4 * q4, p.dv, O[j]);
+        }
+        if constexpr (TRAIN) {
+#pragma unroll
+            for (int j = 0; j < CT; ++j) store_rows<NO>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, col0 + 16 * j, U[j], n, q4);
+        }
+        fetch_tri(next, NS, mf);
+        fetch_gates(next);
+    }
+    if (p.final_state) {
+#pragma unroll
+        for (int d = 0; d < DW; ++d)
 #pragma unroll
             for (int j = 0; j < CT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * d + 4 * q4 + r, col = col0 + 16 * j + n;
+                    const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
                     if (row < p.dk && col < p.dv) p.final_state[sbase + (int64_t)row * p.dv + col] = S[d][j][r];
                 }
     }
     // padding behind the sequence's end
-    const int c0 = slice * NW * CT * 16, cn = (p.dv - c0) < NW * CT * 16 ? (p.dv - c0) : NW * CT * 16;
-    for (int t = len + w; t < p.seqlen; t += NW)
-        for (int cc = lane; cc < cn; cc += 64) ob[(int64_t)t * p.out_seq_stride + c0 + cc] = static_cast<T>(0.f);
+    const int cn = p.dv - col0 < CT * 16 ? p.dv - col0 : CT * 16;
+    for (int t = len + w; t < p.seqlen; t += 4)
+        for (int cc = lane; cc < cn; cc += 64) ob[(int64_t)t * p.out_seq_stride + col0 + cc] = static_cast<T>(0.f);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -434,29 +444,32 @@ int validate(const vms_gated_delta_params& p) {
     return VMS_OK;
 }
 
-template <typename T, int KP, int NW, int CT>
+template <typename T, int KP, int CT, bool WHOLE, bool TRAIN>
 static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStream_t s) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int lds = 2 * NX * tile_bytes<KP>() + 2 * NS * kTri + 3 * C * 4;
-    static_assert(NW * 64 >= 3 * C, "a thread per gate");
+    constexpr int lds = NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + 3 * Exchange<NS, CT, C>::kBytes;
+    static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;
-    if (lds > 65536) {
-        const hipError_t e = once.run([&] {
-            return hipFuncSetAttribute(reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, NW, CT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        });
-        if (e != hipSuccess) { set_error("hipFuncSetAttribute: %s", hipGetErrorString(e)); return VMS_ERR_LAUNCH; }
-    }
-    const int slices = (l.vpad + NW * CT * 16 - 1) / (NW * CT * 16);
-    hipLaunchKernelGGL((gd_scan_kernel<T, KP, NW, CT>), dim3(p.batch * p.heads * slices), dim3(NW * 64), lds, s, p, l, slices);
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, CT, WHOLE, TRAIN>), lds)) return rc;
+    const int slices = (l.vpad + CT * 16 - 1) / (CT * 16);
+    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, WHOLE, TRAIN>), dim3(p.batch * p.heads * slices), dim3(256), lds, s, p, l, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
+#ifndef VMS_GD_CT
+#define VMS_GD_CT 2
+#endif
+constexpr int kCT = VMS_GD_CT;
 template <typename T, int KP>
 static int fwd_launch(const vms_gated_delta_params& p, hipStream_t s) {
     const Layout l = layout(p);
-    hipLaunchKernelGGL((gd_prep_kernel<T, KP>), dim3(l.chunks, p.heads, p.batch), dim3(64), 0, s, p, l);
+    const dim3 grid(l.chunks, p.heads, p.batch);
+    const bool whole = p.dk % 8 == 0;
+    if (whole) hipLaunchKernelGGL((gd_prep_kernel<T, KP, true>), grid, dim3(64), 0, s, p, l);
+    else hipLaunchKernelGGL((gd_prep_kernel<T, KP, false>), grid, dim3(64), 0, s, p, l);
     VMS_LAUNCH_CHECK();
-    return scan_launch<T, KP, 4, 1>(p, l, s);
+    if (p.for_backward) return whole ? scan_launch<T, KP, kCT, true, true>(p, l, s) : scan_launch<T, KP, kCT, false, true>(p, l, s);
+    return whole ? scan_launch<T, KP, kCT, true, false>(p, l, s) : scan_launch<T, KP, kCT, false, false>(p, l, s);
 }
 template <typename T>
 static int fwd_type(const vms_gated_delta_params& p, hipStream_t s) {
