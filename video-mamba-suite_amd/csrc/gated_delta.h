@@ -49,16 +49,27 @@ __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB
             if (i < NA && s - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], acc, 0, 0, 0);
 }
 
-// x -> N bf16 planes whose sum is x up to 2^-(8 N + 1) (round to nearest each)
+// x0, x1 -> their bf16 values (round to nearest) in one register; what is left of them
+__device__ __forceinline__ unsigned take_bf16(float& x0, float& x1, bool last) {
+    using bf16x2 = vec_t<bf16_t, 2>;
+    const bf16x2 h = {static_cast<bf16_t>(x0), static_cast<bf16_t>(x1)};
+    const unsigned u = __builtin_bit_cast(unsigned, h);
+    if (!last) {
+        x0 -= __builtin_bit_cast(float, u << 16);
+        x1 -= __builtin_bit_cast(float, u & 0xffff0000u);
+    }
+    return u;
+}
+// x -> N bf16 planes whose sum is x up to 2^-(8 N + 1)
 template <int N>
 __device__ __forceinline__ void split(float (&x)[8], Frag<N>& f) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) {
+        vec_t<unsigned, 4> u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            f.p[i][e] = static_cast<bf16_t>(x[e]);
-            if (i + 1 < N) x[e] -= static_cast<float>(f.p[i][e]);
-        }
+        for (int e = 0; e < 4; ++e) u[e] = take_bf16(x[2 * e], x[2 * e + 1], i + 1 == N);
+        f.p[i] = __builtin_bit_cast(bf16x8, u);
+    }
 }
 template <int N>
 __device__ __forceinline__ Frag<N> frag_of(const f32x4& a, const f32x4& b) {   // two 16-row tiles, paired order
@@ -67,6 +78,11 @@ __device__ __forceinline__ Frag<N> frag_of(const f32x4& a, const f32x4& b) {   /
     split<N>(x, f);
     return f;
 }
+
+__device__ __forceinline__ bf16x4 read_tr(const char* at) {   // 4 x 16 elements transposed among 16 lanes
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at));
+}
+__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // 8 elements of a row as they stand in memory: columns c .. c+7 of a row of n, any alignment.  WHOLE: n % 8 == 0, one 16- or 32-byte load;
 // otherwise element by element.  Never a branch: what lies outside is read from a place that exists and becomes zero in clear(), when it is
@@ -98,6 +114,87 @@ __device__ __forceinline__ Raw8<T> clear(Raw8<T> r, int c, int n, bool ok) {   /
     }
     return r;
 }
+// The rows of q and k in the order of the walk.  FIT says how dk meets the tile: 0 any, 1 dk % 8 == 0, 2 dk == KP (nothing to clear).  Rows behind the end
+// are the last row again: beta = 0 and the triangles keep them out of everything (gd_prep, the walks).
+template <typename T>
+struct Rows {
+    const T* first;   // token 0 of the walk
+    int step;         // elements to the next one (strides of 2^31 and more are refused)
+    __device__ __forceinline__ Rows(const void* base, int64_t batch_head, int64_t seq_stride, int len, int reverse) {
+        first = static_cast<const T*>(base) + batch_head + (reverse && len > 0 ? (int64_t)(len - 1) * seq_stride : 0);
+        step = reverse ? -(int)seq_stride : (int)seq_stride;
+    }
+    __device__ __forceinline__ const T* row(int i) const { return first + (int64_t)i * step; }
+};
+template <int FIT, typename T>
+__device__ __forceinline__ Raw8<T> fit_load(const T* row, int c, int n) {
+    if constexpr (FIT == 2) {
+        Raw8<T> r;
+        __builtin_memcpy(&r, row + c, sizeof(r));
+        return r;
+    } else {
+        return load_raw8<FIT == 1, T>(row, c, n);
+    }
+}
+template <int FIT, typename T>
+__device__ __forceinline__ Raw8<T> fit_clear(const Raw8<T>& r, int c, int n) {
+    if constexpr (FIT == 2) return r;
+    else return clear<FIT == 1, T>(r, c, n, true);
+}
+inline int fit_of(int dk, int dv) { return dv % 8 || dk % 8 ? 0 : dk == 64 || dk == 128 ? 2 : 1; }
+
+// Columns of a walk's CT tiles: lane n of tile j has column 4 CT (n / 4) + 4 j + n % 4, so that the 4 CT columns a lane holds of a transposed product
+// (rows 4 p + r of the CT tiles) stand side by side in memory: one store of 16 bytes instead of two of 8.
+template <int CT> __device__ __forceinline__ int col_of(int j, int n) { return 4 * CT * (n >> 2) + 4 * j + (n & 3); }
+
+// A wave's 16 tokens x 16 CT columns of v (or of out's gradient), through LDS into accumulator layout (tokens 4 p + r, column col_of(j, n)): one
+// load of whole 16-byte pieces and a transposing read instead of 4 CT loads of single elements, each of which costs the memory pipe 30 cycles.
+template <typename T, int CT, bool WHOLE>
+struct VTile {
+    static constexpr int kRow = 16 * CT * (int)sizeof(T) + 16, kBytes = 16 * kRow;   // per wave
+    static constexpr int kPieces = 16 * CT * 2, kN = (kPieces + 63) / 64;             // pieces of 8 elements
+    char* base;
+    Raw8<T> r[kN];
+    __device__ __forceinline__ void fetch(const Rows<T>& x, int first, int len, int col0, int dv, int lane) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int id = lane + 64 * i, row = (id / (2 * CT)) & 15, at = first + row;
+            r[i] = load_raw8<WHOLE, T>(x.row(at < len ? at : len - 1), col0 + 8 * (id % (2 * CT)), dv);
+        }
+    }
+    // rows behind the end: kept (v, whose beta is 0) or cleared (gradients)
+    __device__ __forceinline__ void hand(int first, int len, int col0, int dv, int lane, bool keep_tail) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int id = lane + 64 * i, row = id / (2 * CT);
+            const Raw8<T> v = clear<WHOLE, T>(r[i], col0 + 8 * (id % (2 * CT)), dv, keep_tail || first + row < len);
+            if (id < kPieces) __builtin_memcpy(base + row * kRow + 8 * (id % (2 * CT)) * (int)sizeof(T), &v, sizeof(v));
+        }
+    }
+    __device__ __forceinline__ f32x4 get(int j, int n, int p) const {
+        f32x4 v;
+        if constexpr (sizeof(T) == 2) {
+            const vec_t<T, 4> h = __builtin_bit_cast(vec_t<T, 4>, read_tr(base + (4 * p + (n >> 2)) * kRow + 2 * (4 * CT * (n & 3) + 4 * j)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(h[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(base + (4 * p + e) * kRow + 4 * col_of<CT>(j, n));
+        }
+        return v;
+    }
+};
+// A wave's gates: gam, bet, del of its 16 tokens and gam of the chunk's last one, one load for all, through LDS
+struct GateTile {
+    static constexpr int kBytes = 256;   // per wave
+    float* base;
+    float r;
+    __device__ __forceinline__ void fetch(const float* g, int w, int lane) { r = g[lane < 48 ? (lane >> 4) * C + 16 * w + (lane & 15) : C - 1]; }
+    __device__ __forceinline__ void hand(int lane) const { base[lane] = r; }
+    __device__ __forceinline__ f32x4 four(int which, int p) const { return *reinterpret_cast<const f32x4*>(base + 16 * which + 4 * p); }
+    __device__ __forceinline__ float gam(int n) const { return base[n]; }
+    __device__ __forceinline__ float last() const { return base[48]; }
+};
 template <typename T>
 __device__ __forceinline__ Frag<Prec<T>::NX> planes_of(const Raw8<T>& r) {
     Frag<Prec<T>::NX> f;
@@ -129,10 +226,6 @@ __device__ __forceinline__ void tile_put(char* tile, int row, int c, const Frag<
 #pragma unroll
     for (int i = 0; i < NX; ++i) *reinterpret_cast<bf16x8*>(tile + i * tile_bytes<KP>() + row * tile_row<KP>() + 2 * c) = f.p[i];
 }
-__device__ __forceinline__ bf16x4 read_tr(const char* at) {   // 4 x 16 elements transposed among 16 lanes
-    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at));
-}
-__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 // lane: column 16 m + n, tokens of block tb (32) in paired order.  ds_read_b64_tr_b16: lane i of 16 names row i / 4, column group i % 4
 template <int KP, int NX>
 __device__ __forceinline__ Frag<NX> tile_cols(const char* tile, int m, int tb, int n, int p) {
@@ -154,13 +247,10 @@ struct Exchange {
         float x[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            bf16x4 h;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                h[e] = static_cast<bf16_t>(x[e]);
-                if (i + 1 < N) x[e] -= static_cast<float>(h[e]);
-            }
-            *reinterpret_cast<bf16x4*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at) = h;
+            vec_t<unsigned, 2> u;
+            u[0] = take_bf16(x[0], x[1], i + 1 == N);
+            u[1] = take_bf16(x[2], x[3], i + 1 == N);
+            *reinterpret_cast<vec_t<unsigned, 2>*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at) = u;
         }
     }
     __device__ __forceinline__ Frag<N> get(int j, int n, int at) const {
@@ -209,7 +299,7 @@ __host__ inline Layout layout(const vms_gated_delta_params& p) {
     l.chunks = (p.seqlen + C - 1) / C;
     l.vpad = ceil_to(p.dv, 32);
     const int64_t slots = (int64_t)p.batch * p.heads * l.chunks;
-    l.tri_slot = (int64_t)(p.for_backward ? 4 : 2) * ns * kTri;   // the planes of T, those of M, and of their transposes
+    l.tri_slot = (int64_t)(ns + no + (p.for_backward ? 2 * ns : 0)) * kTri;   // planes of T (NS), M (NO) and, for the backward's recurrence, their transposes (NS)
     l.s_slot = (int64_t)no * pad_k(p.dk) * l.vpad * 2;
     l.u_slot = (int64_t)no * C * l.vpad * 2;
     int64_t at = 0;
@@ -277,17 +367,38 @@ inline int allow_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
     if (e != hipSuccess) { set_error("hipFuncSetAttribute: %s", hipGetErrorString(e)); return VMS_ERR_LAUNCH; }
     return VMS_OK;
 }
-// one 16 x 16 accumulator tile (rows row0 + 4 p + r, column col0 + n) into NO planes of (rows, vpad): through unit_frag, so that a lane
-// stores 4 consecutive columns of one row
-template <int NO>
-__device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int row0, int col0, const f32x4& v, int n, int p) {
+// CT accumulator tiles (rows row0 + 4 p + r, column col0 + col_of(j, n)) into NO planes of (rows, vpad): through unit_frag, so that a lane
+// stores 4 CT consecutive columns of one row.  vpad and col0 are multiples of 16 CT or of 32: a slice is inside or outside whole, or CT = 1
+template <int NO, int CT>
+__device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int row0, int col0, const f32x4 (&v)[CT], int n, int p) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    const Frag<NO> f = frag_of<NO>(v, zero);
-    if (col0 < vpad) {
+    if (col0 >= vpad) return;
+    Frag<NO> f[CT];
 #pragma unroll
-        for (int i = 0; i < NO; ++i)
-            store_planes4(base + 2 * (((int64_t)i * rows + row0 + n) * vpad + col0 + 4 * p),
-                          __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, p), zero, 0, 0, 0));
+    for (int j = 0; j < CT; ++j) f[j] = frag_of<NO>(v[j], zero);
+#pragma unroll
+    for (int i = 0; i < NO; ++i) {
+        vec_t<bf16_t, 4 * CT> o;
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[j].p[i], unit_frag(0, n, p), zero, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * j + e] = static_cast<bf16_t>(x[e]);
+        }
+        *reinterpret_cast<vec_t<bf16_t, 4 * CT>*>(base + 2 * (((int64_t)i * rows + row0 + n) * vpad + col0 + 4 * CT * p)) = o;
+    }
+}
+template <typename T, int CT>
+__device__ __forceinline__ void store_cols(T* row, int c, int n, const f32x4 (&v)[CT]) {   // columns c .. c + 4 CT - 1 of a row of n
+    T o[4 * CT];
+#pragma unroll
+    for (int e = 0; e < 4 * CT; ++e) o[e] = static_cast<T>(v[e >> 2][e & 3]);
+    if (c + 4 * CT <= n) {
+        __builtin_memcpy(row + c, o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4 * CT; ++e)
+            if (c + e < n) row[c + e] = o[e];
     }
 }
 

@@ -25,7 +25,7 @@ struct BwdArgs {   // what the kernels need of vms_gated_delta_bwd_params (one k
 // ---- the walk over the chunks, from the end ------------------------------------------------------------------
 // Split among the four waves as the forward's walk: wave w has token tile w of dU and Y and dk / 4 rows of dS.  Three exchanges per chunk: dS, dU, Y;
 // dO of the next chunk is handed over while dS is updated, Q and K go through LDS for their transposes.
-template <typename T, int KP, int CT, bool WHOLE>
+template <typename T, int KP, int CT, int FIT>
 __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
     constexpr int KB = KP / 32, DW = KP / 64;
@@ -35,6 +35,7 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
     const Exchange<NS, CT, KP> Sx{Qs + NX * tile_bytes<KP>()};
     const Exchange<NX, CT, C> Ox{Sx.base + Sx.kBytes};                                                                 // dO
     const Exchange<NS, CT, C> Gx{Ox.base + Ox.kBytes}, Ux{Gx.base + Gx.kBytes}, Yx{Ux.base + Ux.kBytes};   // scale gam dO, dU, -beta gam Y
+    char* const own = Yx.base + Yx.kBytes;   // per wave: dO, gates
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
@@ -44,60 +45,42 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
     const int b = pair / p.heads, h = pair % p.heads, hk = h / (p.heads / p.heads_k);
     const int len = length_of(p, b), nc = (len + C - 1) / C;
     const int col0 = slice * CT * 16;
-    const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
-    const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
-    const T* const dob = static_cast<const T*>(a.q.dout) + (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride;
+    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
+    const Rows<T> dO(a.q.dout, (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride, a.q.dout_seq_stride, len, p.reverse);
     const int64_t dv_seq = (int64_t)p.heads * p.dv;
     T* const dvb = static_cast<T*>(a.q.dv) + ((int64_t)b * p.seqlen * p.heads + h) * p.dv;
     const char* const ws = static_cast<const char*>(p.workspace);
     char* const wb = static_cast<char*>(a.q.workspace);
     const int64_t slot0 = (int64_t)pair * l.chunks;
 
-    Raw8<T> kr[KB], qr[KB];   // token 16 w + n
+    Raw8<T> kr[KB], qr[KB], kx[KB], qx[KB];   // token 16 w + n: this chunk's, the next one's
     Frag<NS> tf[2], mf[2];    // columns 16 w + n of T, M (row blocks 0, 1; tiles 2 and 3 have no block 0)
-    T vr[CT][4], vn[CT][4];   // dO at tokens 16 w + 4 q4 + r, column n: this chunk's, the next one's
-    f32x4 ga, be, de;
-    float glast;
-    auto fetch_qk = [&](int c) __attribute__((always_inline)) {
+    VTile<T, CT, FIT != 0> ot{own + w * (VTile<T, CT, FIT != 0>::kBytes + GateTile::kBytes)};   // dO
+    GateTile gt{reinterpret_cast<float*>(ot.base + ot.kBytes)};
+    auto fetch_rows = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {
         const int at = c * C + 16 * w + n;
-        const int64_t t = at < len ? token(at, len, p.reverse) : 0;
+        const T* const row = x.row(at < len ? at : len - 1);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            kr[kb] = load_raw8<WHOLE, T>(kb_ + t * p.k_seq_stride, 32 * kb + 8 * q4, p.dk);
-            qr[kb] = load_raw8<WHOLE, T>(qb + t * p.q_seq_stride, 32 * kb + 8 * q4, p.dk);
-        }
+        for (int kb = 0; kb < KB; ++kb) r[kb] = fit_load<FIT, T>(row, 32 * kb + 8 * q4, p.dk);
     };
-    auto fetch_do = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int at = c * C + 16 * w + 4 * q4 + r;
-            const T* const row = dob + (at < len ? (int64_t)token(at, len, p.reverse) * a.q.dout_seq_stride : 0);
-#pragma unroll
-            for (int j = 0; j < CT; ++j) vn[j][r] = row[col0 + 16 * j + n < p.dv ? col0 + 16 * j + n : 0];
-        }
+    auto fetch_small = [&](int c) __attribute__((always_inline)) {
+        ot.fetch(dO, c * C + 16 * w, len, col0, p.dv, lane);
+        gt.fetch(reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c), w, lane);
     };
-    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // first: 2 NS T, 3 NS M (their transposes)
+    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // first: NS + NO T, 2 NS + NO M (their transposes)
         const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;
         f[0] = tri_cols<NS>(at, w, w >= 2 ? 1 : 0, lane);
         f[1] = tri_cols<NS>(at, w, 1, lane);
     };
-    auto fetch_gates = [&](int c) __attribute__((always_inline)) {
-        const Gates* const g = reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c;
-        ga = *reinterpret_cast<const f32x4*>(&g->gam[16 * w + 4 * q4]);
-        be = *reinterpret_cast<const f32x4*>(&g->bet[16 * w + 4 * q4]);
-        de = *reinterpret_cast<const f32x4*>(&g->del[16 * w + 4 * q4]);
-        glast = g->gam[C - 1];
-    };
-    auto out_grad = [&](int c, int j, int r, const T (&v)[CT][4]) __attribute__((always_inline)) {
-        return c * C + 16 * w + 4 * q4 + r < len && col0 + 16 * j + n < p.dv ? static_cast<float>(v[j][r]) : 0.f;
-    };
-    auto hand_do = [&](int c) __attribute__((always_inline)) {   // vn -> Ox
+    f32x4 out_grad[CT];   // dO of this wave's tokens
+    auto hand_small = [&](int c) __attribute__((always_inline)) {   // gates and dO to this wave, dO to the others
+        ot.hand(c * C + 16 * w, len, col0, p.dv, lane, false);
+        gt.hand(lane);
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-            f32x4 x;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = out_grad(c, j, r, vn);
-            Ox.put(j, n, paired(w, q4), x);
+            out_grad[j] = ot.get(j, n, q4);
+            Ox.put(j, n, paired(w, q4), out_grad[j]);
         }
     };
 
@@ -110,37 +93,37 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
         for (int j = 0; j < CT; ++j) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
+                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
                 dS[d][j][r] = a.q.dfinal_state && row < p.dk && col < p.dv ? a.q.dfinal_state[sbase + (int64_t)row * p.dv + col] : 0.f;
             }
             Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
         }
     if (nc > 0) {
-        fetch_do(nc - 1);
-        fetch_qk(nc - 1);
-        fetch_tri(nc - 1, 2 * NS, tf);
-        fetch_tri(nc - 1, 3 * NS, mf);
-        fetch_gates(nc - 1);
-        hand_do(nc - 1);
+        fetch_rows(K, nc - 1, kx);
+        fetch_rows(Q, nc - 1, qx);
+        fetch_small(nc - 1);
+        fetch_tri(nc - 1, 2 * NS + NO, mf);
+        fetch_tri(nc - 1, NS + NO, tf);
+        hand_small(nc - 1);
     }
     for (int c = nc - 1; c >= 0; --c) {
         const int next = c > 0 ? c - 1 : 0;   // the first chunk again rather than a branch
         const int64_t slot = slot0 + c;
         const bool ok_n = c * C + 16 * w + n < len;
 #pragma unroll
-        for (int j = 0; j < CT; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) vr[j][r] = vn[j][r];
-        fetch_do(next);
+        for (int kb = 0; kb < KB; ++kb) { kr[kb] = kx[kb]; qr[kb] = qx[kb]; }
+        const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
+        const float glast = gt.last();
         __syncthreads();   // dS and dO are there; the tiles of K and Q are no longer read
+        fetch_rows(K, next, kx);   // (a few loads at a time, a chunk ahead: gd_scan)
         // ---- dU = del K dS1 + M^T dO
         f32x4 dU[CT];
 #pragma unroll
         for (int j = 0; j < CT; ++j) dU[j] = zero;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            const Frag<NX> kf = planes_of<T>(clear<WHOLE, T>(kr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
-            const Frag<NX> qf = planes_of<T>(clear<WHOLE, T>(qr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
+            const Frag<NX> kf = planes_of<T>(fit_clear<FIT, T>(kr[kb], 32 * kb + 8 * q4, p.dk));
+            const Frag<NX> qf = planes_of<T>(fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk));
             tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
             tile_put<KP, NX>(Qs, 16 * w + n, 32 * kb + 8 * q4, qf);
 #pragma unroll
@@ -159,15 +142,14 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             Ux.put(j, n, paired(w, q4), dU[j]);
             f32x4 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = p.scale * ga[r] * out_grad(c, j, r, vr);
+            for (int r = 0; r < 4; ++r) x[r] = p.scale * ga[r] * out_grad[j][r];
             Gx.put(j, n, paired(w, q4), x);
         }
-        fetch_qk(next);
-        fetch_tri(next, 3 * NS, mf);
+        fetch_rows(Q, next, qx);
+        fetch_tri(next, 2 * NS + NO, mf);
+        fetch_small(next);
 #pragma unroll
-        for (int d = 0; d < DW; ++d)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) store_rows<NO>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0 + 16 * j, dS[d][j], n, q4);
+        for (int d = 0; d < DW; ++d) store_rows<NO, CT>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0, dS[d], n, q4);
         __syncthreads();
         // ---- Y = T^T dU, dV = beta Y
         f32x4 Y[CT];
@@ -188,15 +170,13 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             for (int r = 0; r < 4; ++r) x[r] = -ga[r] * V[j][r];
             Yx.put(j, n, paired(w, q4), x);
         }
-        const float gl = glast;
-        fetch_tri(next, 2 * NS, tf);
-        fetch_gates(next);
+        fetch_tri(next, NS + NO, tf);
         __syncthreads();
         // ---- dS0 = gam dS1 + Q^T (scale gam dO) - K^T (beta gam Y)
 #pragma unroll
         for (int d = 0; d < DW; ++d)
 #pragma unroll
-            for (int j = 0; j < CT; ++j) dS[d][j] *= gl;
+            for (int j = 0; j < CT; ++j) dS[d][j] *= glast;
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
             Frag<NS> gf[CT], yf[CT];
@@ -216,16 +196,17 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
         for (int d = 0; d < DW; ++d)
 #pragma unroll
             for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
-        hand_do(next);
+        hand_small(next);
+        store_rows<NO, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
+        f32x4 dv[CT];
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-            store_rows<NO>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0 + 16 * j, Y[j], n, q4);
             const Frag<NO> f = frag_of<NO>(V[j], zero);
-            f32x4 dv = zero;
+            dv[j] = zero;
 #pragma unroll
-            for (int i = NO - 1; i >= 0; --i) dv = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv, 0, 0, 0);
-            if (ok_n) store4<T>(dvb + (int64_t)token(c * C + 16 * w + n, len, p.reverse) * dv_seq, col0 + 16 * j + 4 * q4, p.dv, dv);
+            for (int i = NO - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
         }
+        if (ok_n) store_cols<T, CT>(dvb + (int64_t)token(c * C + 16 * w + n, len, p.reverse) * dv_seq, col0 + 4 * CT * q4, p.dv, dv);
     }
     if (a.q.dinitial_state) {
 #pragma unroll
@@ -234,7 +215,7 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             for (int j = 0; j < CT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
+                    const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
                     if (row < p.dk && col < p.dv) a.q.dinitial_state[sbase + (int64_t)row * p.dv + col] = dS[d][j][r];
                 }
     }
@@ -497,15 +478,16 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
-template <typename T, int KP, int CT, bool WHOLE>
+template <typename T, int KP, int CT, int FIT>
 static int bwd_scan_launch(const BwdArgs& a, hipStream_t s) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int lds = 2 * NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + Exchange<NX, CT, C>::kBytes + 3 * Exchange<NS, CT, C>::kBytes;
+    constexpr int lds = 2 * NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + Exchange<NX, CT, C>::kBytes + 3 * Exchange<NS, CT, C>::kBytes
+                        + 4 * (VTile<T, CT, true>::kBytes + GateTile::kBytes);
     static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, KP, CT, WHOLE>), lds)) return rc;
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, KP, CT, FIT>), lds)) return rc;
     const int slices = (a.l.vpad + CT * 16 - 1) / (CT * 16);
-    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, CT, WHOLE>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(256), lds, s, a, slices);
+    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, CT, FIT>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(256), lds, s, a, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
@@ -521,9 +503,10 @@ static int grad_launch(const BwdArgs& a, hipStream_t s) {
 template <typename T, int KP>
 static int bwd_launch(const BwdArgs& a, hipStream_t s) {
     constexpr int kCT = sizeof(T) == 4 ? 1 : 2;   // column tiles of a workgroup: fp32's six planes of K and Q leave LDS for one
-    const bool whole = a.q.f.dk % 8 == 0;
-    if (int rc = whole ? bwd_scan_launch<T, KP, kCT, true>(a, s) : bwd_scan_launch<T, KP, kCT, false>(a, s)) return rc;
-    return whole && a.q.f.dv % 8 == 0 ? grad_launch<T, KP, true>(a, s) : grad_launch<T, KP, false>(a, s);
+    const int fit = fit_of(a.q.f.dk, a.q.f.dv);
+    const int rc = fit == 2 ? bwd_scan_launch<T, KP, kCT, 2>(a, s) : fit == 1 ? bwd_scan_launch<T, KP, kCT, 1>(a, s) : bwd_scan_launch<T, KP, kCT, 0>(a, s);
+    if (rc) return rc;
+    return fit ? grad_launch<T, KP, true>(a, s) : grad_launch<T, KP, false>(a, s);
 }
 template <typename T>
 static int bwd_type(const BwdArgs& a, hipStream_t s) {
@@ -539,6 +522,7 @@ extern "C" int vms_gated_delta_bwd(const vms_gated_delta_bwd_params* qq, void* s
     VMS_CHECK(qq != nullptr, "null params");
     if (int rc = gd::validate(qq->f)) return rc;
     VMS_CHECK(qq->f.for_backward, "the forward must have run with for_backward");
+    VMS_CHECK(qq->dout_seq_stride > -(1LL << 31) && qq->dout_seq_stride < (1LL << 31), "strides along the sequence of less than 2^31 elements");
     VMS_CHECK(qq->dout && qq->dq && qq->dk && qq->dv && qq->dg && qq->dbeta, "dout, dq, dk, dv, dg, dbeta are required");
     gd::BwdArgs a{*qq, gd::layout(qq->f)};
     VMS_CHECK(qq->workspace != nullptr && qq->workspace_bytes >= a.l.bwd_bytes, "workspace is too small (vms_gated_delta_bwd_workspace_bytes)");

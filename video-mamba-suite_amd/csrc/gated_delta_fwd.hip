@@ -18,9 +18,9 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __bui
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
-template <typename T, int KP, bool WHOLE>   // WHOLE: dk % 8 == 0
+template <typename T, int KP, int FIT>
 __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_params p, const Layout l) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
     constexpr int AR = 68;   // row pitch of As, floats
     __shared__ __attribute__((aligned(16))) float As[C * AR];
     __shared__ double Gs[C];
@@ -59,25 +59,21 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
     }
     __syncthreads();
 
-    const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
-    const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
-    auto rows = [&](const T* base, int64_t stride, int rt, int kb) __attribute__((always_inline)) {
+    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
+    auto rows = [&](const Rows<T>& x, int rt, int kb) __attribute__((always_inline)) {
         const int i = c * C + 16 * rt + n;
-        const bool ok = i < len;
-        const T* const row = base + (ok ? (int64_t)token(i, len, p.reverse) * stride : 0);
-        return load_raw8<WHOLE, T>(row, 32 * kb + 8 * q4, p.dk);
+        return fit_load<FIT, T>(x.row(i < len ? i : len - 1), 32 * kb + 8 * q4, p.dk);
     };
-    auto as_frag = [&](const Raw8<T>& r, int rt, int kb) __attribute__((always_inline)) {
-        return planes_of<T>(clear<WHOLE, T>(r, 32 * kb + 8 * q4, p.dk, c * C + 16 * rt + n < len));
-    };
+    auto as_frag = [&](const Raw8<T>& r, int kb) __attribute__((always_inline)) { return planes_of<T>(fit_clear<FIT, T>(r, 32 * kb + 8 * q4, p.dk)); };
     Raw8<T> kraw[4][KP / 32];
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
-        for (int kb = 0; kb < KP / 32; ++kb) kraw[rt][kb] = rows(kb_, p.k_seq_stride, rt, kb);
+        for (int kb = 0; kb < KP / 32; ++kb) kraw[rt][kb] = rows(K, rt, kb);
     char* const tw = ws + l.tri + slot * l.tri_slot;
     char* const mw = tw + NS * kTri;
-    char* const ttw = mw + NS * kTri;   // transposes (for_backward)
+    char* const ttw = mw + NO * kTri;   // transposes (for_backward)
     char* const mtw = ttw + NS * kTri;
     auto put4 = [&](char* at, const f32x4& v) __attribute__((always_inline)) {   // half an operand, NS planes
         float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
@@ -93,13 +89,13 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
         for (int ct = 0; ct < 4; ++ct) { kk[ct] = f32x4{0.f, 0.f, 0.f, 0.f}; qk[ct] = kk[ct]; kq[ct] = kk[ct]; }
         Raw8<T> qraw[KP / 32];
 #pragma unroll
-        for (int kb = 0; kb < KP / 32; ++kb) qraw[kb] = rows(qb, p.q_seq_stride, rt, kb);
+        for (int kb = 0; kb < KP / 32; ++kb) qraw[kb] = rows(Q, rt, kb);
 #pragma unroll
         for (int kb = 0; kb < KP / 32; ++kb) {
-            const Frag<NX> qi = as_frag(qraw[kb], rt, kb), ki = as_frag(kraw[rt][kb], rt, kb);
+            const Frag<NX> qi = as_frag(qraw[kb], kb), ki = as_frag(kraw[rt][kb], kb);
 #pragma unroll
             for (int ct = 0; ct <= rt; ++ct) {   // [j][i]: lane i, 4 consecutive j
-                const Frag<NX> kj = ct == rt ? ki : as_frag(kraw[ct][kb], ct, kb);
+                const Frag<NX> kj = ct == rt ? ki : as_frag(kraw[ct][kb], kb);
                 mma<NS>(kk[ct], kj, ki);
                 mma<NS>(qk[ct], kj, qi);
                 if (p.for_backward) mma<NS>(kq[ct], qi, kj);
@@ -132,9 +128,9 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
         if (p.for_backward && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
 #pragma unroll
         for (int kb = 0; kb <= rt / 2; ++kb) {
-            const Frag<NS> f = frag_of<NS>(qk[2 * kb], qk[2 * kb + 1]);
+            const Frag<NO> f = frag_of<NO>(qk[2 * kb], qk[2 * kb + 1]);
 #pragma unroll
-            for (int i2 = 0; i2 < NS; ++i2)
+            for (int i2 = 0; i2 < NO; ++i2)
                 *reinterpret_cast<bf16x8*>(mw + i2 * kTri + 1024 * tri(rt, kb) + 16 * lane) = f.p[i2];
         }
     }
@@ -233,7 +229,7 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 // a whole chunk of 16 columns to itself (no exchange, every wave reading all of K, Q, T, M from LDS) took 5.4 us per chunk at dk = 128,
 // four waves on one chunk take 1.5: three barriers, but a quarter of the products in a row and each operand of K, Q, T, M read once, straight
 // from memory into the registers of the one wave that uses it.  K alone also goes through LDS, for its transpose.
-template <typename T, int KP, int CT, bool WHOLE, bool TRAIN>
+template <typename T, int KP, int CT, int FIT, bool TRAIN>
 __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
     constexpr int KB = KP / 32, DW = KP / 64;   // 32-column blocks of k; 16-row tiles of S per wave
@@ -241,6 +237,7 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
     char* const Ks = lds;
     const Exchange<NS, CT, KP> Sx{Ks + NX * tile_bytes<KP>()};
     const Exchange<NS, CT, C> Rx{Sx.base + Sx.kBytes}, Ux{Rx.base + Rx.kBytes}, Dx{Ux.base + Ux.kBytes};   // R, U, del U
+    char* const own = Dx.base + Dx.kBytes;   // per wave: v, gates
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
     int pair, slice;
@@ -248,48 +245,43 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
     const int b = pair / p.heads, h = pair % p.heads, hk = h / (p.heads / p.heads_k);
     const int len = length_of(p, b), nc = (len + C - 1) / C;
     const int col0 = slice * CT * 16;
-    const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
-    const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
-    const T* const vb = static_cast<const T*>(p.v) + (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride;
+    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
+    const Rows<T> V(p.v, (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride, p.v_seq_stride, len, p.reverse);
     T* const ob = static_cast<T*>(p.out) + (int64_t)b * p.out_batch_stride + (int64_t)h * p.out_head_stride;
+    const Rows<T> O_(p.out, (int64_t)b * p.out_batch_stride + (int64_t)h * p.out_head_stride, p.out_seq_stride, len, p.reverse);
     char* const ws = static_cast<char*>(p.workspace);
     const int64_t slot0 = (int64_t)pair * l.chunks;
 
-    Raw8<T> kr[KB], qr[KB];   // token 16 w + n
-    Frag<NS> tf[2], mf[2];    // rows 16 w + n of T, M (blocks 0, 1; tiles 0 and 1 have no block 1)
-    T vr[CT][4];              // tokens 16 w + 4 q4 + r, column n
-    f32x4 ga, be, de;         // gates of those tokens
-    float gn, glast;          // gam of token 16 w + n, of the last one
-    auto fetch_qkv = [&](int c) __attribute__((always_inline)) {
+    Raw8<T> kr[KB], qr[KB], kx[KB], qx[KB];   // token 16 w + n: this chunk's, the next one's
+    Frag<NS> tf[2];           // rows 16 w + n of T, M (blocks 0, 1; tiles 0 and 1 have no block 1)
+    Frag<NO> mf[2];
+    VTile<T, CT, FIT != 0> vt{own + w * (VTile<T, CT, FIT != 0>::kBytes + GateTile::kBytes)};
+    GateTile gt{reinterpret_cast<float*>(vt.base + vt.kBytes)};
+    auto fetch_rows = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {
         const int at = c * C + 16 * w + n;
-        const int64_t t = at < len ? token(at, len, p.reverse) : 0;
+        const T* const row = x.row(at < len ? at : len - 1);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            kr[kb] = load_raw8<WHOLE, T>(kb_ + t * p.k_seq_stride, 32 * kb + 8 * q4, p.dk);
-            qr[kb] = load_raw8<WHOLE, T>(qb + t * p.q_seq_stride, 32 * kb + 8 * q4, p.dk);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int at2 = c * C + 16 * w + 4 * q4 + r;
-            const T* const row = vb + (at2 < len ? (int64_t)token(at2, len, p.reverse) * p.v_seq_stride : 0);
-#pragma unroll
-            for (int j = 0; j < CT; ++j) vr[j][r] = row[col0 + 16 * j + n < p.dv ? col0 + 16 * j + n : 0];
-        }
+        for (int kb = 0; kb < KB; ++kb) r[kb] = fit_load<FIT, T>(row, 32 * kb + 8 * q4, p.dk);
     };
-    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // first: 0 T, NS M
-        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;
-        f[0] = tri_rows<NS>(at, w, 0, lane);
-        f[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
+    auto fetch_small = [&](int c) __attribute__((always_inline)) {
+        vt.fetch(V, c * C + 16 * w, len, col0, p.dv, lane);
+        gt.fetch(reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c), w, lane);
     };
-    auto fetch_gates = [&](int c) __attribute__((always_inline)) {
-        const Gates* const g = reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c;
-        ga = *reinterpret_cast<const f32x4*>(&g->gam[16 * w + 4 * q4]);
-        be = *reinterpret_cast<const f32x4*>(&g->bet[16 * w + 4 * q4]);
-        de = *reinterpret_cast<const f32x4*>(&g->del[16 * w + 4 * q4]);
-        gn = g->gam[16 * w + n];
-        glast = g->gam[C - 1];
+    auto hand_small = [&](int c) __attribute__((always_inline)) {   // to this wave itself
+        vt.hand(c * C + 16 * w, len, col0, p.dv, lane, true);
+        gt.hand(lane);
     };
-
+    auto fetch_t = [&](int c) __attribute__((always_inline)) {
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot;
+        tf[0] = tri_rows<NS>(at, w, 0, lane);
+        tf[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
+    };
+    auto fetch_m = [&](int c) __attribute__((always_inline)) {
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + NS * kTri;
+        mf[0] = tri_rows<NO>(at, w, 0, lane);
+        mf[1] = tri_rows<NO>(at, w, w >= 2 ? 1 : 0, lane);
+    };
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     f32x4 S[DW][CT];   // rows 16 (DW w + d) + 4 q4 + r, column n
     const int64_t sbase = (int64_t)pair * p.dk * p.dv;
@@ -299,30 +291,42 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
         for (int j = 0; j < CT; ++j) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
+                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
                 S[d][j][r] = p.initial_state && row < p.dk && col < p.dv ? p.initial_state[sbase + (int64_t)row * p.dv + col] : 0.f;
             }
             Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
         }
     if (nc > 0) {
-        fetch_qkv(0);
-        fetch_tri(0, 0, tf);
-        fetch_tri(0, NS, mf);
-        fetch_gates(0);
+        fetch_rows(K, 0, kx);
+        fetch_rows(Q, 0, qx);
+        fetch_small(0);
+        fetch_t(0);
+        fetch_m(0);
+        hand_small(0);
     }
     for (int c = 0; c < nc; ++c) {
         const int next = c + 1 < nc ? c + 1 : c;   // the last chunk again rather than a branch
         const int64_t slot = slot0 + c;
         const bool ok_n = c * C + 16 * w + n < len;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) { kr[kb] = kx[kb]; qr[kb] = qx[kb]; }
+        const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
+        const float sg = p.scale * gt.gam(n), glast = gt.last();
+        f32x4 vv[CT];
+#pragma unroll
+        for (int j = 0; j < CT; ++j) vv[j] = vt.get(j, n, q4);
         __syncthreads();   // S is there; K's tile is no longer read
+        // Loads return in order, stores among them, and the memory pipe takes 20 .. 50 cycles for each instruction of a wave: what a phase waits
+        // for is asked for a chunk earlier, a few instructions at a time
+        fetch_rows(K, next, kx);
         // ---- P = K S0, O = S0^T Q^T, R
         f32x4 P[CT], O[CT];
 #pragma unroll
         for (int j = 0; j < CT; ++j) { P[j] = zero; O[j] = zero; }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            const Frag<NX> kf = planes_of<T>(clear<WHOLE, T>(kr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
-            const Frag<NX> qf = planes_of<T>(clear<WHOLE, T>(qr[kb], 32 * kb + 8 * q4, p.dk, ok_n));
+            const Frag<NX> kf = planes_of<T>(fit_clear<FIT, T>(kr[kb], 32 * kb + 8 * q4, p.dk));
+            const Frag<NX> qf = planes_of<T>(fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk));
             tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
@@ -336,17 +340,14 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
             f32x4 R;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float v = c * C + 16 * w + 4 * q4 + r < len && col0 + 16 * j + n < p.dv ? static_cast<float>(vr[j][r]) : 0.f;
-                R[r] = be[r] * fmaf(-ga[r], P[j][r], v);
+                R[r] = be[r] * fmaf(-ga[r], P[j][r], vv[j][r]);   // beta = 0 behind the end
             }
             Rx.put(j, n, paired(w, q4), R);
         }
-        fetch_qkv(next);
+        fetch_rows(Q, next, qx);
         if constexpr (TRAIN) {   // S0 by rows: 4 consecutive columns per lane
 #pragma unroll
-            for (int d = 0; d < DW; ++d)
-#pragma unroll
-                for (int j = 0; j < CT; ++j) store_rows<NO>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0 + 16 * j, S[d][j], n, q4);
+            for (int d = 0; d < DW; ++d) store_rows<NO, CT>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0, S[d], n, q4);
         }
         __syncthreads();
         // ---- U = T R
@@ -361,11 +362,12 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
             for (int j = 0; j < CT; ++j) mma<NS>(U[j], tf[1], Rx.get(j, n, 32 + 8 * q4));
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-            f32x4 x = U[j] * de;
+            const f32x4 x = U[j] * de;
             Dx.put(j, n, paired(w, q4), x);
             Ux.put(j, n, paired(w, q4), U[j]);
         }
-        fetch_tri(next, 0, tf);
+        fetch_t(next);
+        fetch_small(next);
         __syncthreads();
         // ---- S1 = gam S0 + K^T (del U)
 #pragma unroll
@@ -389,26 +391,23 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
 #pragma unroll
             for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
         // ---- O += M U
-        const float sg = p.scale * gn;
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
             O[j] *= sg;
-            mma<NS>(O[j], Ux.get(j, n, 8 * q4), mf[0]);
+            mma<NS>(O[j], Ux.get(j, n, 8 * q4), mf[0]);   // (two planes of U keep the error of O at what M's one leaves)
         }
         if (w >= 2)
 #pragma unroll
             for (int j = 0; j < CT; ++j) mma<NS>(O[j], Ux.get(j, n, 32 + 8 * q4), mf[1]);
+        fetch_m(next);
         if (ok_n) {
-            T* const row = ob + (int64_t)token(c * C + 16 * w + n, len, p.reverse) * p.out_seq_stride;
-#pragma unroll
-            for (int j = 0; j < CT; ++j) store4<T>(row, col0 + 16 * j + 4 * q4, p.dv, O[j]);
+            T* const row = const_cast<T*>(O_.row(c * C + 16 * w + n));
+            store_cols<T, CT>(row, col0 + 4 * CT * q4, p.dv, O);
         }
         if constexpr (TRAIN) {
-#pragma unroll
-            for (int j = 0; j < CT; ++j) store_rows<NO>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, col0 + 16 * j, U[j], n, q4);
+            store_rows<NO, CT>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, col0, U, n, q4);
         }
-        fetch_tri(next, NS, mf);
-        fetch_gates(next);
+        hand_small(next);
     }
     if (p.final_state) {
 #pragma unroll
@@ -417,7 +416,7 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
             for (int j = 0; j < CT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + 16 * j + n;
+                    const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
                     if (row < p.dk && col < p.dv) p.final_state[sbase + (int64_t)row * p.dv + col] = S[d][j][r];
                 }
     }
@@ -438,21 +437,23 @@ int validate(const vms_gated_delta_params& p) {
     VMS_CHECK(p.heads <= 65535 && p.batch <= 65535 && p.seqlen <= (1 << 30), "problem too large");
     VMS_CHECK((int64_t)p.batch * p.heads * ((p.dv + 15) / 16) < (1LL << 31), "problem too large");
     VMS_CHECK(p.q && p.k && p.v && p.g && p.beta, "q, k, v, g, beta are required");
+    for (const int64_t n : {p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.out_seq_stride})
+        VMS_CHECK(n > -(1LL << 31) && n < (1LL << 31), "strides along the sequence of less than 2^31 elements");
     const Layout l = layout(p);
     VMS_CHECK(p.workspace != nullptr && p.workspace_bytes >= l.bytes, "workspace is too small (vms_gated_delta_workspace_bytes)");
     VMS_CHECK((reinterpret_cast<uintptr_t>(p.workspace) & 15) == 0, "workspace must be 16-byte aligned");
     return VMS_OK;
 }
 
-template <typename T, int KP, int CT, bool WHOLE, bool TRAIN>
+template <typename T, int KP, int CT, int FIT, bool TRAIN>
 static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStream_t s) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int lds = NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + 3 * Exchange<NS, CT, C>::kBytes;
+    constexpr int lds = NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + 3 * Exchange<NS, CT, C>::kBytes + 4 * (VTile<T, CT, true>::kBytes + GateTile::kBytes);
     static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, CT, WHOLE, TRAIN>), lds)) return rc;
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, CT, FIT, TRAIN>), lds)) return rc;
     const int slices = (l.vpad + CT * 16 - 1) / (CT * 16);
-    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, WHOLE, TRAIN>), dim3(p.batch * p.heads * slices), dim3(256), lds, s, p, l, slices);
+    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, FIT, TRAIN>), dim3(p.batch * p.heads * slices), dim3(256), lds, s, p, l, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
@@ -460,20 +461,25 @@ static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStre
 #define VMS_GD_CT 2
 #endif
 constexpr int kCT = VMS_GD_CT;
-template <typename T, int KP>
+template <typename T, int KP, int FIT>
 static int fwd_launch(const vms_gated_delta_params& p, hipStream_t s) {
     const Layout l = layout(p);
     const dim3 grid(l.chunks, p.heads, p.batch);
-    const bool whole = p.dk % 8 == 0;
-    if (whole) hipLaunchKernelGGL((gd_prep_kernel<T, KP, true>), grid, dim3(64), 0, s, p, l);
-    else hipLaunchKernelGGL((gd_prep_kernel<T, KP, false>), grid, dim3(64), 0, s, p, l);
+    hipLaunchKernelGGL((gd_prep_kernel<T, KP, FIT>), grid, dim3(64), 0, s, p, l);
     VMS_LAUNCH_CHECK();
-    if (p.for_backward) return whole ? scan_launch<T, KP, kCT, true, true>(p, l, s) : scan_launch<T, KP, kCT, false, true>(p, l, s);
-    return whole ? scan_launch<T, KP, kCT, true, false>(p, l, s) : scan_launch<T, KP, kCT, false, false>(p, l, s);
+    return p.for_backward ? scan_launch<T, KP, kCT, FIT, true>(p, l, s) : scan_launch<T, KP, kCT, FIT, false>(p, l, s);
+}
+template <typename T, int KP>
+static int fwd_fit(const vms_gated_delta_params& p, hipStream_t s) {
+    switch (fit_of(p.dk, p.dv)) {
+        case 2: return fwd_launch<T, KP, 2>(p, s);
+        case 1: return fwd_launch<T, KP, 1>(p, s);
+        default: return fwd_launch<T, KP, 0>(p, s);
+    }
 }
 template <typename T>
 static int fwd_type(const vms_gated_delta_params& p, hipStream_t s) {
-    return pad_k(p.dk) == 64 ? fwd_launch<T, 64>(p, s) : fwd_launch<T, 128>(p, s);
+    return pad_k(p.dk) == 64 ? fwd_fit<T, 64>(p, s) : fwd_fit<T, 128>(p, s);
 }
 
 }  // namespace gd
