@@ -12,6 +12,8 @@
 //                  dG_i = q_i.dQ_i - beta_i k_i.W_i - k_i.X_i, and <S1, dS1> = gam_63 <S0, dS1> + sum_j del_j k_j.(U dS1^T)_j at the
 //                  last token; dg = the sums of dG from a token to the chunk's end
 //                No atomics: heads that share q / k are summed by the workgroup that owns the chunk, in order.
+#include <type_traits>
+
 #include "gated_delta.h"
 
 namespace vms {
@@ -236,22 +238,38 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
 }
 __device__ __forceinline__ float L_of(double d) { return fast_exp2((float)(d * 1.4426950408889634)); }
 
-template <typename T, int KP, bool WHOLE>   // WHOLE: dk % 8 == 0 and dv % 8 == 0
-__global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
+// Stage 1 walks v 32 columns at a time: U, Y, dO (64 rows) and S0, dS1 (KP rows) go through registers (the next block is on its way while this one is
+// multiplied) into LDS, 16-byte operands from there; the sums that need no product (Y.V, <S0, dS1>) are taken from the pieces as they pass.  Eight waves:
+// wave w has token tile w % 4 of dQ and W (w < 4: "left", what depends on the token as the later one) or of X (w >= 4: "right"), so that no product is
+// made twice and the accumulators fit.  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
+template <typename T, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
+__global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO, DT = KP / 16, TB = tile_bytes<KP>();
-    constexpr int PK = C * KP / 8 / 256;
+    constexpr int PK = C * KP / 8 / 512;   // 8-element pieces of a q / k tile per thread
+    constexpr int ROW = 80;                 // bytes of 32 columns in LDS: 16 rows fall on all banks
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char* const Ks = lds;
-    char* const Qs = Ks + NX * TB;
-    Gates* const gs = reinterpret_cast<Gates*>(Qs + NX * TB);
+    Gates* const gs = reinterpret_cast<Gates*>(lds);
     float* const dGs = reinterpret_cast<float*>(gs + 1);
-    float* const part = dGs + C;   // one sum per wave
+    float* const kxs = dGs + C;
+    float* const yvs = kxs + C;
+    float* const part = yvs + C;   // one sum per wave
+    char* const big = reinterpret_cast<char*>(part + 8);
+    char* const Ks = big;          // stage 2
+    char* const Qs = Ks + NX * TB;
+    f32x4* const Wx = reinterpret_cast<f32x4*>(Qs + NX * TB);   // beta W, from the left wave to the right one
+    char* const Us = big;          // stage 1
+    char* const Ys = Us + NO * C * ROW;
+    char* const Os = Ys + NO * C * ROW;
+    char* const Ss = Os + NX * C * ROW;
+    char* const Ds = Ss + NO * KP * ROW;
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
+    const int w = w8 & 3;
+    const bool left = w8 < 4;
     const int c = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-    const int rep = p.heads / p.heads_k;
+    const int rep = SHARED ? p.heads / p.heads_k : 1;
     const int len = length_of(p, b);
     const int64_t dk_seq = (int64_t)p.heads_k * p.dk;
     T* const dqb = static_cast<T*>(a.q.dq) + ((int64_t)b * p.seqlen * p.heads_k + hk) * p.dk;
@@ -260,7 +278,7 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
     // padding rows of this chunk
     {
         const int first = c * C > len ? c * C : len, end = (c + 1) * C < p.seqlen ? (c + 1) * C : p.seqlen;
-        for (int t = first + w; t < end; t += 4) {
+        for (int t = first + w8; t < end; t += 8) {
             for (int cc = lane; cc < p.dk; cc += 64) {
                 dqb[(int64_t)t * dk_seq + cc] = static_cast<T>(0.f);
                 dkb[(int64_t)t * dk_seq + cc] = static_cast<T>(0.f);
@@ -274,108 +292,151 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
     }
     if (c * C >= len) return;
 
-    const T* const qb = static_cast<const T*>(p.q) + (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride;
-    const T* const kb_ = static_cast<const T*>(p.k) + (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride;
-#pragma unroll
-    for (int i = 0; i < PK; ++i) {
-        const int id = tid + i * 256, row = id / (KP / 8), cc = 8 * (id % (KP / 8)), at = c * C + row;
-        const bool ok = at < len;
-        const int64_t t = ok ? token(at, len, p.reverse) : 0;
-        tile_put<KP, NX>(Ks, row, cc, planes_of<T>(clear<WHOLE, T>(load_raw8<WHOLE, T>(kb_ + t * p.k_seq_stride, cc, p.dk), cc, p.dk, ok)));
-        tile_put<KP, NX>(Qs, row, cc, planes_of<T>(clear<WHOLE, T>(load_raw8<WHOLE, T>(qb + t * p.q_seq_stride, cc, p.dk), cc, p.dk, ok)));
-    }
+    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
     const char* const ws = static_cast<const char*>(p.workspace);
     const char* const wb = static_cast<const char*>(a.q.workspace);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const int own = 16 * w + n, at_own = c * C + own;   // this lane's token
     const bool ok_own = at_own < len;
-    f32x4 dqs[DT], dks[DT];
+    // stage 1: a thread's piece of U and dO (left) or Y and V (right), of S0 and dS1
+    const int prow = (tid & 255) >> 2, pcol = 8 * (tid & 3), srow = (tid >> 2) & (KP - 1);
+    const bool has_s = tid < 4 * KP;
+    const int at_p = c * C + prow;
+    const bool ok_p = at_p < len;
+    f32x4 total[SHARED ? DT : 1];   // dQ (left), dK (right) over the heads
+    if constexpr (SHARED)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) { dqs[d] = zero; dks[d] = zero; }
+        for (int d = 0; d < DT; ++d) total[d] = zero;
 
     for (int r = 0; r < rep; ++r) {
         const int h = hk * rep + r;
         const int64_t slot = ((int64_t)b * p.heads + h) * l.chunks + c;
-        __syncthreads();   // the tiles are there / the previous head's gates are no longer read
-        {
-            const float* const src = reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot);
-            for (int i = tid; i < (int)(sizeof(Gates) / 4); i += 256) reinterpret_cast<float*>(gs)[i] = src[i];
-        }
-        const char* const Uw = ws + l.U + slot * l.u_slot;
-        const char* const Yw = wb + l.Y + slot * l.u_slot;
+        const char* const Aw = left ? ws + l.U + slot * l.u_slot : wb + l.Y + slot * l.u_slot;
         const char* const Sw = ws + l.S0 + slot * l.s_slot;
         const char* const Dw = wb + l.dS + slot * l.s_slot;
-        const T* const vb = static_cast<const T*>(p.v) + (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride;
-        const T* const dob = static_cast<const T*>(a.q.dout) + (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride;
-        auto planes = [&](const char* base, int rows, int row, int vblk) __attribute__((always_inline)) {   // natural order: 8 columns from 32 vblk + 8 q4
-            Frag<NO> f;
+        const Rows<T> V(p.v, (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride, p.v_seq_stride, len, p.reverse);
+        const Rows<T> dO(a.q.dout, (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride, a.q.dout_seq_stride, len, p.reverse);
+        const T* const brow = (left ? dO : V).row(ok_p ? at_p : len - 1);
+        Frag<NO> ap, sp, dp;
+        Raw8<T> bp;
+        auto fetch = [&](int vk) __attribute__((always_inline)) {
+            const int cc = 32 * vk + pcol;
 #pragma unroll
-            for (int i = 0; i < NO; ++i)
-                f.p[i] = *reinterpret_cast<const bf16x8*>(base + 2 * (((int64_t)i * rows + row) * l.vpad + 32 * vblk + 8 * q4));
+            for (int i = 0; i < NO; ++i) {
+                ap.p[i] = *reinterpret_cast<const bf16x8*>(Aw + 2 * (((int64_t)i * C + prow) * l.vpad + cc));
+                sp.p[i] = *reinterpret_cast<const bf16x8*>(Sw + 2 * (((int64_t)i * KP + srow) * l.vpad + cc));
+                dp.p[i] = *reinterpret_cast<const bf16x8*>(Dw + 2 * (((int64_t)i * KP + srow) * l.vpad + cc));
+            }
+            bp = load_raw8<WHOLE, T>(brow, cc, p.dv);
+        };
+        float yv = 0.f, ss = 0.f;   // this thread's part of Y.V (its token), of <S0, dS1>
+        auto value = [&](const Frag<NO>& f, int e) __attribute__((always_inline)) {
+            float x = 0.f;
+#pragma unroll
+            for (int i = NO - 1; i >= 0; --i) x += static_cast<float>(f.p[i][e]);
+            return x;
+        };
+        auto hand = [&](int vk) __attribute__((always_inline)) {
+            const int cc = 32 * vk + pcol;
+            const Raw8<T> b8 = clear<WHOLE, T>(bp, cc, p.dv, ok_p);
+            char* const at = (left ? Us : Ys) + prow * ROW + 2 * pcol;
+            char* const as = Ss + srow * ROW + 2 * pcol;
+#pragma unroll
+            for (int i = 0; i < NO; ++i) {
+                *reinterpret_cast<bf16x8*>(at + i * C * ROW) = ap.p[i];
+                if (has_s) {
+                    *reinterpret_cast<bf16x8*>(as + i * KP * ROW) = sp.p[i];
+                    *reinterpret_cast<bf16x8*>(as + (Ds - Ss) + i * KP * ROW) = dp.p[i];
+                }
+            }
+            if (has_s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss = fmaf(value(sp, e), value(dp, e), ss);
+            if (left) {
+                const Frag<NX> of = planes_of<T>(b8);
+#pragma unroll
+                for (int i = 0; i < NX; ++i) *reinterpret_cast<bf16x8*>(Os + (i * C + prow) * ROW + 2 * pcol) = of.p[i];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) yv = fmaf(value(ap, e), static_cast<float>(b8.v[e]), yv);
+            }
+        };
+        auto from = [&](const char* base, int rows, int row, auto planes) __attribute__((always_inline)) {
+            Frag<decltype(planes)::value> f;
+#pragma unroll
+            for (int i = 0; i < decltype(planes)::value; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + (i * rows + row) * ROW + 16 * q4);
             return f;
         };
-        auto out_rows = [&](int tok, int vblk) __attribute__((always_inline)) {
-            const int at = c * C + tok;
-            const bool ok = at < len;
-            const int cc = 32 * vblk + 8 * q4;
-            return planes_of<T>(clear<WHOLE, T>(load_raw8<WHOLE, T>(dob + (ok ? (int64_t)token(at, len, p.reverse) * a.q.dout_seq_stride : 0), cc, p.dv), cc, p.dv, ok));
-        };
-        // [j][i]: rows = another tile's tokens, columns (lanes) = this wave's tokens
-        f32x4 dm[4], zl[4];   // this wave's tokens as i, tiles j <= w: dO_i.U_j, Y_i.U_j
-        f32x4 mt[4], zr[4];   // this wave's tokens as j, tiles i >= w
-        f32x4 OS[DT], YS[DT], US[DT];
+        constexpr std::integral_constant<int, NO> no{};
+        constexpr std::integral_constant<int, NX> nx{};
+        // 64 x 64 products [j][i]: rows = another tile's tokens, columns (lanes) = this wave's.  left: m = dO_i.U_j, z = Y_i.U_j with this wave's tokens as i
+        // (tiles j <= w); right: with this wave's tokens as j (tiles i >= w).  A: left dO S0^T -> dQ, right U dS1^T -> X;  B: left Y S0^T -> W
+        f32x4 m[4], z[4], A[DT], B[DT];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) { dm[t] = zero; zl[t] = zero; mt[t] = zero; zr[t] = zero; }
+        for (int t = 0; t < 4; ++t) { m[t] = zero; z[t] = zero; }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) { OS[d] = zero; YS[d] = zero; US[d] = zero; }
-        float yv = 0.f, ss = 0.f;
-        for (int vk = 0; vk < l.vpad / 32; ++vk) {
-            const Frag<NO> yi = planes(Yw, C, own, vk), ui = planes(Uw, C, own, vk);
-            const Frag<NX> oi = out_rows(own, vk);
-            {
-                const int cc = 32 * vk + 8 * q4;
-                const Raw8<T> v = clear<WHOLE, T>(load_raw8<WHOLE, T>(vb + (ok_own ? (int64_t)token(at_own, len, p.reverse) * p.v_seq_stride : 0), cc, p.dv), cc, p.dv, ok_own);
+        for (int d = 0; d < DT; ++d) { A[d] = zero; B[d] = zero; }
+        auto multiply = [&]() __attribute__((always_inline)) {
+            if (left) {
+                const Frag<NO> yi = from(Ys, C, own, no);
+                const Frag<NX> oi = from(Os, C, own, nx);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float y = 0.f;
-#pragma unroll
-                    for (int i = NO - 1; i >= 0; --i) y += static_cast<float>(yi.p[i][e]);
-                    yv = fmaf(y, static_cast<float>(v.v[e]), yv);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (t <= w) {
-                    const Frag<NO> uj = planes(Uw, C, 16 * t + n, vk);
-                    mma<NO>(dm[t], uj, oi);
-                    mma<NO>(zl[t], uj, yi);
-                }
-                if (t >= w) {
-                    mma<NO>(mt[t], out_rows(16 * t + n, vk), ui);
-                    mma<NO>(zr[t], planes(Yw, C, 16 * t + n, vk), ui);
-                }
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const Frag<NO> s0 = planes(Sw, KP, 16 * d + n, vk), s1 = planes(Dw, KP, 16 * d + n, vk);
-                mma<NO>(OS[d], s0, oi);
-                mma<NO>(YS[d], s0, yi);
-                mma<NO>(US[d], s1, ui);
-                if ((d & 3) == w) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float x = 0.f, y = 0.f;
-#pragma unroll
-                        for (int i = NO - 1; i >= 0; --i) { x += static_cast<float>(s0.p[i][e]); y += static_cast<float>(s1.p[i][e]); }
-                        ss = fmaf(x, y, ss);
+                for (int t = 0; t < 4; ++t)
+                    if (t <= w) {
+                        const Frag<NO> uj = from(Us, C, 16 * t + n, no);
+                        mma<NO>(m[t], uj, oi);
+                        mma<NO>(z[t], uj, yi);
                     }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const Frag<NO> s0 = from(Ss, KP, 16 * d + n, no);
+                    mma<NO>(A[d], s0, oi);
+                    mma<NO>(B[d], s0, yi);
                 }
+            } else {
+                const Frag<NO> ui = from(Us, C, own, no);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (t >= w) {
+                        mma<NO>(m[t], from(Os, C, 16 * t + n, nx), ui);
+                        mma<NO>(z[t], from(Ys, C, 16 * t + n, no), ui);
+                    }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) mma<NO>(A[d], from(Ds, KP, 16 * d + n, no), ui);
             }
+        };
+        const int blocks = l.vpad / 32;
+        fetch(0);
+        for (int vk = 0; vk < blocks; ++vk) {
+            __syncthreads();   // LDS is free
+            hand(vk);
+            fetch(vk + 1 < blocks ? vk + 1 : vk);
+            __syncthreads();
+            multiply();
         }
-        __syncthreads();   // gates
-        const float gi = gs->gam[own], di = gs->del[own], bi = gs->bet[own];
+        Raw8<T> kr[PK], qr[PK];
+#pragma unroll
+        for (int i = 0; i < PK; ++i) {
+            const int id = tid + i * 512, row = id / (KP / 8), cc = 8 * (id % (KP / 8)), at = c * C + row;
+            kr[i] = load_raw8<WHOLE, T>(K.row(at < len ? at : len - 1), cc, p.dk);
+            qr[i] = load_raw8<WHOLE, T>(Q.row(at < len ? at : len - 1), cc, p.dk);
+        }
+        if (tid < (int)(sizeof(Gates) / 4))
+            reinterpret_cast<float*>(gs)[tid] = reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot)[tid];
+        yv += __shfl_xor(yv, 1);
+        yv += __shfl_xor(yv, 2);
+        if (!left && (tid & 3) == 0) yvs[prow] = yv;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PK; ++i) {
+            const int id = tid + i * 512, row = id / (KP / 8), cc = 8 * (id % (KP / 8));
+            const bool ok = c * C + row < len;
+            tile_put<KP, NX>(Ks, row, cc, planes_of<T>(clear<WHOLE, T>(kr[i], cc, p.dk, ok)));
+            tile_put<KP, NX>(Qs, row, cc, planes_of<T>(clear<WHOLE, T>(qr[i], cc, p.dk, ok)));
+        }
+        __syncthreads();
         const double Gi = gs->G[own];
-        float ku = 0.f;
         auto rowdot = [&](const char* tile, const f32x4 (&x)[DT]) __attribute__((always_inline)) {
             float s = 0.f;
 #pragma unroll
@@ -392,87 +453,105 @@ __global__ __launch_bounds__(256, 1) void gd_grad_kernel(const BwdArgs a) {
             }
             return s;
         };
+        // the 64 x 64 factors in the state's precision: dg is a difference of sums over pairs, which cancel only as far as the two
+        // roundings of a pair agree
+        if (left) {
+            const float gi = gs->gam[own], bi = gs->bet[own];
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                OS[d][e] *= p.scale * gi;
-                YS[d][e] *= gi;
-                US[d][e] *= di;
-            }
-        ku = rowdot(Ks, US);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int o = 16 * t + 4 * q4 + e;
-                const double Go = gs->G[o];
-                if (t <= w) {   // o = j
-                    const float L = o <= own ? L_of(Gi - Go) : 0.f;
-                    dm[t][e] *= p.scale * L;
-                    zl[t][e] = o < own ? L * zl[t][e] : 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    A[d][e] *= p.scale * gi;
+                    B[d][e] *= gi;
                 }
-                if (t >= w) {   // o = i
-                    const float L = o >= own ? L_of(Go - Gi) : 0.f;
-                    mt[t][e] *= p.scale * L;
-                    zr[t][e] = o > own ? -gs->bet[o] * L * zr[t][e] : 0.f;
-                }
-            }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            if (2 * kb <= w) {
-                const Frag<NS> fm = frag_of<NS>(dm[2 * kb], dm[2 * kb + 1]), fz = frag_of<NS>(zl[2 * kb], zl[2 * kb + 1]);
+            for (int t = 0; t < 4; ++t)
+                if (t <= w)
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const Frag<NX> kc = tile_cols<KP, NX>(Ks, d, kb, n, q4);
-                    mma<NS>(OS[d], kc, fm);
-                    mma<NS>(YS[d], kc, fz);
-                }
-            }
-            if (2 * kb + 1 >= w) {
-                const Frag<NS> fm = frag_of<NS>(mt[2 * kb], mt[2 * kb + 1]), fz = frag_of<NS>(zr[2 * kb], zr[2 * kb + 1]);
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = 16 * t + 4 * q4 + e;
+                        const float L = j <= own ? L_of(Gi - gs->G[j]) : 0.f;
+                        m[t][e] *= p.scale * L;
+                        z[t][e] = j < own ? L * z[t][e] : 0.f;
+                    }
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    mma<NS>(US[d], tile_cols<KP, NX>(Qs, d, kb, n, q4), fm);
-                    mma<NS>(US[d], tile_cols<KP, NX>(Ks, d, kb, n, q4), fz);
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb <= w) {
+                    const Frag<NS> fm = frag_of<NS>(m[2 * kb], m[2 * kb + 1]), fz = frag_of<NS>(z[2 * kb], z[2 * kb + 1]);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const Frag<NX> kc = tile_cols<KP, NX>(Ks, d, kb, n, q4);
+                        mma<NS>(A[d], kc, fm);
+                        mma<NS>(B[d], kc, fz);
+                    }
                 }
+            const float qd = quarters_sum(rowdot(Qs, A)), kw = quarters_sum(rowdot(Ks, B));
+#pragma unroll
+            for (int d = 0; d < DT; ++d) Wx[(w * DT + d) * 64 + lane] = B[d] * bi;
+            if (q4 == 0) {
+                dGs[own] = qd - bi * kw;
+                if (ok_own) st_gate(a.q.dbeta, ((int64_t)b * p.seqlen + token(at_own, len, p.reverse)) * p.heads + h, p.gate_dtype, yvs[own] - kw);
             }
+        } else {
+            const float di = gs->del[own];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) A[d] *= di;
+            ss = fmaf(gs->gam[C - 1], ss, rowdot(Ks, A));   // + the state's own part, below
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t >= w)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 16 * t + 4 * q4 + e;
+                        const float L = i >= own ? L_of(gs->G[i] - Gi) : 0.f;
+                        m[t][e] *= p.scale * L;
+                        z[t][e] = i > own ? -gs->bet[i] * L * z[t][e] : 0.f;
+                    }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb + 1 >= w) {
+                    const Frag<NS> fm = frag_of<NS>(m[2 * kb], m[2 * kb + 1]), fz = frag_of<NS>(z[2 * kb], z[2 * kb + 1]);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        mma<NS>(A[d], tile_cols<KP, NX>(Qs, d, kb, n, q4), fm);
+                        mma<NS>(A[d], tile_cols<KP, NX>(Ks, d, kb, n, q4), fz);
+                    }
+                }
+            const float kx = quarters_sum(rowdot(Ks, A));
+            if (q4 == 0) kxs[own] = kx;
         }
-        const float qd = quarters_sum(rowdot(Qs, OS)), kw = quarters_sum(rowdot(Ks, YS)), kx = quarters_sum(rowdot(Ks, US));
-        yv = quarters_sum(yv);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dqs[d][e] += OS[d][e];
-                dks[d][e] += US[d][e] - bi * YS[d][e];
-            }
-        const int64_t gate_at = ok_own ? ((int64_t)b * p.seqlen + token(at_own, len, p.reverse)) * p.heads + h : 0;
-        if (q4 == 0) {
-            dGs[own] = qd - bi * kw - kx;
-            if (ok_own) st_gate(a.q.dbeta, gate_at, p.gate_dtype, yv - kw);
-        }
-        ss = wave_sum(gs->gam[C - 1] * ss + ku);
-        if (lane == 0) part[w] = ss;
+        ss = wave_sum(left ? gs->gam[C - 1] * ss : ss);
+        if (lane == 0) part[w8] = ss;
         __syncthreads();
-        if (w == 0) {   // lane = token
-            float x = dGs[lane];
+        if (w8 == 0) {   // lane = token
+            float x = dGs[lane] - kxs[lane];
 #pragma unroll
             for (int s = 1; s < 64; s *= 2) {
                 const float o = __shfl_down(x, s);
                 if (lane + s < 64) x += o;
             }
-            x += part[0] + part[1] + part[2] + part[3];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x += part[i];
             const int at = c * C + lane;
             if (at < len) st_gate(a.q.dg, ((int64_t)b * p.seqlen + token(at, len, p.reverse)) * p.heads + h, p.gate_dtype, x);
         }
-    }
-    if (ok_own) {
-        const int64_t t = token(at_own, len, p.reverse);
+        if (!left)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            store4<T>(dqb + t * dk_seq, 16 * d + 4 * q4, p.dk, dqs[d]);
-            store4<T>(dkb + t * dk_seq, 16 * d + 4 * q4, p.dk, dks[d]);
+            for (int d = 0; d < DT; ++d) A[d] -= Wx[(w * DT + d) * 64 + lane];   // dK
+        if constexpr (SHARED) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) total[d] += A[d];
+        } else if (ok_own) {
+            T* const row = (left ? dqb : dkb) + token(at_own, len, p.reverse) * dk_seq;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) store4<T>(row, 16 * d + 4 * q4, p.dk, A[d]);
+        }
+    }
+    if constexpr (SHARED) {
+        if (ok_own) {
+            T* const row = (left ? dqb : dkb) + token(at_own, len, p.reverse) * dk_seq;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) store4<T>(row, 16 * d + 4 * q4, p.dk, total[d]);
         }
     }
 }
@@ -491,12 +570,15 @@ static int bwd_scan_launch(const BwdArgs& a, hipStream_t s) {
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-template <typename T, int KP, bool WHOLE>
+template <typename T, int KP, bool WHOLE, bool SHARED>
 static int grad_launch(const BwdArgs& a, hipStream_t s) {
-    constexpr int lds = 2 * Prec<T>::NX * tile_bytes<KP>() + (int)sizeof(Gates) + (C + 4) * 4;
+    constexpr int NX = Prec<T>::NX, NO = Prec<T>::NO;
+    constexpr int one = (2 * NO + NX) * C * 80 + 2 * NO * KP * 80, two = 2 * NX * tile_bytes<KP>() + C * KP * 4;
+    constexpr int lds = (int)sizeof(Gates) + (3 * C + 8) * 4 + (one > two ? one : two);
+    static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_grad_kernel<T, KP, WHOLE>), lds)) return rc;
-    hipLaunchKernelGGL((gd_grad_kernel<T, KP, WHOLE>), dim3(a.l.chunks, a.q.f.heads_k, a.q.f.batch), dim3(256), lds, s, a);
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_grad_kernel<T, KP, WHOLE, SHARED>), lds)) return rc;
+    hipLaunchKernelGGL((gd_grad_kernel<T, KP, WHOLE, SHARED>), dim3(a.l.chunks, a.q.f.heads_k, a.q.f.batch), dim3(512), lds, s, a);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
@@ -506,7 +588,8 @@ static int bwd_launch(const BwdArgs& a, hipStream_t s) {
     const int fit = fit_of(a.q.f.dk, a.q.f.dv);
     const int rc = fit == 2 ? bwd_scan_launch<T, KP, kCT, 2>(a, s) : fit == 1 ? bwd_scan_launch<T, KP, kCT, 1>(a, s) : bwd_scan_launch<T, KP, kCT, 0>(a, s);
     if (rc) return rc;
-    return fit ? grad_launch<T, KP, true>(a, s) : grad_launch<T, KP, false>(a, s);
+    if (a.q.f.heads == a.q.f.heads_k) return fit ? grad_launch<T, KP, true, false>(a, s) : grad_launch<T, KP, false, false>(a, s);
+    return fit ? grad_launch<T, KP, true, true>(a, s) : grad_launch<T, KP, false, true>(a, s);
 }
 template <typename T>
 static int bwd_type(const BwdArgs& a, hipStream_t s) {
