@@ -402,6 +402,11 @@ __device__ __forceinline__ void store_cols(T* row, int c, int n, const f32x4 (&v
     }
 }
 
+// A walk's workgroup takes 32 columns of a head, or 16 where that leaves half of the CUs without one: a chunk of 16 columns takes 0.7 .. 0.9 of the time of one of
+// 32 (its chain is the same).  (2, 2304, 8 heads, 64 x 64): 32 workgroups 65 us, 64 workgroups 50 us; (8, 8192, 8 heads, 128 x 128): 256 workgroups
+// 356 us, 512 workgroups 464 us.
+inline bool narrow(const vms_gated_delta_params& p, const Layout& l) { return (int64_t)p.batch * p.heads * (l.vpad / 32) <= device_cu_count() / 2; }
+
 int validate(const vms_gated_delta_params& p);   // gated_delta_fwd.hip
 
 }  // namespace gd

@@ -570,6 +570,10 @@ static int bwd_scan_launch(const BwdArgs& a, hipStream_t s) {
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
+template <typename T, int KP, int CT>
+static int bwd_scan_fit(const BwdArgs& a, int fit, hipStream_t s) {
+    return fit == 2 ? bwd_scan_launch<T, KP, CT, 2>(a, s) : fit == 1 ? bwd_scan_launch<T, KP, CT, 1>(a, s) : bwd_scan_launch<T, KP, CT, 0>(a, s);
+}
 template <typename T, int KP, bool WHOLE, bool SHARED>
 static int grad_launch(const BwdArgs& a, hipStream_t s) {
     constexpr int NX = Prec<T>::NX, NO = Prec<T>::NO;
@@ -584,9 +588,12 @@ static int grad_launch(const BwdArgs& a, hipStream_t s) {
 }
 template <typename T, int KP>
 static int bwd_launch(const BwdArgs& a, hipStream_t s) {
-    constexpr int kCT = sizeof(T) == 4 ? 1 : 2;   // column tiles of a workgroup: fp32's six planes of K and Q leave LDS for one
     const int fit = fit_of(a.q.f.dk, a.q.f.dv);
-    const int rc = fit == 2 ? bwd_scan_launch<T, KP, kCT, 2>(a, s) : fit == 1 ? bwd_scan_launch<T, KP, kCT, 1>(a, s) : bwd_scan_launch<T, KP, kCT, 0>(a, s);
+    int rc;
+    if constexpr (sizeof(T) == 4)   // (fp32: the six planes of K and Q leave LDS for one column tile)
+        rc = bwd_scan_fit<T, KP, 1>(a, fit, s);
+    else
+        rc = narrow(a.q.f, a.l) ? bwd_scan_fit<T, KP, 1>(a, fit, s) : bwd_scan_fit<T, KP, 2>(a, fit, s);
     if (rc) return rc;
     if (a.q.f.heads == a.q.f.heads_k) return fit ? grad_launch<T, KP, true, false>(a, s) : grad_launch<T, KP, false, false>(a, s);
     return fit ? grad_launch<T, KP, true, true>(a, s) : grad_launch<T, KP, false, true>(a, s);

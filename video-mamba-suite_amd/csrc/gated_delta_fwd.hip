@@ -457,17 +457,14 @@ static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStre
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-#ifndef VMS_GD_CT
-#define VMS_GD_CT 2
-#endif
-constexpr int kCT = VMS_GD_CT;
 template <typename T, int KP, int FIT>
 static int fwd_launch(const vms_gated_delta_params& p, hipStream_t s) {
     const Layout l = layout(p);
     const dim3 grid(l.chunks, p.heads, p.batch);
     hipLaunchKernelGGL((gd_prep_kernel<T, KP, FIT>), grid, dim3(64), 0, s, p, l);
     VMS_LAUNCH_CHECK();
-    return p.for_backward ? scan_launch<T, KP, kCT, FIT, true>(p, l, s) : scan_launch<T, KP, kCT, FIT, false>(p, l, s);
+    if (narrow(p, l)) return p.for_backward ? scan_launch<T, KP, 1, FIT, true>(p, l, s) : scan_launch<T, KP, 1, FIT, false>(p, l, s);
+    return p.for_backward ? scan_launch<T, KP, 2, FIT, true>(p, l, s) : scan_launch<T, KP, 2, FIT, false>(p, l, s);
 }
 template <typename T, int KP>
 static int fwd_fit(const vms_gated_delta_params& p, hipStream_t s) {
