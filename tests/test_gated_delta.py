@@ -380,3 +380,31 @@ def test_on_another_stream_and_captured():
             o = gated_delta_rule_fn(**half)
             assert torch.equal(out, o)
             assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(o, list(half.values()), dout)))
+
+
+@pytest.mark.gpu
+def test_compiled_and_ctypes_calls_are_one(monkeypatch):
+    """the compiled binding's node and the ctypes one: the same bits, the same refusals, and no second derivative in either"""
+    import vms_hip
+    ext = vms_hip.ext()
+    assert ext is not None
+    t = inputs(2, 100, 1, 2, 40, 48, torch.bfloat16, state=True)
+    lens = torch.tensor([100, 31], device="cuda")
+    dout = torch.randn_like(t["v"])
+    runs = []
+    for use in (ext, None):
+        monkeypatch.setattr(vms_hip, "_ext", use)
+        leaf = {k: v.clone().requires_grad_() for k, v in t.items()}
+        out, s = gated_delta_rule_fn(**leaf, return_final_state=True, reverse=True, seq_lens=lens)
+        runs.append([out, s, *torch.autograd.grad((out, s), list(leaf.values()), (dout, s.detach()))])
+        with torch.no_grad():
+            runs[-1].append(gated_delta_rule_fn(**leaf, scale=0.5))
+        leaf = {k: v.float().requires_grad_() for k, v in t.items()}
+        g, = torch.autograd.grad(gated_delta_rule_fn(**leaf).square().sum(), leaf["v"], create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+        for bad in ({"q": t["q"][..., :3]}, {"k": t["k"].float()}, {"beta": t["beta"].half()}, {"initial_state": t["initial_state"].half()},
+                    {"seq_lens": lens.float()}, {"seq_lens": lens[:1]}, {"g": t["g"].cpu()}):
+            with pytest.raises(RuntimeError, match="gated_delta_rule"):
+                gated_delta_rule_fn(**{**t, **bad})
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -150,3 +150,22 @@ def test_prompt_then_steps(dtype):
     rest = [gated_delta_state_update(state, **{k: v[:, i] for k, v in t.items()}) for i in range(75, 90)]
     close(torch.cat([out, torch.stack(rest, 1)], 1), whole, 2 * TOL[dtype])
     close(state, final, 4e-4 if dtype != torch.float32 else 4e-5)
+
+
+@pytest.mark.gpu
+def test_compiled_and_ctypes_steps_are_one(monkeypatch):
+    import vms_hip
+    ext = vms_hip.ext()
+    assert ext is not None
+    state, t = step_inputs(2, 2, 4, 40, 48, torch.float16, torch.float16)
+    runs = []
+    for use in (ext, None):
+        monkeypatch.setattr(vms_hip, "_ext", use)
+        s = state.clone()
+        version = s._version
+        runs.append([gated_delta_state_update(s, **t), s, gated_delta_state_update(s.clone(), **t, scale=0.25)])
+        assert s._version > version   # autograd sees the update
+        for bad in (state.transpose(2, 3), state[:1].expand(2, -1, -1, -1), state.double(), state.cpu()):
+            with pytest.raises(RuntimeError, match="gated_delta_rule"):
+                gated_delta_state_update(bad, **t)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -278,3 +278,23 @@ def test_a_block_of_them():
     for name, a, b_ in zip(["y", "s", *w], got, want):
         # padded tokens have a zero block output: 1 / deviation = 1000 there, which multiplies what the fp32 products leave
         close(a, b_, 4e-4, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "channel", "ones", "batch", "token"])
+def test_compiled_and_ctypes_calls_are_one(gate, monkeypatch):
+    import vms_hip
+    ext = vms_hip.ext()
+    assert ext is not None
+    t = make((3, 20, 136), torch.bfloat16, torch.float32, gate=gate, gate_dtype=torch.float16, weight_dtype=torch.bfloat16)
+    runs = []
+    for use in (ext, None):
+        monkeypatch.setattr(vms_hip, "_ext", use)
+        leaf = {k: v.clone().requires_grad_() for k, v in t.items()}
+        y, s = sandwich_norm_fn(**leaf, residual_scale=0.6)
+        runs.append([y, s, *torch.autograd.grad((y, s), list(leaf.values()), (t["x"], s.detach()))])
+        runs[-1] += [*sandwich_norm_fn(**{**t, "residual": None}, is_rms_norm=True)]
+        g, = torch.autograd.grad(sandwich_norm_fn(**leaf)[1].square().sum(), leaf["x"], create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.float().sum().backward()
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(*runs))

@@ -12,8 +12,11 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <atomic>
+#include <cmath>
 #include <limits>
 #include <mutex>
 #include <string>
@@ -955,6 +958,287 @@ std::vector<std::tuple<std::string, double>> timing_stop() {
     return out;
 }
 
+// ---- gated delta rule, single-token step, norms around a block: checks, allocations and autograd nodes ---------------
+// The same calls as mamba_ssm/ops/gated_delta_rule.py and ops/triton/layernorm.py make through ctypes, message for message; a node in C++
+// costs ~10 us of host time each way instead of ~80 (what (2, 2304, 512) training steps wait for).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+Tensor unit_last(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+bool tracked(std::initializer_list<Tensor> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor& t : ts)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+// gradients of a node that is differentiable once: a second derivative raises instead of being zero
+variable_list once(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    std::vector<size_t> at;
+    variable_list in;
+    for (size_t i = 0; i < grads.size(); ++i)
+        if (grads[i].defined()) {
+            at.push_back(i);
+            in.push_back(grads[i]);
+            in.back().set_requires_grad(true);
+        }
+    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", in.size());
+    variable_list out = (*error)(std::move(in));
+    for (size_t i = 0; i < at.size(); ++i) grads[at[i]] = out[i];
+    return grads;
+}
+
+#define GD_CHECK(cond, msg) TORCH_CHECK(cond, "gated_delta_rule: " msg)
+void gated_delta_checks(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, int64_t lead) {
+    GD_CHECK(q.sizes() == k.sizes() && q.dim() == lead + 2 && v.dim() == lead + 2, "q, k (..., heads_k, dk) and v (..., heads, dv) expected");
+    GD_CHECK(q.sizes().slice(0, lead) == v.sizes().slice(0, lead), "q, k and v must agree in batch and length");
+    GD_CHECK(k.size(lead) > 0 && v.size(lead) % k.size(lead) == 0, "the heads of v must be a multiple of the heads of q and k");
+    GD_CHECK(g.sizes() == v.sizes().slice(0, lead + 1) && beta.sizes() == g.sizes(), "g and beta must have the shape of v without its last axis");
+    GD_CHECK(k.size(-1) >= 1 && k.size(-1) <= 128, "key heads of 1 to 128 are supported");
+    GD_CHECK(v.size(-1) >= 1 && v.size(-1) <= 4096, "value heads of 1 to 4096 are supported");
+    GD_CHECK(q.scalar_type() == v.scalar_type() && k.scalar_type() == v.scalar_type(), "q, k and v must have one dtype");
+    GD_CHECK(is_itype(v), "fp32, fp16 or bf16 expected");
+    GD_CHECK(g.scalar_type() == beta.scalar_type() && (g.scalar_type() == v.scalar_type() || g.scalar_type() == at::kFloat),
+             "g and beta must have one dtype: fp32 or that of v");
+    for (const Tensor* t : {&q, &k, &g, &beta}) GD_CHECK(t->device() == v.device(), "all tensors must be on one device");
+}
+
+void gated_delta_fill(vms_gated_delta_params& p, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale,
+                      const Tensor& seq_lens, bool reverse, bool for_backward) {
+    p.batch = v.size(0); p.seqlen = v.size(1); p.heads = v.size(2); p.dv = v.size(3);
+    p.heads_k = k.size(2); p.dk = k.size(3);
+    p.dtype = dtype_code(v); p.gate_dtype = dtype_code(g);
+    p.reverse = reverse; p.for_backward = for_backward; p.scale = (float)scale;
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.g = g.data_ptr(); p.beta = beta.data_ptr();
+    p.seq_lens = seq_lens.defined() ? static_cast<const int32_t*>(seq_lens.data_ptr()) : nullptr;
+    p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_head_stride = q.stride(2);
+    p.k_batch_stride = k.stride(0); p.k_seq_stride = k.stride(1); p.k_head_stride = k.stride(2);
+    p.v_batch_stride = v.stride(0); p.v_seq_stride = v.stride(1); p.v_head_stride = v.stride(2);
+    p.g_batch_stride = g.stride(0); p.g_seq_stride = g.stride(1); p.g_head_stride = g.stride(2);
+    p.beta_batch_stride = beta.stride(0); p.beta_seq_stride = beta.stride(1); p.beta_head_stride = beta.stride(2);
+}
+Tensor bytes_like(const Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
+
+struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g, const Tensor& beta,
+                                 const OptT& initial_state, double scale, bool reverse, const OptT& seq_lens_, bool want_final, bool for_backward) {
+        const Tensor q = unit_last(q_), k = unit_last(k_), v = unit_last(v_);
+        const Tensor seq_lens = seq_lens_.has_value() ? *seq_lens_ : Tensor();
+        c10::DeviceGuard guard(v.device());
+        Tensor out = at::empty(v.sizes(), v.options());
+        const auto f32 = v.options().dtype(at::kFloat);
+        Tensor fin = want_final ? at::empty({v.size(0), v.size(2), k.size(3), v.size(3)}, f32) : Tensor();
+        const Tensor s0 = initial_state.has_value() ? initial_state->contiguous() : Tensor();
+        vms_gated_delta_params p{};
+        gated_delta_fill(p, q, k, v, g, beta, scale, seq_lens, reverse, for_backward);
+        p.initial_state = s0.defined() ? s0.data_ptr<float>() : nullptr;
+        p.final_state = fin.defined() ? fin.data_ptr<float>() : nullptr;
+        p.out = out.data_ptr();
+        p.out_batch_stride = out.stride(0); p.out_seq_stride = out.stride(1); p.out_head_stride = out.stride(2);
+        const Tensor ws = bytes_like(v, vms_gated_delta_workspace_bytes(&p));
+        p.workspace = ws.data_ptr(); p.workspace_bytes = ws.numel();
+        call("vms_gated_delta_fwd", vms_gated_delta_fwd, p, v);
+        if (for_backward) {
+            ctx->save_for_backward({q, k, v, g, beta, seq_lens, ws});
+            ctx->saved_data["scale"] = scale;
+            ctx->saved_data["reverse"] = reverse;
+            ctx->saved_data["state"] = initial_state.has_value();
+            ctx->set_materialize_grads(false);
+        }
+        return want_final ? variable_list{out, fin} : variable_list{out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &beta = saved[4], &seq_lens = saved[5], &ws = saved[6];
+        c10::DeviceGuard guard(v.device());
+        variable_list r(11);
+        {
+            at::NoGradGuard no_grad;
+            const Tensor dout = grads[0].defined() ? unit_last(grads[0].to(v.scalar_type())) : at::zeros(v.sizes(), v.options());
+            const Tensor dfin = grads.size() > 1 && grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : Tensor();
+            vms_gated_delta_bwd_params b{};
+            gated_delta_fill(b.f, q, k, v, g, beta, ctx->saved_data["scale"].toDouble(), seq_lens, ctx->saved_data["reverse"].toBool(), true);
+            b.f.workspace = ws.data_ptr(); b.f.workspace_bytes = ws.numel();
+            r[0] = at::empty(q.sizes(), q.options());
+            r[1] = at::empty(k.sizes(), k.options());
+            r[2] = at::empty(v.sizes(), v.options());
+            r[3] = at::empty(g.sizes(), g.options());
+            r[4] = at::empty(beta.sizes(), beta.options());
+            if (ctx->saved_data["state"].toBool()) r[5] = at::empty({v.size(0), v.size(2), k.size(3), v.size(3)}, v.options().dtype(at::kFloat));
+            b.dout = dout.data_ptr();
+            b.dout_batch_stride = dout.stride(0); b.dout_seq_stride = dout.stride(1); b.dout_head_stride = dout.stride(2);
+            b.dfinal_state = dfin.defined() ? dfin.data_ptr<float>() : nullptr;
+            b.dinitial_state = r[5].defined() ? r[5].data_ptr<float>() : nullptr;
+            b.dq = r[0].data_ptr(); b.dk = r[1].data_ptr(); b.dv = r[2].data_ptr(); b.dg = r[3].data_ptr(); b.dbeta = r[4].data_ptr();
+            const Tensor own = bytes_like(v, vms_gated_delta_bwd_workspace_bytes(&b.f));
+            b.workspace = own.data_ptr(); b.workspace_bytes = own.numel();
+            call("vms_gated_delta_bwd", vms_gated_delta_bwd, b, v);
+        }
+        return once(std::move(r));
+    }
+};
+
+std::vector<Tensor> gated_delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, c10::optional<double> scale,
+                                     const OptT& initial_state, bool want_final, bool reverse, OptT seq_lens) {
+    gated_delta_checks(q, k, v, g, beta, 2);
+    const int64_t batch = v.size(0);
+    if (initial_state.has_value())
+        GD_CHECK(initial_state->sizes() == at::IntArrayRef({batch, v.size(2), k.size(3), v.size(3)}) && initial_state->scalar_type() == at::kFloat &&
+                     initial_state->device() == v.device(),
+                 "initial_state must be fp32 (batch, heads, dk, dv) on the device of v");
+    GD_CHECK(v.is_cuda(), "tensors must be on a GPU (no CPU path in this library)");
+    if (seq_lens.has_value()) {
+        GD_CHECK(seq_lens->dim() == 1 && seq_lens->size(0) == batch && seq_lens->device() == v.device() &&
+                     (seq_lens->scalar_type() == at::kInt || seq_lens->scalar_type() == at::kLong),
+                 "seq_lens must be int32 or int64 (batch,) on the device of v");
+        if (seq_lens->scalar_type() == at::kLong) seq_lens = seq_lens->clamp(0, v.size(1)).to(at::kInt);   // clamped before the narrowing
+        seq_lens = seq_lens->contiguous();
+    }
+    const bool grad = tracked({q, k, v, g, beta, initial_state.has_value() ? *initial_state : Tensor()});
+    return GatedDeltaFn::apply(q, k, v, g, beta, initial_state, scale.has_value() ? *scale : 1.0 / std::sqrt((double)k.size(3)), reverse, seq_lens, want_final, grad);
+}
+
+bool separate_states(const Tensor& s) {
+    const int64_t dk = s.size(2), dv = s.size(3);
+    if (!(dv == 1 || s.stride(3) == 1) || !(dk == 1 || s.stride(2) == dv)) return false;
+    int64_t least = dk * dv;
+    const int lo = s.stride(0) < s.stride(1) ? 0 : 1;
+    for (int i : {lo, 1 - lo})
+        if (s.size(i) > 1) {
+            if (s.stride(i) < least) return false;
+            least = s.stride(i) * s.size(i);
+        }
+    return true;
+}
+Tensor gated_delta_state_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g, const Tensor& beta,
+                                c10::optional<double> scale) {
+    gated_delta_checks(q_, k_, v_, g, beta, 1);
+    GD_CHECK(state.dim() == 4 && state.sizes() == at::IntArrayRef({v_.size(0), v_.size(1), k_.size(2), v_.size(2)}), "state must be (batch, heads, dk, dv)");
+    GD_CHECK(is_itype(state) && state.device() == v_.device(), "state must be fp32, fp16 or bf16 on the device of v");
+    GD_CHECK(separate_states(state), "the (dk, dv) states must be contiguous and must not overlap: they are updated in place");
+    GD_CHECK(!tracked({state, q_, k_, v_, g, beta}), "the single-token step has no gradient: call it under torch.no_grad(), or gated_delta_rule_fn");
+    GD_CHECK(v_.is_cuda(), "tensors must be on a GPU (no CPU path in this library)");
+    const Tensor q = unit_last(q_), k = unit_last(k_), v = unit_last(v_);
+    c10::DeviceGuard guard(v.device());
+    Tensor out = at::empty(v.sizes(), v.options());
+    if (v.numel() == 0) return out;
+    vms_gated_delta_step_params p{};
+    p.batch = v.size(0); p.heads = v.size(1); p.heads_k = k.size(1); p.dk = k.size(2); p.dv = v.size(2);
+    p.state_dtype = dtype_code(state); p.dtype = dtype_code(v); p.gate_dtype = dtype_code(g);
+    p.scale = scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)k.size(2)));
+    p.state = state.data_ptr(); p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.g = g.data_ptr(); p.beta = beta.data_ptr(); p.out = out.data_ptr();
+    p.state_batch_stride = state.stride(0); p.state_head_stride = state.stride(1);
+    p.q_batch_stride = q.stride(0); p.q_head_stride = q.stride(1);
+    p.k_batch_stride = k.stride(0); p.k_head_stride = k.stride(1);
+    p.v_batch_stride = v.stride(0); p.v_head_stride = v.stride(1);
+    p.out_batch_stride = out.stride(0); p.out_head_stride = out.stride(1);
+    p.g_batch_stride = g.stride(0); p.g_head_stride = g.stride(1);
+    p.beta_batch_stride = beta.stride(0); p.beta_head_stride = beta.stride(1);
+    call("vms_gated_delta_state_update", vms_gated_delta_state_update, p, v);
+    state.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
+Tensor flat_rows(const Tensor& t) {
+    const Tensor t2 = t.reshape({-1, t.size(-1)});
+    return unit_last(t2);
+}
+void sandwich_fill(vms_sandwich_norm_params& p, const Tensor& x, const Tensor& residual, const Tensor& gate, int64_t rows_per_gate, const Tensor* par,
+                   at::ScalarType stream, double residual_scale, double eps, bool rms, const Tensor& stats) {
+    p.rows = x.size(0); p.cols = x.size(1);
+    p.x_dtype = dtype_code(x); p.res_dtype = stream == at::kFloat ? VMS_F32 : p.x_dtype; p.is_rms = rms;
+    p.eps = (float)eps; p.residual_scale = (float)residual_scale;
+    auto f = [](const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+    p.x = x.data_ptr(); p.x_row_stride = x.stride(0);
+    if (residual.defined()) { p.residual = residual.data_ptr(); p.residual_row_stride = residual.stride(0); }
+    if (gate.defined()) { p.gate = gate.data_ptr(); p.gate_dtype = dtype_code(gate); p.rows_per_gate = rows_per_gate; p.gate_row_stride = gate.stride(0); }
+    p.post_weight = f(par[0]); p.post_bias = f(par[1]); p.pre_weight = f(par[2]); p.pre_bias = f(par[3]);
+    p.stats = f(stats);
+}
+
+struct SandwichNormFn : public torch::autograd::Function<SandwichNormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x_, const OptT& residual_, const Tensor& post_w, const Tensor& pre_w, const OptT& post_b,
+                                 const OptT& pre_b, const OptT& gate_, int64_t rows_per_gate, double residual_scale, bool stream32, double eps, bool rms, bool for_backward) {
+        c10::DeviceGuard guard(x_.device());
+        const Tensor x = flat_rows(x_), residual = residual_.has_value() ? flat_rows(*residual_) : Tensor(), gate = gate_.has_value() ? flat_rows(*gate_) : Tensor();
+        auto f32 = [](const OptT& t) { return t.has_value() && t->defined() ? t->to(at::kFloat).contiguous() : Tensor(); };
+        const Tensor par[4] = {f32(post_w), f32(post_b), f32(pre_w), f32(pre_b)};
+        const at::ScalarType stream = stream32 ? at::kFloat : x.scalar_type();
+        Tensor y = at::empty(x_.sizes(), x.options()), out = at::empty(x_.sizes(), x.options().dtype(stream));
+        const Tensor stats = for_backward ? at::empty({x.size(0), 4}, x.options().dtype(at::kFloat)) : Tensor();
+        vms_sandwich_norm_params p{};
+        sandwich_fill(p, x, residual, gate, rows_per_gate, par, stream, residual_scale, eps, rms, stats);
+        p.y = y.data_ptr(); p.residual_out = out.data_ptr();
+        p.y_row_stride = p.residual_out_row_stride = x.size(1);
+        call("vms_sandwich_norm_fwd", vms_sandwich_norm_fwd, p, x);
+        if (for_backward) {
+            ctx->save_for_backward({x, residual, gate, par[0], par[1], par[2], par[3], stats});
+            ctx->saved_data["shape"] = x_.sizes().vec();
+            ctx->saved_data["gate_shape"] = gate_.has_value() ? gate_->sizes().vec() : std::vector<int64_t>{};
+            ctx->saved_data["rows_per_gate"] = rows_per_gate;
+            ctx->saved_data["residual_scale"] = residual_scale;
+            ctx->saved_data["stream32"] = stream32;
+            ctx->saved_data["eps"] = eps;
+            ctx->saved_data["rms"] = rms;
+            auto code = [](const OptT& t) { return t.has_value() ? (int64_t)t->scalar_type() : (int64_t)at::kFloat; };
+            ctx->saved_data["types"] = std::vector<int64_t>{code(post_w), code(post_b), code(pre_w), code(pre_b)};
+            ctx->set_materialize_grads(false);
+        }
+        return {y, out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &residual = saved[1], &gate = saved[2], &stats = saved[7];
+        const Tensor par[4] = {saved[3], saved[4], saved[5], saved[6]};
+        c10::DeviceGuard guard(x.device());
+        variable_list r(13);
+        {
+            at::NoGradGuard no_grad;
+            const at::ScalarType stream = ctx->saved_data["stream32"].toBool() ? at::kFloat : x.scalar_type();
+            const auto shape = ctx->saved_data["shape"].toIntVector(), gate_shape = ctx->saved_data["gate_shape"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+            const Tensor dy = grads[0].defined() ? flat_rows(grads[0].to(x.scalar_type())) : Tensor();
+            const Tensor dout = grads[1].defined() ? flat_rows(grads[1].to(stream)) : Tensor();
+            vms_sandwich_norm_bwd_params b{};
+            sandwich_fill(b.f, x, residual, gate, ctx->saved_data["rows_per_gate"].toInt(), par, stream, ctx->saved_data["residual_scale"].toDouble(),
+                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool(), stats);
+            r[0] = at::empty(shape, x.options());
+            b.dx = r[0].data_ptr(); b.dx_row_stride = x.size(1);
+            if (residual.defined()) {
+                r[1] = at::empty(shape, residual.options());
+                b.dresidual = r[1].data_ptr(); b.dresidual_row_stride = x.size(1);
+            }
+            if (gate.defined()) {
+                r[6] = at::empty(gate_shape, gate.options());
+                b.dgate = r[6].data_ptr();
+            }
+            Tensor d[4];
+            float* at4[4] = {};
+            for (int i = 0; i < 4; ++i)
+                if (par[i].defined()) {
+                    d[i] = at::empty({x.size(1)}, x.options().dtype(at::kFloat));
+                    at4[i] = d[i].data_ptr<float>();
+                }
+            b.dpost_weight = at4[0]; b.dpost_bias = at4[1]; b.dpre_weight = at4[2]; b.dpre_bias = at4[3];
+            if (dy.defined()) { b.dy = dy.data_ptr(); b.dy_row_stride = dy.stride(0); }
+            if (dout.defined()) { b.dresidual_out = dout.data_ptr(); b.dresidual_out_row_stride = dout.stride(0); }
+            const Tensor ws = bytes_like(x, vms_sandwich_norm_bwd_workspace_bytes(&b.f));
+            b.workspace = ws.data_ptr(); b.workspace_bytes = ws.numel();
+            call("vms_sandwich_norm_bwd", vms_sandwich_norm_bwd, b, x);
+            const int slot[4] = {2, 4, 3, 5};   // post_weight, post_bias, pre_weight, pre_bias among the inputs
+            for (int i = 0; i < 4; ++i)
+                if (d[i].defined()) r[slot[i]] = d[i].to((at::ScalarType)types[i]);
+        }
+        return once(std::move(r));
+    }
+};
+
+std::vector<Tensor> sandwich_norm(const Tensor& x, const OptT& residual, const Tensor& post_w, const Tensor& pre_w, const OptT& post_b, const OptT& pre_b,
+                                  const OptT& gate, int64_t rows_per_gate, double residual_scale, bool stream32, double eps, bool rms) {
+    auto of = [](const OptT& t) { return t.has_value() ? *t : Tensor(); };
+    const bool grad = tracked({x, of(residual), post_w, pre_w, of(post_b), of(pre_b), of(gate)});
+    return SandwichNormFn::apply(x, residual, post_w, pre_w, post_b, pre_b, gate, rows_per_gate, residual_scale, stream32, eps, rms, grad);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -982,6 +1266,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("inner_bwd", &inner_bwd);
     m.def("inner_bwd_dual", &inner_bwd_dual);
     m.def("scan_bwd_dual", &scan_bwd_dual);
+    m.def("gated_delta_rule", &gated_delta_rule);
+    m.def("gated_delta_state_update", &gated_delta_state_update);
+    m.def("sandwich_norm", &sandwich_norm);
     m.def("timing_start", &timing_start, pybind11::arg("reserve") = 0, pybind11::arg("only") = "");
     m.def("timing_stop", &timing_stop);
     m.def("timing_stop_detail", &timing_stop_detail);   // + the kernel each launch chose (tools/suite_shapes.py)

@@ -38,6 +38,12 @@ def _check_gpu(v):
     _check(v.is_cuda, "tensors must be on a GPU (no CPU path in this library)")
 
 
+def _compiled(name, on_gpu):
+    """the compiled binding's form of a call (the same checks and launches), None where it is not built"""
+    ext = _k.ext() if on_gpu else None
+    return getattr(ext, name, None)
+
+
 class GatedDeltaRuleFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, initial_state, scale, reverse, seq_lens, return_final_state):
@@ -77,6 +83,10 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
     device: the valid tokens of each batch entry, first in memory in either direction (values are clamped to 0 .. seqlen); the rest is padding
     that leaves the state alone, gives 0 and receives gradient 0.
     -> out (batch, seqlen, heads, dv), with return_final_state (out, final_state fp32).  Differentiable once in q, k, v, g, beta, initial_state."""
+    fast = _compiled("gated_delta_rule", v.is_cuda and v.numel())
+    if fast is not None:
+        r = fast(q, k, v, g, beta, scale, initial_state, return_final_state, reverse, seq_lens)
+        return tuple(r) if return_final_state else r[0]
     _check_inputs(q, k, v, g, beta, 2)
     batch, seqlen, heads, dv = v.shape
     dk = k.shape[-1]
@@ -141,6 +151,9 @@ def gated_delta_state_update(state, q, k, v, g, beta, scale=None):
     """One token.  state (batch, heads, dk, dv) [in/out], fp32, fp16 or bf16, each (dk, dv) contiguous; q, k (batch, heads_k, dk), v (batch, heads, dv),
     one dtype; g, beta (batch, heads), that dtype or fp32; scale: default dk ** -0.5 -> out (batch, heads, dv).  The arithmetic is fp32; a
     16-bit state is rounded as it is stored, out is computed before that rounding.  Not differentiable."""
+    fast = _compiled("gated_delta_state_update", v.is_cuda)
+    if fast is not None:
+        return fast(state, q, k, v, g, beta, scale)
     _check_inputs(q, k, v, g, beta, 1)
     _check(state.dim() == 4 and tuple(state.shape) == (*v.shape[:2], k.shape[-1], v.shape[-1]), "state must be (batch, heads, dk, dv)")
     _check(state.dtype in (torch.float32, torch.float16, torch.bfloat16) and state.device == v.device, "state must be fp32, fp16 or bf16 on the device of v")
@@ -151,6 +164,7 @@ def gated_delta_state_update(state, q, k, v, g, beta, scale=None):
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     if v.numel():
         _k.gated_delta_step(state, _unit_last(q), _unit_last(k), _unit_last(v), g, beta, k.shape[-1] ** -0.5 if scale is None else scale, out)
+        torch.autograd.graph.increment_version(state)
     return out
 
 
