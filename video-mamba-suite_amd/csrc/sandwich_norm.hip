@@ -1,8 +1,8 @@
 // sandwich_norm.hip -- the norm after a block, its gate, the scaled residual add and the norm before the next block, one pass each way:
 //   h = norm(x; w1, b1);  r' = residual_scale * r + gate * h;  y = norm(r'; w2, b2)
 // Streaming kernels (forward: x, r in, y, r' out; backward: x, r, dy, dr' in, dx, dr out) with two dependent row reductions.  A row
-// belongs to a team of 64, 256 or 1024 lanes (8 or 16 columns a lane, all of the row's values in registers from the load to the store);
-// one wave per row as long as that fits (cols <= 1024), since its reductions are DPP sums without barriers.  Statistics are two-pass in fp32
+// belongs to a team of lanes (forward: 8 or 16 columns a lane, one wave up to 1024 columns, whose reductions are DPP sums without barriers; backward: 8 a
+// lane, its sums over rows want the registers), all of its values in registers from the load to the store.  Statistics are two-pass in fp32
 // (mean first, then squares of differences).  y is the norm of the sum before it is rounded to the stream's type; the backward rebuilds that
 // sum from x and r (the bytes of reading r' instead) and the four saved statistics of a row.
 // Sums over rows (dw, db, dgate): in registers over the rows a team walks, one partial row per workgroup, a finish launch adds them in a fixed order.
@@ -12,36 +12,66 @@
 namespace vms {
 namespace sn {
 
-template <typename T>
+// 16 bytes at any alignment
+typedef unsigned __attribute__((ext_vector_type(4), aligned(2))) u4_any;
+
+// 8 columns c .. c+7 of a row of n, any alignment; zeros outside.  WHOLE: n % 8 == 0.  No branch around a load (its registers would be written by the other side
+// too, and the wave would wait for each load before the next), and zeros are put in word by word (element by element the compiler takes the load apart).
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void ld8(const T* row, int c, int n, float (&o)[8]) {
-    T v[8];
-    if (c + 8 <= n) __builtin_memcpy(v, row + c, sizeof(v));
-    else
+    constexpr int V = sizeof(T) / 2;   // 16-byte vectors
+    if constexpr (WHOLE) {
+        const u4_any* const at = reinterpret_cast<const u4_any*>(row + (c < n ? c : 0));
+        unsigned w[4 * V];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < n ? row[c + e] : static_cast<T>(0.f);
+        for (int i = 0; i < V; ++i) {
+            const u4_any x = at[i];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(v[e]);
+            for (int e = 0; e < 4; ++e) w[4 * i + e] = x[e];
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * V; ++i) w[i] = c < n ? w[i] : 0u;
+        T v[8];
+        __builtin_memcpy(v, w, sizeof(v));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(v[e]);
+    } else {
+        T v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = row[c + e < n ? c + e : 0];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = c + e < n ? static_cast<float>(v[e]) : 0.f;
+    }
 }
-template <typename T>
+template <bool WHOLE, typename T>   // c < n
 __device__ __forceinline__ void st8(T* row, int c, int n, const float (&o)[8]) {
     T v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = static_cast<T>(o[e]);
-    if (c + 8 <= n) __builtin_memcpy(row + c, v, sizeof(v));
-    else
+    if constexpr (WHOLE) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            vec_t<unsigned, 4> x;
+            __builtin_memcpy(&x, reinterpret_cast<const char*>(v) + 16 * i, 16);
+            reinterpret_cast<u4_any*>(row + c)[i] = x;
+        }
+    } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (c + e < n) row[c + e] = v[e];
+    }
 }
+template <bool WHOLE>
 __device__ __forceinline__ void ld8_any(const void* base, int64_t row, int c, int n, int dt, float (&o)[8]) {
-    if (dt == VMS_F32) ld8<float>(static_cast<const float*>(base) + row, c, n, o);
-    else if (dt == VMS_F16) ld8<f16_t>(static_cast<const f16_t*>(base) + row, c, n, o);
-    else ld8<bf16_t>(static_cast<const bf16_t*>(base) + row, c, n, o);
+    if (dt == VMS_F32) ld8<WHOLE, float>(static_cast<const float*>(base) + row, c, n, o);
+    else if (dt == VMS_F16) ld8<WHOLE, f16_t>(static_cast<const f16_t*>(base) + row, c, n, o);
+    else ld8<WHOLE, bf16_t>(static_cast<const bf16_t*>(base) + row, c, n, o);
 }
+template <bool WHOLE>
 __device__ __forceinline__ void st8_any(void* base, int64_t row, int c, int n, int dt, const float (&o)[8]) {
-    if (dt == VMS_F32) st8<float>(static_cast<float*>(base) + row, c, n, o);
-    else if (dt == VMS_F16) st8<f16_t>(static_cast<f16_t*>(base) + row, c, n, o);
-    else st8<bf16_t>(static_cast<bf16_t*>(base) + row, c, n, o);
+    if (dt == VMS_F32) st8<WHOLE, float>(static_cast<float*>(base) + row, c, n, o);
+    else if (dt == VMS_F16) st8<WHOLE, f16_t>(static_cast<f16_t*>(base) + row, c, n, o);
+    else st8<WHOLE, bf16_t>(static_cast<bf16_t*>(base) + row, c, n, o);
 }
 
 // sums over a team; red: 2 x 2 x 16 floats of LDS, used in turn so that one barrier per sum is enough
@@ -71,7 +101,7 @@ struct Team {
     }
 };
 
-template <typename TX, typename TR, bool RMS, int TS, int K>
+template <typename TX, typename TR, int TS, int K, bool WHOLE>
 __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const vms_sandwich_norm_params p) {
     constexpr int TEAMS = TS == 64 ? 4 : 1;
     __shared__ float red[64];
@@ -82,16 +112,16 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const
         const TX* const x = static_cast<const TX*>(p.x) + row * p.x_row_stride;
         float v[K][8], r[K][8];
 #pragma unroll
-        for (int k = 0; k < K; ++k) ld8<TX>(x, 8 * (lane + TS * k), N, v[k]);
+        for (int k = 0; k < K; ++k) ld8<WHOLE, TX>(x, 8 * (lane + TS * k), N, v[k]);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if (p.residual) ld8<TR>(static_cast<const TR*>(p.residual) + row * p.residual_row_stride, 8 * (lane + TS * k), N, r[k]);
+            if (p.residual) ld8<WHOLE, TR>(static_cast<const TR*>(p.residual) + row * p.residual_row_stride, 8 * (lane + TS * k), N, r[k]);
             else
                 for (int e = 0; e < 8; ++e) r[k][e] = 0.f;
         }
         auto norm = [&](float (&z)[K][8], float& mean, float& rstd) __attribute__((always_inline)) {
             mean = 0.f;
-            if constexpr (!RMS) {
+            if (!p.is_rms) {
                 float s = 0.f;
 #pragma unroll
                 for (int k = 0; k < K; ++k)
@@ -118,9 +148,9 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const
             const int c = 8 * (lane + TS * k);
             if (c < N) {
                 float w[8], b[8], g[8];
-                ld8<float>(p.post_weight, c, N, w);
-                if (p.post_bias) ld8<float>(p.post_bias, c, N, b);
-                if (p.gate) ld8_any(p.gate, gate_row, c, N, p.gate_dtype, g);
+                ld8<WHOLE, float>(p.post_weight, c, N, w);
+                if (p.post_bias) ld8<WHOLE, float>(p.post_bias, c, N, b);
+                if (p.gate) ld8_any<WHOLE>(p.gate, gate_row, c, N, p.gate_dtype, g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float h = v[k][e] * s1 * w[e];
@@ -128,7 +158,7 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const
                     if (p.gate) h *= g[e];
                     r[k][e] = c + e < N ? fmaf(p.residual_scale, r[k][e], h) : 0.f;
                 }
-                st8<TR>(static_cast<TR*>(p.residual_out) + row * p.residual_out_row_stride, c, N, r[k]);
+                st8<WHOLE, TR>(static_cast<TR*>(p.residual_out) + row * p.residual_out_row_stride, c, N, r[k]);
             }
         }
         norm(r, m2, s2);
@@ -137,14 +167,14 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const
             const int c = 8 * (lane + TS * k);
             if (c < N) {
                 float w[8], b[8];
-                ld8<float>(p.pre_weight, c, N, w);
-                if (p.pre_bias) ld8<float>(p.pre_bias, c, N, b);
+                ld8<WHOLE, float>(p.pre_weight, c, N, w);
+                if (p.pre_bias) ld8<WHOLE, float>(p.pre_bias, c, N, b);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     r[k][e] *= s2 * w[e];
                     if (p.pre_bias) r[k][e] += b[e];
                 }
-                st8<TX>(static_cast<TX*>(p.y) + row * p.y_row_stride, c, N, r[k]);
+                st8<WHOLE, TX>(static_cast<TX*>(p.y) + row * p.y_row_stride, c, N, r[k]);
             }
         }
         if (p.stats && lane == 0) *reinterpret_cast<float4*>(p.stats + 4 * row) = make_float4(m1, s1, m2, s2);
@@ -155,189 +185,141 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const
 // written row by row).  Few groups: `parts` workgroups share each (whole = 0).  More groups than workgroups: a team walks whole groups (whole = 1).
 struct Plan { int groups, parts, whole, partials; int64_t rpg; };
 constexpr int kMostWgs = 1024;   // 4 per CU
-static int team_size(int cols) { return cols <= 1024 ? 64 : cols <= 4096 ? 256 : 1024; }
+// lanes of a row in the backward: 8 columns each
+static int team_of(int cols) { return cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024; }
 static Plan plan_of(const vms_sandwich_norm_params& p) {
     Plan l{};
     l.rpg = p.gate && p.rows_per_gate > 1 ? p.rows_per_gate : p.rows;
     l.groups = (int)(p.rows / l.rpg);
-    const int teams = team_size(p.cols) == 64 ? 4 : 1;
-    l.whole = l.groups > kMostWgs / 2;
+    const int ts = team_of(p.cols), teams = ts == 64 ? 4 : 1, most_wgs = ts == 128 ? 3 * kMostWgs / 2 : kMostWgs;   // (as many as are resident)
+    l.whole = l.groups > most_wgs / 2;
     if (l.whole) {
         const int want = (l.groups + teams - 1) / teams;
         l.parts = 1;
-        l.partials = want < kMostWgs ? want : kMostWgs;
+        l.partials = want < most_wgs ? want : most_wgs;
     } else {
         const int64_t most = (l.rpg + teams - 1) / teams;
-        l.parts = kMostWgs / l.groups;
+        l.parts = most_wgs / l.groups;
         if (l.parts > most) l.parts = (int)most;
         l.partials = l.groups * l.parts;
     }
     return l;
 }
 
-template <typename TX, typename TR, bool RMS, int TS, int K>
-__global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_bwd_kernel(const vms_sandwich_norm_bwd_params q, const Plan plan) {
+// GROUPS: whole groups per team (Plan::whole)
+template <typename TX, typename TR, int TS, bool WHOLE, bool GROUPS>
+__global__ __launch_bounds__(TS < 128 ? 256 : TS, TS == 1024 ? 4 : 3) void sandwich_bwd_kernel(const vms_sandwich_norm_bwd_params q, const Plan plan) {
     constexpr int TEAMS = TS == 64 ? 4 : 1;
     __shared__ float red[64];
-    __shared__ float sums[TEAMS > 1 ? (TEAMS - 1) * K * 8 * 64 : 1];
+    __shared__ float sums[TEAMS > 1 ? (TEAMS - 1) * 8 * 64 : 1];
     const vms_sandwich_norm_params& p = q.f;
     Team<TS> team{red};
-    const int lane = threadIdx.x % TS, tm = threadIdx.x / TS, N = p.cols;
-    const float inv_n = 1.f / N;
+    const int lane = threadIdx.x % TS, tm = threadIdx.x / TS, N = p.cols, c = 8 * lane;
+    const float inv_n = 1.f / N, center = p.is_rms ? 0.f : inv_n;
     const bool row_gate = p.gate && p.rows_per_gate == 1, col_gate = p.gate && p.rows_per_gate > 1;
-    float P1[K][8], P0[K][8], Q1[K][8], Q0[K][8];   // sums over this team's rows
-    float A1[K][8], A0[K][8];                        // whole groups: the gate-weighted sums of P1, P0
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { P1[k][e] = 0.f; P0[k][e] = 0.f; Q1[k][e] = 0.f; Q0[k][e] = 0.f; A1[k][e] = 0.f; A0[k][e] = 0.f; }
+    float P1[8] = {}, P0[8] = {}, Q1[8] = {}, Q0[8] = {};   // sums over this team's rows
+    float A1[GROUPS ? 8 : 1] = {}, A0[GROUPS ? 8 : 1] = {};   // whole groups: the gate-weighted sums of P1, P0
 
     auto one_row = [&](int64_t row) __attribute__((always_inline)) {
         const float4 st = *reinterpret_cast<const float4*>(p.stats + 4 * row);
-        float xh[K][8], rh[K][8], t[K][8], dr[K][8];
+        float xh[8], rh[8] = {}, t[8] = {}, dr[8] = {}, g[8], w1[8], b[8] = {};
         const int64_t gate_row = p.gate ? row / p.rows_per_gate * p.gate_row_stride : 0;
+        ld8<WHOLE, TX>(static_cast<const TX*>(p.x) + row * p.x_row_stride, c, N, xh);
+        if (p.residual) ld8<WHOLE, TR>(static_cast<const TR*>(p.residual) + row * p.residual_row_stride, c, N, rh);
+        if (q.dy) ld8<WHOLE, TX>(static_cast<const TX*>(q.dy) + row * q.dy_row_stride, c, N, t);
+        if (q.dresidual_out) ld8<WHOLE, TR>(static_cast<const TR*>(q.dresidual_out) + row * q.dresidual_out_row_stride, c, N, dr);
+        ld8<WHOLE, float>(p.post_weight, c, N, w1);
+        if (p.post_bias) ld8<WHOLE, float>(p.post_bias, c, N, b);
+        if (p.gate) ld8_any<WHOLE>(p.gate, gate_row, c, N, p.gate_dtype, g);
+        else
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = 8 * (lane + TS * k);
-            ld8<TX>(static_cast<const TX*>(p.x) + row * p.x_row_stride, c, N, xh[k]);
-            if (p.residual) ld8<TR>(static_cast<const TR*>(p.residual) + row * p.residual_row_stride, c, N, rh[k]);
-            else
-                for (int e = 0; e < 8; ++e) rh[k][e] = 0.f;
-            if (q.dy) ld8<TX>(static_cast<const TX*>(q.dy) + row * q.dy_row_stride, c, N, t[k]);
-            else
-                for (int e = 0; e < 8; ++e) t[k][e] = 0.f;
-            if (q.dresidual_out) ld8<TR>(static_cast<const TR*>(q.dresidual_out) + row * q.dresidual_out_row_stride, c, N, dr[k]);
-            else
-                for (int e = 0; e < 8; ++e) dr[k][e] = 0.f;
-        }
-        float g[K][8], w1[K][8];
+            for (int e = 0; e < 8; ++e) g[e] = 1.f;
+        float w2[8];
+        ld8<WHOLE, float>(p.pre_weight, c, N, w2);
         float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = 8 * (lane + TS * k);
-            float b[8], w2[8];
-            ld8<float>(p.post_weight, c, N, w1[k]);
-            ld8<float>(p.pre_weight, c, N, w2);
-            if (p.post_bias) ld8<float>(p.post_bias, c, N, b);
-            if (p.gate) ld8_any(p.gate, gate_row, c, N, p.gate_dtype, g[k]);
-            float dg[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool in = c + e < N;
-                xh[k][e] = in ? (xh[k][e] - st.x) * st.y : 0.f;
-                float h = xh[k][e] * w1[k][e];
-                if (p.post_bias) h += b[e];
-                dg[e] = h;
-                if (p.gate) h *= g[k][e];
-                rh[k][e] = in ? (fmaf(p.residual_scale, rh[k][e], h) - st.z) * st.w : 0.f;
-                Q1[k][e] = fmaf(t[k][e], rh[k][e], Q1[k][e]);
-                Q0[k][e] += t[k][e];
-                t[k][e] *= w2[e];
-                c1 = fmaf(t[k][e], rh[k][e], c1);
-                c2 += t[k][e];
-            }
+        for (int e = 0; e < 8; ++e) {
+            const bool in = c + e < N;
+            xh[e] = in ? (xh[e] - st.x) * st.y : 0.f;
+            const float h = fmaf(xh[e], w1[e], b[e]) * g[e];
+            rh[e] = in ? (fmaf(p.residual_scale, rh[e], h) - st.z) * st.w : 0.f;
+            Q1[e] = fmaf(t[e], rh[e], Q1[e]);
+            Q0[e] += t[e];
+            t[e] *= w2[e];
+            c1 = fmaf(t[e], rh[e], c1);
+            c2 += t[e];
         }
         team.sum2(c1, c2);
         c1 *= inv_n;
-        c2 = RMS ? 0.f : c2 * inv_n;
-        float d1 = 0.f, d2 = 0.f;
+        c2 *= center;
+        float d1 = 0.f, d2 = 0.f, o[8];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = 8 * (lane + TS * k);
-            float o[8];
+        for (int e = 0; e < 8; ++e) {
+            dr[e] = c + e < N ? fmaf(t[e] - fmaf(rh[e], c1, c2), st.w, dr[e]) : 0.f;
+            o[e] = p.residual_scale * dr[e];
+        }
+        if (q.dresidual && c < N) st8<WHOLE, TR>(static_cast<TR*>(q.dresidual) + row * q.dresidual_row_stride, c, N, o);
+        if (row_gate && c < N) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float d = c + e < N ? fmaf(t[k][e] - fmaf(rh[k][e], c1, c2), st.w, dr[k][e]) : 0.f;
-                dr[k][e] = d;
-                o[e] = p.residual_scale * d;
-            }
-            if (q.dresidual && c < N) st8<TR>(static_cast<TR*>(q.dresidual) + row * q.dresidual_row_stride, c, N, o);
-            if (row_gate && c < N) {
-                float b[8];
-                if (p.post_bias) ld8<float>(p.post_bias, c, N, b);
+            for (int e = 0; e < 8; ++e) o[e] = dr[e] * fmaf(xh[e], w1[e], b[e]);
+            st8_any<WHOLE>(q.dgate, row * (int64_t)N, c, N, p.gate_dtype, o);
+        }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = dr[k][e] * (p.post_bias ? fmaf(xh[k][e], w1[k][e], b[e]) : xh[k][e] * w1[k][e]);
-                if (q.dgate) st8_any(q.dgate, row * (int64_t)N, c, N, p.gate_dtype, o);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float d = dr[k][e];
-                if (!col_gate && p.gate) d *= g[k][e];   // a row's own gate enters the sums here, a shared one afterwards
-                P1[k][e] = fmaf(d, xh[k][e], P1[k][e]);
-                P0[k][e] += d;
-                if (col_gate) d *= g[k][e];
-                d *= w1[k][e];
-                t[k][e] = d;
-                d1 = fmaf(d, xh[k][e], d1);
-                d2 += d;
-            }
+        for (int e = 0; e < 8; ++e) {
+            const float gated = dr[e] * g[e];
+            const float d = col_gate ? dr[e] : gated;   // a row's own gate enters the sums here, a shared one afterwards
+            P1[e] = fmaf(d, xh[e], P1[e]);
+            P0[e] += d;
+            t[e] = gated * w1[e];
+            d1 = fmaf(t[e], xh[e], d1);
+            d2 += t[e];
         }
         team.sum2(d1, d2);
         d1 *= inv_n;
-        d2 = RMS ? 0.f : d2 * inv_n;
+        d2 *= center;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = 8 * (lane + TS * k);
-            float o[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = (t[k][e] - fmaf(xh[k][e], d1, d2)) * st.y;
-            if (c < N) st8<TX>(static_cast<TX*>(q.dx) + row * q.dx_row_stride, c, N, o);
-        }
+        for (int e = 0; e < 8; ++e) o[e] = (t[e] - fmaf(xh[e], d1, d2)) * st.y;
+        if (c < N) st8<WHOLE, TX>(static_cast<TX*>(q.dx) + row * q.dx_row_stride, c, N, o);
     };
 
-    if (!plan.whole) {
+    if constexpr (!GROUPS) {
         const int64_t first = (int64_t)(blockIdx.x / plan.parts) * plan.rpg;
         for (int64_t i = (int64_t)(blockIdx.x % plan.parts) * TEAMS + tm; i < plan.rpg; i += (int64_t)plan.parts * TEAMS) one_row(first + i);
     } else {
         for (int64_t gr = (int64_t)blockIdx.x * TEAMS + tm; gr < plan.groups; gr += (int64_t)gridDim.x * TEAMS) {
             for (int64_t i = 0; i < plan.rpg; ++i) one_row(gr * plan.rpg + i);
+            float w[8], b[8] = {}, g[8], o[8];
+            ld8<WHOLE, float>(p.post_weight, c, N, w);
+            if (p.post_bias) ld8<WHOLE, float>(p.post_bias, c, N, b);
+            ld8_any<WHOLE>(p.gate, gr * p.gate_row_stride, c, N, p.gate_dtype, g);
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int c = 8 * (lane + TS * k);
-                if (c < N) {
-                    float w[8], b[8], g[8], o[8];
-                    ld8<float>(p.post_weight, c, N, w);
-                    if (p.post_bias) ld8<float>(p.post_bias, c, N, b);
-                    ld8_any(p.gate, gr * p.gate_row_stride, c, N, p.gate_dtype, g);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        o[e] = w[e] * P1[k][e] + (p.post_bias ? b[e] * P0[k][e] : 0.f);
-                        A1[k][e] = fmaf(g[e], P1[k][e], A1[k][e]);
-                        A0[k][e] = fmaf(g[e], P0[k][e], A0[k][e]);
-                        P1[k][e] = 0.f;
-                        P0[k][e] = 0.f;
-                    }
-                    if (q.dgate) st8_any(q.dgate, gr * (int64_t)N, c, N, p.gate_dtype, o);
-                }
+            for (int e = 0; e < 8; ++e) {
+                o[e] = fmaf(w[e], P1[e], b[e] * P0[e]);
+                A1[e] = fmaf(g[e], P1[e], A1[e]);
+                A0[e] = fmaf(g[e], P0[e], A0[e]);
+                P1[e] = 0.f;
+                P0[e] = 0.f;
             }
+            if (c < N) st8_any<WHOLE>(q.dgate, gr * (int64_t)N, c, N, p.gate_dtype, o);
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { P1[k][e] = A1[k][e]; P0[k][e] = A0[k][e]; }
+        for (int e = 0; e < 8; ++e) { P1[e] = A1[e]; P0[e] = A0[e]; }
     }
     float* const out = static_cast<float*>(q.workspace) + (int64_t)blockIdx.x * 4 * N;
-    auto emit = [&](float (&a)[K][8], int which) __attribute__((always_inline)) {
+    auto emit = [&](float (&a)[8], int which) __attribute__((always_inline)) {
         if constexpr (TEAMS > 1) {
             __syncthreads();
             if (tm > 0)
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) sums[((tm - 1) * K * 8 + k * 8 + e) * 64 + lane] = a[k][e];
+                for (int e = 0; e < 8; ++e) sums[((tm - 1) * 8 + e) * 64 + lane] = a[e];
             __syncthreads();
+            if (tm == 0)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int t2 = 0; t2 < TEAMS - 1; ++t2) a[e] += sums[(t2 * 8 + e) * 64 + lane];
         }
-        if (tm == 0)
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int c = 8 * (lane + TS * k);
-                if constexpr (TEAMS > 1)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-#pragma unroll
-                        for (int t2 = 0; t2 < TEAMS - 1; ++t2) a[k][e] += sums[(t2 * K * 8 + k * 8 + e) * 64 + lane];
-                if (c < N) st8<float>(out + (int64_t)which * N, c, N, a[k]);
-            }
+        if (tm == 0 && c < N) st8<WHOLE, float>(out + (int64_t)which * N, c, N, a);
     };
     emit(P1, 0);
     emit(P0, 1);
@@ -345,58 +327,77 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_bwd_kernel(const
     emit(Q0, 3);
 }
 
-// ---- the partial rows' sums.  A workgroup owns 16 columns, 64 row lanes x 4 column groups.  blockIdx.y < gate_rows: dgate of that gate row
-// from its `parts` partial rows; the last y: dw1, db1 (with the gate of each partial row's group where `weigh`), dw2, db2
-__global__ __launch_bounds__(256) void sandwich_finish_kernel(const vms_sandwich_norm_bwd_params q, const Plan plan, const int gate_rows, const int weigh) {
-    __shared__ float red[4][64][17];
+// ---- the partial rows' sums.  A workgroup owns 64 columns (16 groups of 4) of one of the four arrays, 64 row lanes (with 16, one load at a time: 47 us
+// for 1536 rows of 1024); blockIdx.z < 4: dw1, db1 (with the
+// gate of each partial row's group where `weigh`), dw2, db2;  blockIdx.z >= 4: dgate of gate row z - 4 from its `parts` partial rows of P1 and P0
+__global__ __launch_bounds__(1024) void sandwich_finish_kernel(const vms_sandwich_norm_bwd_params q, const Plan plan, const int weigh) {
+    __shared__ float red[2][64][65];
     const vms_sandwich_norm_params& p = q.f;
-    const int N = p.cols, rl = threadIdx.x >> 2, cg = threadIdx.x & 3, c0 = blockIdx.x * 16 + 4 * cg;
-    const bool weights = (int)blockIdx.y == gate_rows;
+    const int N = p.cols, rl = threadIdx.x >> 4, cg = threadIdx.x & 15, c0 = blockIdx.x * 64 + 4 * cg;
     const float* const src = static_cast<const float*>(q.workspace);
-    const int r0 = weights ? 0 : blockIdx.y * plan.parts, r1 = weights ? plan.partials : r0 + plan.parts, arrays = weights ? 4 : 2;
-    float a[4][4] = {};
-    for (int r = r0 + rl; r < r1; r += 64)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int c = c0 + e;
-            if (c < N) {
-                const float* const row = src + (int64_t)r * 4 * N + c;
-                float g = 1.f;
-                if (weights && weigh) {
-                    const int64_t at = (int64_t)(r / plan.parts) * p.gate_row_stride + c;
-                    g = p.gate_dtype == VMS_F32 ? static_cast<const float*>(p.gate)[at]
-                        : p.gate_dtype == VMS_F16 ? static_cast<float>(static_cast<const f16_t*>(p.gate)[at]) : static_cast<float>(static_cast<const bf16_t*>(p.gate)[at]);
-                }
-                a[0][e] = fmaf(g, row[0], a[0][e]);
-                a[1][e] = fmaf(g, row[N], a[1][e]);
-                if (arrays == 4) {
-                    a[2][e] += row[2 * (int64_t)N];
-                    a[3][e] += row[3 * (int64_t)N];
-                }
-            }
-        }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) red[i][rl][4 * cg + e] = a[i][e];
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        const int i = threadIdx.x >> 4, cc = threadIdx.x & 15, c = blockIdx.x * 16 + cc;
-        float t = 0.f;
-#pragma unroll 8
-        for (int r = 0; r < 64; ++r) t += red[i][r][cc];
-        if (weights) {
-            float* const dst = i == 0 ? q.dpost_weight : i == 1 ? q.dpost_bias : i == 2 ? q.dpre_weight : q.dpre_bias;
-            if (dst && c < N) dst[c] = t;
+    const int z = blockIdx.y;
+    const bool gate = z >= 4;
+    const int r0 = gate ? (z - 4) * plan.parts : 0, r1 = gate ? r0 + plan.parts : plan.partials;
+    const int which = gate ? 0 : z;
+    float a[4] = {}, a2[4] = {};
+    const bool vec = N % 4 == 0;
+    auto ld4 = [&](const float* row, float (&v)[4]) __attribute__((always_inline)) {   // columns c0 .. c0 + 3
+        if (vec) {
+            const float4 x = *reinterpret_cast<const float4*>(row + (c0 < N ? c0 : 0));
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
         } else {
-            const float p0 = __shfl(t, 16 + cc);   // i == 0 holds the sum of P1, i == 1 that of P0
-            if (i == 0 && c < N) {
-                const float d = p.post_weight[c] * t + (p.post_bias ? p.post_bias[c] * p0 : 0.f);
-                const int64_t at = (int64_t)blockIdx.y * N + c;
-                if (p.gate_dtype == VMS_F32) static_cast<float*>(q.dgate)[at] = d;
-                else if (p.gate_dtype == VMS_F16) static_cast<f16_t*>(q.dgate)[at] = static_cast<f16_t>(d);
-                else static_cast<bf16_t*>(q.dgate)[at] = static_cast<bf16_t>(d);
-            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = row[c0 + e < N ? c0 + e : 0];
+        }
+    };
+    auto gate_at = [&](int64_t at) __attribute__((always_inline)) {
+        return p.gate_dtype == VMS_F32 ? static_cast<const float*>(p.gate)[at]
+               : p.gate_dtype == VMS_F16 ? static_cast<float>(static_cast<const f16_t*>(p.gate)[at]) : static_cast<float>(static_cast<const bf16_t*>(p.gate)[at]);
+    };
+    if (gate) {
+#pragma unroll 4
+        for (int r = r0 + rl; r < r1; r += 64) {
+            float v[4], v2[4];
+            ld4(src + (int64_t)r * 4 * N, v);
+            ld4(src + (int64_t)r * 4 * N + N, v2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { a[e] += v[e]; a2[e] += v2[e]; }
+        }
+    } else if (weigh && which < 2 && plan.groups > 1) {
+#pragma unroll 4
+        for (int r = r0 + rl; r < r1; r += 64) {
+            float v[4];
+            ld4(src + ((int64_t)r * 4 + which) * N, v);
+            const int64_t at = (int64_t)(r / plan.parts) * p.gate_row_stride;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = fmaf(gate_at(at + (c0 + e < N ? c0 + e : 0)), v[e], a[e]);
+        }
+    } else {
+#pragma unroll 8
+        for (int r = r0 + rl; r < r1; r += 64) {
+            float v[4];
+            ld4(src + ((int64_t)r * 4 + which) * N, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] += v[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { red[0][rl][4 * cg + e] = a[e]; red[1][rl][4 * cg + e] = a2[e]; }
+    __syncthreads();
+    const int c = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && c < N) {
+        float t = 0.f, t2 = 0.f;
+#pragma unroll
+        for (int r = 0; r < 64; ++r) { t += red[0][r][threadIdx.x]; t2 += red[1][r][threadIdx.x]; }
+        if (!gate) {
+            float* const dst = z == 0 ? q.dpost_weight : z == 1 ? q.dpost_bias : z == 2 ? q.dpre_weight : q.dpre_bias;
+            if (dst) dst[c] = weigh && z < 2 && plan.groups == 1 ? t * gate_at(c) : t;   // (one gate row: a factor of the sum)
+        } else {
+            const float d = p.post_weight[c] * t + (p.post_bias ? p.post_bias[c] * t2 : 0.f);
+            const int64_t at = (int64_t)(z - 4) * N + c;
+            if (p.gate_dtype == VMS_F32) static_cast<float*>(q.dgate)[at] = d;
+            else if (p.gate_dtype == VMS_F16) static_cast<f16_t*>(q.dgate)[at] = static_cast<f16_t>(d);
+            else static_cast<bf16_t*>(q.dgate)[at] = static_cast<bf16_t>(d);
         }
     }
 }
@@ -417,50 +418,51 @@ static int validate(const vms_sandwich_norm_params& p) {
     return VMS_OK;
 }
 
-template <typename TX, typename TR, bool RMS>
+template <typename TX, typename TR, bool WHOLE>
 static int fwd_launch(const vms_sandwich_norm_params& p, hipStream_t s) {
-    const int ts = team_size(p.cols);
+    const int ts = p.cols <= 1024 ? 64 : p.cols <= 4096 ? 256 : 1024;
     const int64_t want = ts == 64 ? (p.rows + 3) / 4 : p.rows;
     const dim3 grid((unsigned)(want < 2048 ? want : 2048)), block(ts < 256 ? 256 : ts);
-    if (p.cols <= 512) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, RMS, 64, 1>), grid, block, 0, s, p);
-    else if (ts == 64) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, RMS, 64, 2>), grid, block, 0, s, p);
-    else if (p.cols <= 2048) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, RMS, 256, 1>), grid, block, 0, s, p);
-    else if (ts == 256) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, RMS, 256, 2>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, RMS, 1024, 1>), grid, block, 0, s, p);
+    if (p.cols <= 512) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, 64, 1, WHOLE>), grid, block, 0, s, p);
+    else if (ts == 64) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, 64, 2, WHOLE>), grid, block, 0, s, p);
+    else if (p.cols <= 2048) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, 256, 1, WHOLE>), grid, block, 0, s, p);
+    else if (ts == 256) hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, 256, 2, WHOLE>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((sandwich_fwd_kernel<TX, TR, 1024, 1, WHOLE>), grid, block, 0, s, p);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-template <typename TX, typename TR, bool RMS>
+template <typename TX, typename TR, bool WHOLE, bool GROUPS>
+static void bwd_team(const vms_sandwich_norm_bwd_params& q, const Plan& plan, hipStream_t s) {
+    const int ts = team_of(q.f.cols);
+    const dim3 grid(plan.partials), block(ts == 64 ? 256 : ts);
+    if (ts == 64) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, 64, WHOLE, GROUPS>), grid, block, 0, s, q, plan);
+    else if (ts == 128) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, 128, WHOLE, GROUPS>), grid, block, 0, s, q, plan);
+    else if (ts == 256) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, 256, WHOLE, GROUPS>), grid, block, 0, s, q, plan);
+    else if (ts == 512) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, 512, WHOLE, GROUPS>), grid, block, 0, s, q, plan);
+    else hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, 1024, WHOLE, GROUPS>), grid, block, 0, s, q, plan);
+}
+template <typename TX, typename TR, bool WHOLE>
 static int bwd_launch(const vms_sandwich_norm_bwd_params& q, hipStream_t s) {
     const vms_sandwich_norm_params& p = q.f;
     const Plan plan = plan_of(p);
-    const int ts = team_size(p.cols);
-    const dim3 grid(plan.partials), block(ts < 256 ? 256 : ts);
-    if (p.cols <= 512) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, RMS, 64, 1>), grid, block, 0, s, q, plan);
-    else if (ts == 64) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, RMS, 64, 2>), grid, block, 0, s, q, plan);
-    else if (p.cols <= 2048) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, RMS, 256, 1>), grid, block, 0, s, q, plan);
-    else if (ts == 256) hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, RMS, 256, 2>), grid, block, 0, s, q, plan);
-    else hipLaunchKernelGGL((sandwich_bwd_kernel<TX, TR, RMS, 1024, 1>), grid, block, 0, s, q, plan);
+    if (plan.whole) bwd_team<TX, TR, WHOLE, true>(q, plan, s);
+    else bwd_team<TX, TR, WHOLE, false>(q, plan, s);
     VMS_LAUNCH_CHECK();
-    const bool col_gate = p.gate && p.rows_per_gate > 1;
-    const int gate_rows = col_gate && !plan.whole && q.dgate ? plan.groups : 0;
-    hipLaunchKernelGGL(sandwich_finish_kernel, dim3((p.cols + 15) / 16, gate_rows + 1), dim3(256), 0, s, q, plan, gate_rows, col_gate && !plan.whole ? 1 : 0);
+    const bool shared = p.gate && p.rows_per_gate > 1 && !plan.whole;   // gate rows that collect sums over workgroups
+    hipLaunchKernelGGL(sandwich_finish_kernel, dim3((p.cols + 63) / 64, 4 + (shared ? plan.groups : 0)), dim3(1024), 0, s, q, plan, shared ? 1 : 0);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
 
+#define VMS_SN_TYPES(FN, TX, TR, P_, ARG, s)                                                                                             \
+    (((P_).cols % 8 == 0) ? FN<TX, TR, true>(ARG, s) : FN<TX, TR, false>(ARG, s))
 #define VMS_SN_DISPATCH(FN, P_, ARG, s)                                                                                                  \
     do {                                                                                                                                 \
-        const bool f32_ = (P_).res_dtype == VMS_F32, rms_ = (P_).is_rms != 0;                                                            \
+        const bool f32_ = (P_).res_dtype == VMS_F32;                                                                                     \
         switch ((P_).x_dtype) {                                                                                                          \
-            case VMS_F32: rc = rms_ ? FN<float, float, true>(ARG, s) : FN<float, float, false>(ARG, s); break;                           \
-            case VMS_F16:                                                                                                                \
-                rc = f32_ ? (rms_ ? FN<f16_t, float, true>(ARG, s) : FN<f16_t, float, false>(ARG, s))                                    \
-                          : (rms_ ? FN<f16_t, f16_t, true>(ARG, s) : FN<f16_t, f16_t, false>(ARG, s));                                   \
-                break;                                                                                                                   \
-            default:                                                                                                                     \
-                rc = f32_ ? (rms_ ? FN<bf16_t, float, true>(ARG, s) : FN<bf16_t, float, false>(ARG, s))                                  \
-                          : (rms_ ? FN<bf16_t, bf16_t, true>(ARG, s) : FN<bf16_t, bf16_t, false>(ARG, s));                               \
+            case VMS_F32: rc = VMS_SN_TYPES(FN, float, float, P_, ARG, s); break;                                                        \
+            case VMS_F16: rc = f32_ ? VMS_SN_TYPES(FN, f16_t, float, P_, ARG, s) : VMS_SN_TYPES(FN, f16_t, f16_t, P_, ARG, s); break;    \
+            default: rc = f32_ ? VMS_SN_TYPES(FN, bf16_t, float, P_, ARG, s) : VMS_SN_TYPES(FN, bf16_t, bf16_t, P_, ARG, s);             \
         }                                                                                                                                \
     } while (0)
 
@@ -489,6 +491,7 @@ extern "C" int vms_sandwich_norm_bwd(const vms_sandwich_norm_bwd_params* qq, voi
     if (int rc = sn::validate(q.f)) return rc;
     VMS_CHECK(q.f.stats && q.dx && q.dpost_weight && q.dpre_weight, "stats, dx, dpost_weight, dpre_weight are required");
     VMS_CHECK(!q.f.gate || q.dgate, "dgate comes with gate");
+    VMS_CHECK(aligned16(q.workspace), "workspace must be 16-byte aligned");
     VMS_CHECK(q.workspace && q.workspace_bytes >= vms_sandwich_norm_bwd_workspace_bytes(&q.f), "workspace is too small (vms_sandwich_norm_bwd_workspace_bytes)");
     int rc = VMS_OK;
     VMS_SN_DISPATCH(sn::bwd_launch, q.f, q, static_cast<hipStream_t>(stream));
