@@ -118,6 +118,7 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
         const float glast = gt.last();
         __syncthreads();   // dS and dO are there; the tiles of K and Q are no longer read
         fetch_rows(K, next, kx);   // (a few loads at a time, a chunk ahead: gd_scan)
+        fetch_small(next);
         // ---- dU = del K dS1 + M^T dO
         f32x4 dU[CT];
 #pragma unroll
@@ -149,7 +150,6 @@ __global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
         }
         fetch_rows(Q, next, qx);
         fetch_tri(next, 2 * NS + NO, mf);
-        fetch_small(next);
 #pragma unroll
         for (int d = 0; d < DW; ++d) store_rows<NO, CT>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0, dS[d], n, q4);
         __syncthreads();

@@ -302,7 +302,6 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
         fetch_small(0);
         fetch_t(0);
         fetch_m(0);
-        hand_small(0);
     }
     for (int c = 0; c < nc; ++c) {
         const int next = c + 1 < nc ? c + 1 : c;   // the last chunk again rather than a branch
@@ -310,15 +309,12 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
         const bool ok_n = c * C + 16 * w + n < len;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) { kr[kb] = kx[kb]; qr[kb] = qx[kb]; }
-        const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
-        const float sg = p.scale * gt.gam(n), glast = gt.last();
-        f32x4 vv[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) vv[j] = vt.get(j, n, q4);
+        hand_small(c);
         __syncthreads();   // S is there; K's tile is no longer read
         // Loads return in order, stores among them, and the memory pipe takes 20 .. 50 cycles for each instruction of a wave: what a phase waits
         // for is asked for a chunk earlier, a few instructions at a time
         fetch_rows(K, next, kx);
+        fetch_small(next);
         // ---- P = K S0, O = S0^T Q^T, R
         f32x4 P[CT], O[CT];
 #pragma unroll
@@ -335,6 +331,11 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
                 mma<NO>(O[j], sf, qf);    // [v][token]: the lanes of a store hold 4 consecutive v
             }
         }
+        const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
+        const float sg = p.scale * gt.gam(n), glast = gt.last();
+        f32x4 vv[CT];
+#pragma unroll
+        for (int j = 0; j < CT; ++j) vv[j] = vt.get(j, n, q4);
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
             f32x4 R;
@@ -367,7 +368,6 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
             Ux.put(j, n, paired(w, q4), U[j]);
         }
         fetch_t(next);
-        fetch_small(next);
         __syncthreads();
         // ---- S1 = gam S0 + K^T (del U)
 #pragma unroll
@@ -407,7 +407,6 @@ __global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_p
         if constexpr (TRAIN) {
             store_rows<NO, CT>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, col0, U, n, q4);
         }
-        hand_small(next);
     }
     if (p.final_state) {
 #pragma unroll
