@@ -209,12 +209,13 @@ __device__ __forceinline__ Frag<Prec<T>::NX> planes_of(const Raw8<T>& r) {
     return f;
 }
 
-// B operand that copies columns 16 half .. 16 half + 15 of a paired-order operand out of a product: D = A I.  Turns an operand
+// B operand that copies columns 16 half .. 16 half + 15 of an operand out of a product: D = A I.  Turns an operand
 // whose lanes hold a column (4 consecutive rows in a register each) into one whose lanes hold a row: 8-byte stores instead of 2-byte ones.
+template <bool PAIRED = true>
 __device__ __forceinline__ bf16x8 unit_frag(int half, int n, int p) {
     bf16x8 f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = static_cast<bf16_t>((e >> 2) == half && 4 * p + (e & 3) == n ? 1.f : 0.f);
+    for (int e = 0; e < 8; ++e) f[e] = static_cast<bf16_t>((PAIRED ? 16 * (e >> 2) + 4 * p + (e & 3) : 8 * p + e) == 16 * half + n ? 1.f : 0.f);
     return f;
 }
 
@@ -225,6 +226,13 @@ template <int KP, int NX>
 __device__ __forceinline__ void tile_put(char* tile, int row, int c, const Frag<NX>& f) {   // columns c .. c+7
 #pragma unroll
     for (int i = 0; i < NX; ++i) *reinterpret_cast<bf16x8*>(tile + i * tile_bytes<KP>() + row * tile_row<KP>() + 2 * c) = f.p[i];
+}
+template <int KP, int NX>
+__device__ __forceinline__ Frag<NX> tile_rows(const char* tile, int row, int c) {
+    Frag<NX> f;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(tile + i * tile_bytes<KP>() + row * tile_row<KP>() + 2 * c);
+    return f;
 }
 // lane: column 16 m + n, tokens of block tb (32) in paired order.  ds_read_b64_tr_b16: lane i of 16 names row i / 4, column group i % 4
 template <int KP, int NX>
@@ -253,10 +261,11 @@ struct Exchange {
             *reinterpret_cast<vec_t<unsigned, 2>*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at) = u;
         }
     }
-    __device__ __forceinline__ Frag<N> get(int j, int n, int at) const {
-        Frag<N> f;
+    template <int M = N>   // the first M planes
+    __device__ __forceinline__ Frag<M> get(int j, int n, int at) const {
+        Frag<M> f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at);
+        for (int i = 0; i < M; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at);
         return f;
     }
 };
@@ -388,6 +397,25 @@ __device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int r
         *reinterpret_cast<vec_t<bf16_t, 4 * CT>*>(base + 2 * (((int64_t)i * rows + row0 + n) * vpad + col0 + 4 * CT * p)) = o;
     }
 }
+// The same from operands (lane: column col_of(j, n), 32 rows): rows row0 .. of NO planes.  PAIRED: the 16 rows of one half, else both halves
+template <int NO, int CT, bool PAIRED, int NF>
+__device__ __forceinline__ void store_frag(char* base, int rows, int vpad, int row0, int half, int col0, const Frag<NF> (&f)[CT], int n, int p) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    if (col0 >= vpad) return;
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int hh = 0; hh < (PAIRED ? 1 : 2); ++hh) {
+            vec_t<bf16_t, 4 * CT> o;
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[j].p[i], unit_frag<PAIRED>(PAIRED ? half : hh, n, p), zero, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[4 * j + e] = static_cast<bf16_t>(x[e]);
+            }
+            *reinterpret_cast<vec_t<bf16_t, 4 * CT>*>(base + 2 * (((int64_t)i * rows + row0 + 16 * hh + n) * vpad + col0 + 4 * CT * p)) = o;
+        }
+}
 template <typename T, int CT>
 __device__ __forceinline__ void store_cols(T* row, int c, int n, const f32x4 (&v)[CT]) {   // columns c .. c + 4 CT - 1 of a row of n
     T o[4 * CT];
@@ -401,6 +429,34 @@ __device__ __forceinline__ void store_cols(T* row, int c, int n, const f32x4 (&v
             if (c + e < n) row[c + e] = o[e];
     }
 }
+
+// A wave's 16 tokens x 16 CT columns of an output, from accumulators [column 4 p + r of tile j][token n] through LDS (a VTile's place) to whole lines
+template <typename T, int CT, bool WHOLE>
+struct OTile {
+    char* base;
+    static constexpr int kRow = VTile<T, CT, WHOLE>::kRow;
+    __device__ __forceinline__ void put(const f32x4 (&v)[CT], int lane) const {
+        vec_t<T, 4 * CT> o;
+#pragma unroll
+        for (int e = 0; e < 4 * CT; ++e) o[e] = static_cast<T>(v[e >> 2][e & 3]);
+        __builtin_memcpy(__builtin_assume_aligned(base + (lane & 15) * kRow + 4 * CT * (lane >> 4) * (int)sizeof(T), 8), &o, sizeof(o));
+    }
+    __device__ __forceinline__ void store(const Rows<T>& out, int first, int len, int col0, int dv, int lane) const {
+        const int id = lane & (32 * CT - 1), row = id / (2 * CT), c = col0 + 8 * (id % (2 * CT));
+        Raw8<T> r;
+        __builtin_memcpy(&r, __builtin_assume_aligned(base + row * kRow + 8 * (id % (2 * CT)) * (int)sizeof(T), 16), sizeof(r));
+        if (lane < 32 * CT && first + row < len) {
+            T* const at = const_cast<T*>(out.row(first + row)) + c;
+            if (WHOLE) {
+                if (c < dv) __builtin_memcpy(at, &r, sizeof(r));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < dv) at[e] = r.v[e];
+            }
+        }
+    }
+};
 
 // A walk's workgroup takes 32 columns of a head, or 16 where that leaves half of the CUs without one: a chunk of 16 columns takes 0.7 .. 0.9 of the time of one of
 // 32 (its chain is the same).  (2, 2304, 8 heads, 64 x 64): 32 workgroups 65 us, 64 workgroups 50 us; (8, 8192, 8 heads, 128 x 128): 256 workgroups

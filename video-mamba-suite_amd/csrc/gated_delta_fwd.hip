@@ -4,6 +4,8 @@
 //   gd_scan   the walk over the chunks.  The columns of S (and of V, U, O) never meet: a workgroup owns 16 CT of them for the whole
 //             sequence.  Its four waves split the chunk's 64 tokens and S's dk rows: wave w computes token tile w of K S0, U and O
 //             and dk / 4 rows of S, which stay in its accumulators.
+#include <type_traits>
+
 #include "gated_delta.h"
 
 namespace vms {
@@ -229,200 +231,297 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 // a whole chunk of 16 columns to itself (no exchange, every wave reading all of K, Q, T, M from LDS) took 5.4 us per chunk at dk = 128,
 // four waves on one chunk take 1.5: three barriers, but a quarter of the products in a row and each operand of K, Q, T, M read once, straight
 // from memory into the registers of the one wave that uses it.  K alone also goes through LDS, for its transpose.
+template <typename T, int KP, int CT, int FIT>
+struct ScanLds {   // bytes and places in LDS
+    static constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    static constexpr bool kStaged = !(sizeof(T) == 4 && KP == 128);   // K and Q come through LDS; two tiles of three planes do not fit
+    static constexpr int kK = NX * tile_bytes<KP>(), kPiece = VTile<T, CT, FIT != 0>::kBytes;
+    static constexpr int kQRow = KP * (int)sizeof(T) + 16, kQ = kStaged ? 16 * kQRow : 0;   // per wave
+    static constexpr int S = (kStaged ? 2 : 1) * kK, R = S + Exchange<NS, CT, KP>::kBytes, U = R + Exchange<NS, CT, C>::kBytes, D = U + Exchange<NS, CT, C>::kBytes,
+                         V = D + Exchange<NS, CT, C>::kBytes,           // V, O: one and one per wave and buffer
+                         G = V + 3 * 4 * kPiece, Q = G + 2 * 4 * GateTile::kBytes, kBytes = Q + 4 * kQ;
+    static_assert(kBytes <= 163840, "160 KB of LDS");
+};
+
 template <typename T, int KP, int CT, int FIT, bool TRAIN>
-__global__ __launch_bounds__(256, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
+__global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
     constexpr int KB = KP / 32, DW = KP / 64;   // 32-column blocks of k; 16-row tiles of S per wave
+    constexpr bool WHOLE = FIT != 0;
+    using Lds = ScanLds<T, KP, CT, FIT>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char* const Ks = lds;
-    const Exchange<NS, CT, KP> Sx{Ks + NX * tile_bytes<KP>()};
-    const Exchange<NS, CT, C> Rx{Sx.base + Sx.kBytes}, Ux{Rx.base + Rx.kBytes}, Dx{Ux.base + Ux.kBytes};   // R, U, del U
-    char* const own = Dx.base + Dx.kBytes;   // per wave: v, gates
+    const Exchange<NS, CT, KP> Sx{lds + Lds::S};
+    const Exchange<NS, CT, C> Rx{lds + Lds::R}, Ux{lds + Lds::U}, Dx{lds + Lds::D};   // R, U, del U
 
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
     int pair, slice;
     pair_of(blockIdx.x, p.batch * p.heads, slices, pair, slice);
     const int b = pair / p.heads, h = pair % p.heads, hk = h / (p.heads / p.heads_k);
     const int len = length_of(p, b), nc = (len + C - 1) / C;
     const int col0 = slice * CT * 16;
-    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
-    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
-    const Rows<T> V(p.v, (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride, p.v_seq_stride, len, p.reverse);
-    T* const ob = static_cast<T*>(p.out) + (int64_t)b * p.out_batch_stride + (int64_t)h * p.out_head_stride;
-    const Rows<T> O_(p.out, (int64_t)b * p.out_batch_stride + (int64_t)h * p.out_head_stride, p.out_seq_stride, len, p.reverse);
     char* const ws = static_cast<char*>(p.workspace);
     const int64_t slot0 = (int64_t)pair * l.chunks;
-
-    Raw8<T> kr[KB], qr[KB], kx[KB], qx[KB];   // token 16 w + n: this chunk's, the next one's
-    Frag<NS> tf[2];           // rows 16 w + n of T, M (blocks 0, 1; tiles 0 and 1 have no block 1)
-    Frag<NO> mf[2];
-    VTile<T, CT, FIT != 0> vt{own + w * (VTile<T, CT, FIT != 0>::kBytes + GateTile::kBytes)};
-    GateTile gt{reinterpret_cast<float*>(vt.base + vt.kBytes)};
-    auto fetch_rows = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {
+    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    auto tile = [&](int odd) __attribute__((always_inline)) { return lds + (Lds::kStaged ? odd * Lds::kK : 0); };
+    auto v_at = [&](int odd) __attribute__((always_inline)) { return lds + Lds::V + (4 * odd + w) * Lds::kPiece; };
+    auto g_at = [&](int odd) __attribute__((always_inline)) { return reinterpret_cast<float*>(lds + Lds::G + (4 * odd + w) * GateTile::kBytes); };
+    auto fetch_rows = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {   // operands: token 16 w + n
         const int at = c * C + 16 * w + n;
         const T* const row = x.row(at < len ? at : len - 1);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) r[kb] = fit_load<FIT, T>(row, 32 * kb + 8 * q4, p.dk);
     };
-    auto fetch_small = [&](int c) __attribute__((always_inline)) {
-        vt.fetch(V, c * C + 16 * w, len, col0, p.dv, lane);
-        gt.fetch(reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c), w, lane);
-    };
-    auto hand_small = [&](int c) __attribute__((always_inline)) {   // to this wave itself
-        vt.hand(c * C + 16 * w, len, col0, p.dv, lane, true);
-        gt.hand(lane);
-    };
-    auto fetch_t = [&](int c) __attribute__((always_inline)) {
-        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot;
-        tf[0] = tri_rows<NS>(at, w, 0, lane);
-        tf[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
-    };
-    auto fetch_m = [&](int c) __attribute__((always_inline)) {
-        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + NS * kTri;
-        mf[0] = tri_rows<NO>(at, w, 0, lane);
-        mf[1] = tri_rows<NO>(at, w, w >= 2 ? 1 : 0, lane);
-    };
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 S[DW][CT];   // rows 16 (DW w + d) + 4 q4 + r, column n
-    const int64_t sbase = (int64_t)pair * p.dk * p.dv;
+    // the same 16 rows by lines: piece i of 8 columns
+    auto piece_row = [&](int i) __attribute__((always_inline)) { return (lane + 64 * i) / (KP / 8); };
+    auto piece_col = [&](int i) __attribute__((always_inline)) { return 8 * ((lane + 64 * i) % (KP / 8)); };
+    auto fetch_lines = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < DW; ++d)
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
-                S[d][j][r] = p.initial_state && row < p.dk && col < p.dv ? p.initial_state[sbase + (int64_t)row * p.dv + col] : 0.f;
-            }
-            Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
+        for (int i = 0; i < KB; ++i) {
+            const int at = c * C + 16 * w + piece_row(i);
+            r[i] = fit_load<FIT, T>(x.row(at < len ? at : len - 1), piece_col(i), p.dk);
         }
-    if (nc > 0) {
-        fetch_rows(K, 0, kx);
-        fetch_rows(Q, 0, qx);
-        fetch_small(0);
-        fetch_t(0);
-        fetch_m(0);
-    }
-    for (int c = 0; c < nc; ++c) {
-        const int next = c + 1 < nc ? c + 1 : c;   // the last chunk again rather than a branch
-        const int64_t slot = slot0 + c;
-        const bool ok_n = c * C + 16 * w + n < len;
+    };
+    // Both sides below meet at three barriers per chunk: S is there; R is there; U is there.  Loads are asked for two chunks ahead.
+    if (wave < 4) {
+        // ---- the chain: U, S
+        __builtin_amdgcn_s_setprio(2);   // the other wave of this SIMD has slack
+        f32x4 S[DW][CT];   // rows 16 (DW w + d) + 4 q4 + r, column n
+        const int64_t sbase = (int64_t)pair * p.dk * p.dv;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) { kr[kb] = kx[kb]; qr[kb] = qx[kb]; }
-        hand_small(c);
-        __syncthreads();   // S is there; K's tile is no longer read
-        // Loads return in order, stores among them, and the memory pipe takes 20 .. 50 cycles for each instruction of a wave: what a phase waits
-        // for is asked for a chunk earlier, a few instructions at a time
-        fetch_rows(K, next, kx);
-        fetch_small(next);
-        // ---- P = K S0, O = S0^T Q^T, R
-        f32x4 P[CT], O[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) { P[j] = zero; O[j] = zero; }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            const Frag<NX> kf = planes_of<T>(fit_clear<FIT, T>(kr[kb], 32 * kb + 8 * q4, p.dk));
-            const Frag<NX> qf = planes_of<T>(fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk));
-            tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
+        for (int d = 0; d < DW; ++d)
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
-                const Frag<NS> sf = Sx.get(j, n, 32 * kb + 8 * q4);
-                mma<NS>(P[j], kf, sf);    // [token][v]
-                mma<NO>(O[j], sf, qf);    // [v][token]: the lanes of a store hold 4 consecutive v
-            }
-        }
-        const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
-        const float sg = p.scale * gt.gam(n), glast = gt.last();
-        f32x4 vv[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) vv[j] = vt.get(j, n, q4);
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            f32x4 R;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                R[r] = be[r] * fmaf(-ga[r], P[j][r], vv[j][r]);   // beta = 0 behind the end
-            }
-            Rx.put(j, n, paired(w, q4), R);
-        }
-        fetch_rows(Q, next, qx);
-        if constexpr (TRAIN) {   // S0 by rows: 4 consecutive columns per lane
-#pragma unroll
-            for (int d = 0; d < DW; ++d) store_rows<NO, CT>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0, S[d], n, q4);
-        }
-        __syncthreads();
-        // ---- U = T R
-        f32x4 U[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            U[j] = zero;
-            mma<NS>(U[j], tf[0], Rx.get(j, n, 8 * q4));
-        }
-        if (w >= 2)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) mma<NS>(U[j], tf[1], Rx.get(j, n, 32 + 8 * q4));
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            const f32x4 x = U[j] * de;
-            Dx.put(j, n, paired(w, q4), x);
-            Ux.put(j, n, paired(w, q4), U[j]);
-        }
-        fetch_t(next);
-        __syncthreads();
-        // ---- S1 = gam S0 + K^T (del U)
-#pragma unroll
-        for (int d = 0; d < DW; ++d)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) S[d][j] *= glast;
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
-            Frag<NS> uf[CT];
-#pragma unroll
-            for (int j = 0; j < CT; ++j) uf[j] = Dx.get(j, n, 32 * tb + 8 * q4);
-#pragma unroll
-            for (int d = 0; d < DW; ++d) {
-                const Frag<NX> kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
-#pragma unroll
-                for (int j = 0; j < CT; ++j) mma<NS>(S[d][j], kc, uf[j]);
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < DW; ++d)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
-        // ---- O += M U
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            O[j] *= sg;
-            mma<NS>(O[j], Ux.get(j, n, 8 * q4), mf[0]);   // (two planes of U keep the error of O at what M's one leaves)
-        }
-        if (w >= 2)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) mma<NS>(O[j], Ux.get(j, n, 32 + 8 * q4), mf[1]);
-        fetch_m(next);
-        if (ok_n) {
-            T* const row = const_cast<T*>(O_.row(c * C + 16 * w + n));
-            store_cols<T, CT>(row, col0 + 4 * CT * q4, p.dv, O);
-        }
-        if constexpr (TRAIN) {
-            store_rows<NO, CT>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, col0, U, n, q4);
-        }
-    }
-    if (p.final_state) {
-#pragma unroll
-        for (int d = 0; d < DW; ++d)
-#pragma unroll
-            for (int j = 0; j < CT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
-                    if (row < p.dk && col < p.dv) p.final_state[sbase + (int64_t)row * p.dv + col] = S[d][j][r];
+                    S[d][j][r] = p.initial_state && row < p.dk && col < p.dv ? p.initial_state[sbase + (int64_t)row * p.dv + col] : 0.f;
                 }
+                Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
+            }
+        auto fetch_t = [&](int c, Frag<NS> (&t)[2]) __attribute__((always_inline)) {   // rows 16 w + n of T (blocks 0, 1; tiles 0 and 1 have no block 1)
+            const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot;
+            t[0] = tri_rows<NS>(at, w, 0, lane);
+            t[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
+        };
+        Raw8<T> kr[KB];
+        auto chunk = [&](int c, auto odd_c, Frag<NS> (&tf)[2]) __attribute__((always_inline)) {
+            constexpr int odd = decltype(odd_c)::value;
+            char* const Ks = tile(odd);
+            VTile<T, CT, WHOLE> vt;
+            vt.base = v_at(odd);
+            GateTile gt;
+            gt.base = g_at(odd);
+            __syncthreads();   // S is there; (not staged) K's tile is no longer read
+            f32x4 P[CT];   // K S0
+#pragma unroll
+            for (int j = 0; j < CT; ++j) P[j] = zero;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                Frag<NX> kf;
+                if constexpr (Lds::kStaged) {
+                    kf = tile_rows<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4);
+                } else {
+                    kf = planes_of<T>(fit_clear<FIT, T>(kr[kb], 32 * kb + 8 * q4, p.dk));
+                    tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
+                }
+#pragma unroll
+                for (int j = 0; j < CT; ++j) mma<NS>(P[j], kf, Sx.get(j, n, 32 * kb + 8 * q4));
+            }
+            if constexpr (!Lds::kStaged) fetch_rows(K, c + 1 < nc ? c + 1 : c, kr);
+            const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
+            const float glast = gt.last();
+            f32x4 vv[CT];
+#pragma unroll
+            for (int j = 0; j < CT; ++j) vv[j] = vt.get(j, n, q4);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                f32x4 R;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) R[r] = be[r] * fmaf(-ga[r], P[j][r], vv[j][r]);   // beta = 0 behind the end
+                Rx.put(j, n, paired(w, q4), R);
+            }
+            __syncthreads();
+            f32x4 U[CT];   // T R
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                U[j] = zero;
+                mma<NS>(U[j], tf[0], Rx.get(j, n, 8 * q4));
+            }
+            if (w >= 2)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) mma<NS>(U[j], tf[1], Rx.get(j, n, 32 + 8 * q4));
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                const f32x4 x = U[j] * de;
+                Dx.put(j, n, paired(w, q4), x);
+                Ux.put(j, n, paired(w, q4), U[j]);
+            }
+            __syncthreads();
+            // S1 = gam S0 + K^T (del U)
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) S[d][j] *= glast;
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+                Frag<NS> uf[CT];
+#pragma unroll
+                for (int j = 0; j < CT; ++j) uf[j] = Dx.get(j, n, 32 * tb + 8 * q4);
+#pragma unroll
+                for (int d = 0; d < DW; ++d) {
+                    const Frag<NX> kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) mma<NS>(S[d][j], kc, uf[j]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, S[d][j]);
+            fetch_t(c + 2 < nc ? c + 2 : nc - 1, tf);
+        };
+        if (nc > 0) {
+            Frag<NS> t0[2], t1[2];
+            if constexpr (!Lds::kStaged) fetch_rows(K, 0, kr);
+            fetch_t(0, t0);
+            fetch_t(nc > 1 ? 1 : 0, t1);
+            for (int c = 0;;) {
+                chunk(c, std::integral_constant<int, 0>{}, t0);
+                if (++c == nc) break;
+                chunk(c, std::integral_constant<int, 1>{}, t1);
+                if (++c == nc) break;
+            }
+        }
+        if (p.final_state) {
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
+                        if (row < p.dk && col < p.dv) p.final_state[sbase + (int64_t)row * p.dv + col] = S[d][j][r];
+                    }
+        }
+    } else {
+        // ---- the outputs (O, and S0 and U for the backward), and what both sides read
+        const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+        const Rows<T> V(p.v, (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride, p.v_seq_stride, len, p.reverse);
+        const Rows<T> O_(p.out, (int64_t)b * p.out_batch_stride + (int64_t)h * p.out_head_stride, p.out_seq_stride, len, p.reverse);
+        const Gates* const gates = reinterpret_cast<const Gates*>(ws + l.gates) + slot0;
+        char* const Qs = lds + Lds::Q + w * Lds::kQ;
+        struct Ahead {
+            Raw8<T> k[KB], q[KB];   // token 16 w + n, or its lines
+            VTile<T, CT, WHOLE> v;
+            GateTile g;
+        };
+        auto fetch_m = [&](int c, Frag<NO> (&m)[2]) __attribute__((always_inline)) {   // rows 16 w + n of M
+            const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + NS * kTri;
+            m[0] = tri_rows<NO>(at, w, 0, lane);
+            m[1] = tri_rows<NO>(at, w, w >= 2 ? 1 : 0, lane);
+        };
+        auto fetch_q = [&](int c, Ahead& a) __attribute__((always_inline)) {
+            if constexpr (Lds::kStaged) fetch_lines(Q, c, a.q);
+        };
+        auto fetch_kv = [&](int c, Ahead& a) __attribute__((always_inline)) {
+            if constexpr (Lds::kStaged) fetch_lines(K, c, a.k);
+            a.v.fetch(V, c * C + 16 * w, len, col0, p.dv, lane);
+            a.g.fetch(reinterpret_cast<const float*>(gates + c), w, lane);
+        };
+        auto hand = [&](int c, auto odd_c, Ahead& a) __attribute__((always_inline)) {   // into LDS; Q, V's and the gates' places are this wave's and its twin's
+            constexpr int odd = decltype(odd_c)::value;
+            if constexpr (Lds::kStaged) {
+#pragma unroll
+                for (int i = 0; i < KB; ++i) {
+                    tile_put<KP, NX>(tile(odd), 16 * w + piece_row(i), piece_col(i), planes_of<T>(fit_clear<FIT, T>(a.k[i], piece_col(i), p.dk)));
+                    const Raw8<T> x = fit_clear<FIT, T>(a.q[i], piece_col(i), p.dk);
+                    __builtin_memcpy(__builtin_assume_aligned(Qs + piece_row(i) * Lds::kQRow + piece_col(i) * (int)sizeof(T), 16), &x, sizeof(x));
+                }
+            }
+            a.v.base = v_at(odd);
+            a.g.base = g_at(odd);
+            a.v.hand(c * C + 16 * w, len, col0, p.dv, lane, true);
+            a.g.hand(lane);
+        };
+        const OTile<T, CT, WHOLE> ot{v_at(2)};
+        Raw8<T> qr[KB];
+        auto chunk = [&](int c, auto odd_c, Ahead& other, Frag<NO> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
+            constexpr int odd = decltype(odd_c)::value;
+            const int64_t slot = slot0 + c;
+            __syncthreads();
+            if (c > 0) ot.store(O_, (c - 1) * C + 16 * w, len, col0, p.dv, lane);
+            const float sg = p.scale * g_at(odd)[n];
+            f32x4 O[CT];   // S0^T Q^T, [v][token]: a lane holds 4 consecutive v
+#pragma unroll
+            for (int j = 0; j < CT; ++j) O[j] = zero;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                Raw8<T> x;
+                if constexpr (Lds::kStaged) __builtin_memcpy(&x, __builtin_assume_aligned(Qs + n * Lds::kQRow + (32 * kb + 8 * q4) * (int)sizeof(T), 16), sizeof(x));
+                else x = fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk);
+                const Frag<NX> qf = planes_of<T>(x);
+                Frag<NO> sf[CT];
+#pragma unroll
+                for (int j = 0; j < CT; ++j) {
+                    sf[j] = Sx.template get<NO>(j, n, 32 * kb + 8 * q4);
+                    mma<NO>(O[j], sf[j], qf);
+                }
+                if constexpr (TRAIN) {
+                    if ((kb & 3) == w) store_frag<NO, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * kb, 0, col0, sf, n, q4);
+                }
+            }
+            if constexpr (!Lds::kStaged) fetch_rows(Q, c + 1 < nc ? c + 1 : c, qr);
+            __syncthreads();
+            hand(c + 1, std::integral_constant<int, 1 - odd>{}, other);
+            const int next = c + 3 < nc ? c + 3 : nc - 1;
+            fetch_kv(next, other);
+            __syncthreads();
+            fetch_q(next, other);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) O[j] *= sg;
+            // O += M U (two planes of U keep the error of O at what M's one leaves)
+            Frag<NS> uf[CT];
+#pragma unroll
+            for (int j = 0; j < CT; ++j) uf[j] = Ux.get(j, n, 8 * q4);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) mma<NS>(O[j], uf[j], mf[0]);
+            if (w >= 2) {
+#pragma unroll
+                for (int j = 0; j < CT; ++j) uf[j] = Ux.get(j, n, 32 + 8 * q4);
+#pragma unroll
+                for (int j = 0; j < CT; ++j) mma<NS>(O[j], uf[j], mf[1]);
+            }
+            fetch_m(c + 2 < nc ? c + 2 : nc - 1, mf);
+            ot.put(O, lane);
+            if constexpr (TRAIN) store_frag<NO, CT, true>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, w & 1, col0, uf, n, q4);
+        };
+        if (nc > 0) {
+            Ahead a0, a1;
+            Frag<NO> m0[2], m1[2];
+            if constexpr (!Lds::kStaged) fetch_rows(Q, 0, qr);
+            auto fetch = [&](int c, Ahead& a) __attribute__((always_inline)) { fetch_kv(c, a); fetch_q(c, a); };
+            fetch(0, a0);
+            fetch(nc > 1 ? 1 : 0, a1);
+            fetch_m(0, m0);
+            fetch_m(nc > 1 ? 1 : 0, m1);
+            hand(0, std::integral_constant<int, 0>{}, a0);
+            fetch(nc > 2 ? 2 : nc - 1, a0);
+            for (int c = 0;;) {
+                chunk(c, std::integral_constant<int, 0>{}, a1, m0);
+                if (++c == nc) break;
+                chunk(c, std::integral_constant<int, 1>{}, a0, m1);
+                if (++c == nc) break;
+            }
+            ot.store(O_, (nc - 1) * C + 16 * w, len, col0, p.dv, lane);
+        }
+        // padding behind the sequence's end
+        T* const ob = static_cast<T*>(p.out) + (int64_t)b * p.out_batch_stride + (int64_t)h * p.out_head_stride;
+        const int cn = p.dv - col0 < CT * 16 ? p.dv - col0 : CT * 16;
+        for (int t = len + w; t < p.seqlen; t += 4)
+            for (int cc = lane; cc < cn; cc += 64) ob[(int64_t)t * p.out_seq_stride + col0 + cc] = static_cast<T>(0.f);
     }
-    // padding behind the sequence's end
-    const int cn = p.dv - col0 < CT * 16 ? p.dv - col0 : CT * 16;
-    for (int t = len + w; t < p.seqlen; t += 4)
-        for (int cc = lane; cc < cn; cc += 64) ob[(int64_t)t * p.out_seq_stride + col0 + cc] = static_cast<T>(0.f);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -446,13 +545,11 @@ int validate(const vms_gated_delta_params& p) {
 
 template <typename T, int KP, int CT, int FIT, bool TRAIN>
 static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStream_t s) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int lds = NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + 3 * Exchange<NS, CT, C>::kBytes + 4 * (VTile<T, CT, true>::kBytes + GateTile::kBytes);
-    static_assert(lds <= 163840, "160 KB of LDS");
+    constexpr int lds = ScanLds<T, KP, CT, FIT>::kBytes;
     static PerDeviceOnce once;
     if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, CT, FIT, TRAIN>), lds)) return rc;
     const int slices = (l.vpad + CT * 16 - 1) / (CT * 16);
-    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, FIT, TRAIN>), dim3(p.batch * p.heads * slices), dim3(256), lds, s, p, l, slices);
+    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, FIT, TRAIN>), dim3(p.batch * p.heads * slices), dim3(512), lds, s, p, l, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
