@@ -425,8 +425,10 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
         auto fetch_q = [&](int c, Ahead& a) __attribute__((always_inline)) {
             if constexpr (Lds::kStaged) fetch_lines(Q, c, a.q);
         };
-        auto fetch_kv = [&](int c, Ahead& a) __attribute__((always_inline)) {
+        auto fetch_k = [&](int c, Ahead& a) __attribute__((always_inline)) {
             if constexpr (Lds::kStaged) fetch_lines(K, c, a.k);
+        };
+        auto fetch_v = [&](int c, Ahead& a) __attribute__((always_inline)) {
             a.v.fetch(V, c * C + 16 * w, len, col0, p.dv, lane);
             a.g.fetch(reinterpret_cast<const float*>(gates + c), w, lane);
         };
@@ -447,7 +449,7 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
         };
         const OTile<T, CT, WHOLE> ot{v_at(2)};
         Raw8<T> qr[KB];
-        auto chunk = [&](int c, auto odd_c, Ahead& other, Frag<NO> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
+        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NO> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
             constexpr int odd = decltype(odd_c)::value;
             const int64_t slot = slot0 + c;
             __syncthreads();
@@ -462,21 +464,23 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
                 if constexpr (Lds::kStaged) __builtin_memcpy(&x, __builtin_assume_aligned(Qs + n * Lds::kQRow + (32 * kb + 8 * q4) * (int)sizeof(T), 16), sizeof(x));
                 else x = fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk);
                 const Frag<NX> qf = planes_of<T>(x);
-                Frag<NO> sf[CT];
 #pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    sf[j] = Sx.template get<NO>(j, n, 32 * kb + 8 * q4);
-                    mma<NO>(O[j], sf[j], qf);
-                }
-                if constexpr (TRAIN) {
-                    if ((kb & 3) == w) store_frag<NO, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * kb, 0, col0, sf, n, q4);
+                for (int j = 0; j < CT; ++j) mma<NO>(O[j], Sx.template get<NO>(j, n, 32 * kb + 8 * q4), qf);
+            }
+            if constexpr (TRAIN) {
+                if (w < KB) {   // S0, 32 rows per wave
+                    Frag<NO> sf[CT];
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) sf[j] = Sx.template get<NO>(j, n, 32 * w + 8 * q4);
+                    store_frag<NO, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
                 }
             }
             if constexpr (!Lds::kStaged) fetch_rows(Q, c + 1 < nc ? c + 1 : c, qr);
+            fetch_k(c + 2 < nc ? c + 2 : nc - 1, mine);
             __syncthreads();
             hand(c + 1, std::integral_constant<int, 1 - odd>{}, other);
             const int next = c + 3 < nc ? c + 3 : nc - 1;
-            fetch_kv(next, other);
+            fetch_v(next, other);
             __syncthreads();
             fetch_q(next, other);
 #pragma unroll
@@ -501,17 +505,18 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
             Ahead a0, a1;
             Frag<NO> m0[2], m1[2];
             if constexpr (!Lds::kStaged) fetch_rows(Q, 0, qr);
-            auto fetch = [&](int c, Ahead& a) __attribute__((always_inline)) { fetch_kv(c, a); fetch_q(c, a); };
+            auto fetch = [&](int c, Ahead& a) __attribute__((always_inline)) { fetch_k(c, a); fetch_v(c, a); fetch_q(c, a); };
             fetch(0, a0);
             fetch(nc > 1 ? 1 : 0, a1);
             fetch_m(0, m0);
             fetch_m(nc > 1 ? 1 : 0, m1);
             hand(0, std::integral_constant<int, 0>{}, a0);
-            fetch(nc > 2 ? 2 : nc - 1, a0);
+            fetch_v(nc > 2 ? 2 : nc - 1, a0);
+            fetch_q(nc > 2 ? 2 : nc - 1, a0);
             for (int c = 0;;) {
-                chunk(c, std::integral_constant<int, 0>{}, a1, m0);
+                chunk(c, std::integral_constant<int, 0>{}, a0, a1, m0);
                 if (++c == nc) break;
-                chunk(c, std::integral_constant<int, 1>{}, a0, m1);
+                chunk(c, std::integral_constant<int, 1>{}, a1, a0, m1);
                 if (++c == nc) break;
             }
             ot.store(O_, (nc - 1) * C + 16 * w, len, col0, p.dv, lane);
