@@ -25,205 +25,307 @@ struct BwdArgs {   // what the kernels need of vms_gated_delta_bwd_params (one k
 };
 
 // ---- the walk over the chunks, from the end ------------------------------------------------------------------
-// Split among the four waves as the forward's walk: wave w has token tile w of dU and Y and dk / 4 rows of dS.  Three exchanges per chunk: dS, dU, Y;
-// dO of the next chunk is handed over while dS is updated, Q and K go through LDS for their transposes.
+// Split among eight waves as the forward's walk: of the chain's four, wave w has token tile w of dU and Y and dk / 4 rows of dS; the other four load, make
+// what depends on no dS (M^T dO, the planes of dO and of scale gam dO) and store.
 template <typename T, int KP, int CT, int FIT>
-__global__ __launch_bounds__(256, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
+struct BwdScanLds {   // bytes and places in LDS
+    static constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    static constexpr int kK = NX * tile_bytes<KP>(), kPiece = VTile<T, CT, FIT != 0>::kBytes, kSum = 4 * CT * 1024;
+    static constexpr int S = 0, O = S + Exchange<NS, CT, KP>::kBytes, G = O + Exchange<NX, CT, C>::kBytes, U = G + Exchange<NS, CT, C>::kBytes,
+                         Y = U + Exchange<NS, CT, C>::kBytes, E = Y + Exchange<NS, CT, C>::kBytes, V = E + kSum, B = V + 4 * kPiece, K = B + 2 * 4 * GateTile::kBytes;
+    static constexpr bool kStaged = K + 4 * kK <= 163840;   // two tiles each of K and Q; else one each, and K straight into the chain's registers
+    static constexpr int Q = K + (kStaged ? 2 : 1) * kK, kBytes = Q + (kStaged ? 2 : 1) * kK;
+};
+
+template <typename T, int KP, int CT, int FIT>
+__global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
     constexpr int KB = KP / 32, DW = KP / 64;
+    constexpr bool WHOLE = FIT != 0;
+    using Lds = BwdScanLds<T, KP, CT, FIT>;
+    static_assert(Lds::kBytes <= 163840, "160 KB of LDS");
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char* const Ks = lds;
-    char* const Qs = Ks + NX * tile_bytes<KP>();
-    const Exchange<NS, CT, KP> Sx{Qs + NX * tile_bytes<KP>()};
-    const Exchange<NX, CT, C> Ox{Sx.base + Sx.kBytes};                                                                 // dO
-    const Exchange<NS, CT, C> Gx{Ox.base + Ox.kBytes}, Ux{Gx.base + Gx.kBytes}, Yx{Ux.base + Ux.kBytes};   // scale gam dO, dU, -beta gam Y
-    char* const own = Yx.base + Yx.kBytes;   // per wave: dO, gates
+    const Exchange<NS, CT, KP> Sx{lds + Lds::S};
+    const Exchange<NX, CT, C> Ox{lds + Lds::O};                                        // dO
+    const Exchange<NS, CT, C> Gx{lds + Lds::G}, Ux{lds + Lds::U}, Yx{lds + Lds::Y};   // scale gam dO, dU, -beta gam Y
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
     int pair, slice;
     pair_of(blockIdx.x, p.batch * p.heads, slices, pair, slice);
     const int b = pair / p.heads, h = pair % p.heads, hk = h / (p.heads / p.heads_k);
     const int len = length_of(p, b), nc = (len + C - 1) / C;
     const int col0 = slice * CT * 16;
-    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
     const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
-    const Rows<T> dO(a.q.dout, (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride, a.q.dout_seq_stride, len, p.reverse);
-    const int64_t dv_seq = (int64_t)p.heads * p.dv;
-    T* const dvb = static_cast<T*>(a.q.dv) + ((int64_t)b * p.seqlen * p.heads + h) * p.dv;
     const char* const ws = static_cast<const char*>(p.workspace);
     char* const wb = static_cast<char*>(a.q.workspace);
     const int64_t slot0 = (int64_t)pair * l.chunks;
-
-    Raw8<T> kr[KB], qr[KB], kx[KB], qx[KB];   // token 16 w + n: this chunk's, the next one's
-    Frag<NS> tf[2], mf[2];    // columns 16 w + n of T, M (row blocks 0, 1; tiles 2 and 3 have no block 0)
-    VTile<T, CT, FIT != 0> ot{own + w * (VTile<T, CT, FIT != 0>::kBytes + GateTile::kBytes)};   // dO
-    GateTile gt{reinterpret_cast<float*>(ot.base + ot.kBytes)};
-    auto fetch_rows = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    auto k_tile = [&](int odd) __attribute__((always_inline)) { return lds + Lds::K + (Lds::kStaged ? odd * Lds::kK : 0); };
+    auto q_tile = [&](int odd) __attribute__((always_inline)) { return lds + Lds::Q + (Lds::kStaged ? odd * Lds::kK : 0); };
+    auto g_at = [&](int odd) __attribute__((always_inline)) { return GateTile{reinterpret_cast<float*>(lds + Lds::B + (4 * odd + w) * GateTile::kBytes), 0.f}; };
+    f32x4* const sums = reinterpret_cast<f32x4*>(lds + Lds::E) + 64 * CT * w + lane;   // M^T dO to the chain, Y from it: fp32, lane by lane
+    auto fetch_rows = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {   // operands: token 16 w + n
         const int at = c * C + 16 * w + n;
         const T* const row = x.row(at < len ? at : len - 1);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) r[kb] = fit_load<FIT, T>(row, 32 * kb + 8 * q4, p.dk);
     };
-    auto fetch_small = [&](int c) __attribute__((always_inline)) {
-        ot.fetch(dO, c * C + 16 * w, len, col0, p.dv, lane);
-        gt.fetch(reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c), w, lane);
+    auto piece_row = [&](int i) __attribute__((always_inline)) { return (lane + 64 * i) / (KP / 8); };   // the same 16 rows by lines: piece i of 8 columns
+    auto piece_col = [&](int i) __attribute__((always_inline)) { return 8 * ((lane + 64 * i) % (KP / 8)); };
+    auto fetch_lines = [&](const Rows<T>& x, int c, Raw8<T> (&r)[KB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+            const int at = c * C + 16 * w + piece_row(i);
+            r[i] = fit_load<FIT, T>(x.row(at < len ? at : len - 1), piece_col(i), p.dk);
+        }
     };
-    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // first: NS + NO T, 2 NS + NO M (their transposes)
-        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;
+    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // columns 16 w + n (row blocks 0, 1; tiles 2 and 3 have no block 0)
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;            // first: NS + NO T, 2 NS + NO M (their transposes)
         f[0] = tri_cols<NS>(at, w, w >= 2 ? 1 : 0, lane);
         f[1] = tri_cols<NS>(at, w, 1, lane);
     };
-    f32x4 out_grad[CT];   // dO of this wave's tokens
-    auto hand_small = [&](int c) __attribute__((always_inline)) {   // gates and dO to this wave, dO to the others
-        ot.hand(c * C + 16 * w, len, col0, p.dv, lane, false);
-        gt.hand(lane);
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            out_grad[j] = ot.get(j, n, q4);
-            Ox.put(j, n, paired(w, q4), out_grad[j]);
-        }
-    };
-
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 dS[DW][CT];
-    const int64_t sbase = (int64_t)pair * p.dk * p.dv;
-#pragma unroll
-    for (int d = 0; d < DW; ++d)
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
-                dS[d][j][r] = a.q.dfinal_state && row < p.dk && col < p.dv ? a.q.dfinal_state[sbase + (int64_t)row * p.dv + col] : 0.f;
-            }
-            Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
-        }
-    if (nc > 0) {
-        fetch_rows(K, nc - 1, kx);
-        fetch_rows(Q, nc - 1, qx);
-        fetch_small(nc - 1);
-        fetch_tri(nc - 1, 2 * NS + NO, mf);
-        fetch_tri(nc - 1, NS + NO, tf);
-        hand_small(nc - 1);
-    }
-    for (int c = nc - 1; c >= 0; --c) {
-        const int next = c > 0 ? c - 1 : 0;   // the first chunk again rather than a branch
-        const int64_t slot = slot0 + c;
-        const bool ok_n = c * C + 16 * w + n < len;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) { kr[kb] = kx[kb]; qr[kb] = qx[kb]; }
-        const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
-        const float glast = gt.last();
-        __syncthreads();   // dS and dO are there; the tiles of K and Q are no longer read
-        fetch_rows(K, next, kx);   // (a few loads at a time, a chunk ahead: gd_scan)
-        fetch_small(next);
-        // ---- dU = del K dS1 + M^T dO
-        f32x4 dU[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) dU[j] = zero;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            const Frag<NX> kf = planes_of<T>(fit_clear<FIT, T>(kr[kb], 32 * kb + 8 * q4, p.dk));
-            const Frag<NX> qf = planes_of<T>(fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk));
-            tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
-            tile_put<KP, NX>(Qs, 16 * w + n, 32 * kb + 8 * q4, qf);
-#pragma unroll
-            for (int j = 0; j < CT; ++j) mma<NS>(dU[j], kf, Sx.get(j, n, 32 * kb + 8 * q4));
-        }
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            dU[j] *= de;
-            mma<NS>(dU[j], mf[1], Ox.get(j, n, 32 + 8 * q4));
-        }
-        if (w < 2)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) mma<NS>(dU[j], mf[0], Ox.get(j, n, 8 * q4));
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            Ux.put(j, n, paired(w, q4), dU[j]);
-            f32x4 x;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = p.scale * ga[r] * out_grad[j][r];
-            Gx.put(j, n, paired(w, q4), x);
-        }
-        fetch_rows(Q, next, qx);
-        fetch_tri(next, 2 * NS + NO, mf);
-#pragma unroll
-        for (int d = 0; d < DW; ++d) store_rows<NO, CT>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 16 * (DW * w + d), col0, dS[d], n, q4);
-        __syncthreads();
-        // ---- Y = T^T dU, dV = beta Y
-        f32x4 Y[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            Y[j] = zero;
-            mma<NS>(Y[j], tf[1], Ux.get(j, n, 32 + 8 * q4));
-        }
-        if (w < 2)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) mma<NS>(Y[j], tf[0], Ux.get(j, n, 8 * q4));
-        f32x4 V[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            V[j] = be * Y[j];
-            f32x4 x;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = -ga[r] * V[j][r];
-            Yx.put(j, n, paired(w, q4), x);
-        }
-        fetch_tri(next, NS + NO, tf);
-        __syncthreads();
-        // ---- dS0 = gam dS1 + Q^T (scale gam dO) - K^T (beta gam Y)
+    auto before = [&](int c, int by) __attribute__((always_inline)) { return c > by ? c - by : 0; };
+    // Both sides below meet at three barriers per chunk: dS and M^T dO are there; dU is there; Y is there
+    if (wave < 4) {
+        // ---- the chain: dU, Y, dS
+        __builtin_amdgcn_s_setprio(2);   // the other wave of this SIMD has slack
+        f32x4 dS[DW][CT];
+        const int64_t sbase = (int64_t)pair * p.dk * p.dv;
 #pragma unroll
         for (int d = 0; d < DW; ++d)
 #pragma unroll
-            for (int j = 0; j < CT; ++j) dS[d][j] *= glast;
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
-            Frag<NS> gf[CT], yf[CT];
-#pragma unroll
-            for (int j = 0; j < CT; ++j) { gf[j] = Gx.get(j, n, 32 * tb + 8 * q4); yf[j] = Yx.get(j, n, 32 * tb + 8 * q4); }
-#pragma unroll
-            for (int d = 0; d < DW; ++d) {
-                const Frag<NX> qc = tile_cols<KP, NX>(Qs, DW * w + d, tb, n, q4), kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
-#pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    mma<NS>(dS[d][j], qc, gf[j]);
-                    mma<NS>(dS[d][j], kc, yf[j]);
-                }
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < DW; ++d)
-#pragma unroll
-            for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
-        hand_small(next);
-        store_rows<NO, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
-        f32x4 dv[CT];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            const Frag<NO> f = frag_of<NO>(V[j], zero);
-            dv[j] = zero;
-#pragma unroll
-            for (int i = NO - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
-        }
-        if (ok_n) store_cols<T, CT>(dvb + (int64_t)token(c * C + 16 * w + n, len, p.reverse) * dv_seq, col0 + 4 * CT * q4, p.dv, dv);
-    }
-    if (a.q.dinitial_state) {
-#pragma unroll
-        for (int d = 0; d < DW; ++d)
-#pragma unroll
-            for (int j = 0; j < CT; ++j)
+            for (int j = 0; j < CT; ++j) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
-                    if (row < p.dk && col < p.dv) a.q.dinitial_state[sbase + (int64_t)row * p.dv + col] = dS[d][j][r];
+                    dS[d][j][r] = a.q.dfinal_state && row < p.dk && col < p.dv ? a.q.dfinal_state[sbase + (int64_t)row * p.dv + col] : 0.f;
                 }
+                Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
+            }
+        Raw8<T> kr[KB];
+        auto chunk = [&](int c, auto odd_c, Frag<NS> (&tf)[2]) __attribute__((always_inline)) {
+            constexpr int odd = decltype(odd_c)::value;
+            char* const Ks = k_tile(odd);
+            const char* const Qs = q_tile(odd);
+            const GateTile gt = g_at(odd);
+            __syncthreads();   // (not staged) K's tile is no longer read
+            // dU = del K dS1 + M^T dO
+            f32x4 dU[CT];
+#pragma unroll
+            for (int j = 0; j < CT; ++j) dU[j] = zero;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                Frag<NX> kf;
+                if constexpr (Lds::kStaged) {
+                    kf = tile_rows<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4);
+                } else {
+                    kf = planes_of<T>(fit_clear<FIT, T>(kr[kb], 32 * kb + 8 * q4, p.dk));
+                    tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
+                }
+#pragma unroll
+                for (int j = 0; j < CT; ++j) mma<NS>(dU[j], kf, Sx.get(j, n, 32 * kb + 8 * q4));
+            }
+            if constexpr (!Lds::kStaged) fetch_rows(K, before(c, 1), kr);
+            const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
+            const float glast = gt.last();
+#pragma unroll
+            for (int j = 0; j < CT; ++j) Ux.put(j, n, paired(w, q4), dU[j] * de + sums[64 * j]);
+            __syncthreads();
+            // Y = T^T dU
+            f32x4 Y[CT];
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                Y[j] = zero;
+                mma<NS>(Y[j], tf[1], Ux.get(j, n, 32 + 8 * q4));
+            }
+            if (w < 2)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) mma<NS>(Y[j], tf[0], Ux.get(j, n, 8 * q4));
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                sums[64 * j] = Y[j];
+                f32x4 x;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = -ga[r] * (be[r] * Y[j][r]);
+                Yx.put(j, n, paired(w, q4), x);
+            }
+            __syncthreads();
+            // dS0 = gam dS1 + Q^T (scale gam dO) - K^T (beta gam Y)
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) dS[d][j] *= glast;
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+                Frag<NS> gf[CT], yf[CT];
+#pragma unroll
+                for (int j = 0; j < CT; ++j) { gf[j] = Gx.get(j, n, 32 * tb + 8 * q4); yf[j] = Yx.get(j, n, 32 * tb + 8 * q4); }
+#pragma unroll
+                for (int d = 0; d < DW; ++d) {
+                    const Frag<NX> qc = tile_cols<KP, NX>(Qs, DW * w + d, tb, n, q4), kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) {
+                        mma<NS>(dS[d][j], qc, gf[j]);
+                        mma<NS>(dS[d][j], kc, yf[j]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
+            fetch_tri(before(c, 2), NS + NO, tf);
+        };
+        if (nc > 0) {
+            Frag<NS> t0[2], t1[2];
+            if constexpr (!Lds::kStaged) fetch_rows(K, nc - 1, kr);
+            fetch_tri(nc - 1, NS + NO, t0);
+            fetch_tri(before(nc - 1, 1), NS + NO, t1);
+            __syncthreads();   // dO of the last chunk is there, for the other side
+            for (int c = nc - 1;;) {
+                chunk(c, std::integral_constant<int, 0>{}, t0);
+                if (--c < 0) break;
+                chunk(c, std::integral_constant<int, 1>{}, t1);
+                if (--c < 0) break;
+            }
+        }
+        if (a.q.dinitial_state) {
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = 16 * (DW * w + d) + 4 * q4 + r, col = col0 + col_of<CT>(j, n);
+                        if (row < p.dk && col < p.dv) a.q.dinitial_state[sbase + (int64_t)row * p.dv + col] = dS[d][j][r];
+                    }
+        }
+    } else {
+        // ---- what both sides read, dS and Y for the gradients, dV
+        const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+        const Rows<T> dO(a.q.dout, (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride, a.q.dout_seq_stride, len, p.reverse);
+        const int64_t dv_seq = (int64_t)p.heads * p.dv;
+        const Rows<T> dV(a.q.dv, ((int64_t)b * p.seqlen * p.heads + h) * p.dv, dv_seq, len, p.reverse);
+        struct Ahead {
+            Raw8<T> k[KB], q[KB];
+            VTile<T, CT, WHOLE> o;   // dO
+            GateTile g;
+        };
+        const OTile<T, CT, WHOLE> ot{lds + Lds::V + w * Lds::kPiece};   // (dO's place: handed on before dV comes, stored before the next dO)
+        auto fetch_k = [&](int c, Ahead& x) __attribute__((always_inline)) {
+            if constexpr (Lds::kStaged) fetch_lines(K, c, x.k);
+        };
+        auto fetch_q = [&](int c, Ahead& x) __attribute__((always_inline)) {
+            if constexpr (Lds::kStaged) fetch_lines(Q, c, x.q);
+        };
+        auto fetch_small = [&](int c, Ahead& x) __attribute__((always_inline)) {
+            x.o.fetch(dO, c * C + 16 * w, len, col0, p.dv, lane);
+            x.g.fetch(reinterpret_cast<const float*>(reinterpret_cast<const Gates*>(ws + l.gates) + slot0 + c), w, lane);
+        };
+        f32x4 scaled[CT];   // of the chunk that was handed over last: the place of the one before is read until the barrier
+        auto hand = [&](int c, auto odd_c, Ahead& x) __attribute__((always_inline)) {   // into LDS
+            constexpr int odd = decltype(odd_c)::value;
+            if constexpr (Lds::kStaged) {
+#pragma unroll
+                for (int i = 0; i < KB; ++i) {
+                    tile_put<KP, NX>(k_tile(odd), 16 * w + piece_row(i), piece_col(i), planes_of<T>(fit_clear<FIT, T>(x.k[i], piece_col(i), p.dk)));
+                    tile_put<KP, NX>(q_tile(odd), 16 * w + piece_row(i), piece_col(i), planes_of<T>(fit_clear<FIT, T>(x.q[i], piece_col(i), p.dk)));
+                }
+            }
+            x.o.base = lds + Lds::V + w * Lds::kPiece;
+            x.g.base = g_at(odd).base;
+            x.o.hand(c * C + 16 * w, len, col0, p.dv, lane, false);
+            x.g.hand(lane);
+            const f32x4 ga = x.g.four(0, q4);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                const f32x4 g = x.o.get(j, n, q4);
+                Ox.put(j, n, paired(w, q4), g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) scaled[j][r] = p.scale * ga[r] * g[r];
+            }
+        };
+        auto other_grad = [&](const Frag<NS> (&mf)[2]) __attribute__((always_inline)) {   // M^T dO
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                f32x4 e = zero;
+                mma<NS>(e, mf[1], Ox.get(j, n, 32 + 8 * q4));
+                if (w < 2) mma<NS>(e, mf[0], Ox.get(j, n, 8 * q4));
+                sums[64 * j] = e;
+            }
+        };
+        Raw8<T> qr[KB];
+        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NS> (&mf)[2]) __attribute__((always_inline)) {   // other, mf: of chunk c - 1
+            constexpr int odd = decltype(odd_c)::value;
+            const int64_t slot = slot0 + c;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < CT; ++j) Gx.put(j, n, paired(w, q4), scaled[j]);
+            if (c + 1 < nc) ot.store(dV, (c + 1) * C + 16 * w, len, col0, p.dv, lane);
+            if constexpr (!Lds::kStaged) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) tile_put<KP, NX>(q_tile(0), 16 * w + n, 32 * kb + 8 * q4, planes_of<T>(fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk)));
+                fetch_rows(Q, before(c, 1), qr);
+            }
+            if (w < KB) {
+                Frag<NO> sf[CT];
+#pragma unroll
+                for (int j = 0; j < CT; ++j) sf[j] = Sx.template get<NO>(j, n, 32 * w + 8 * q4);
+                store_frag<NO, CT, false>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
+            }
+            fetch_k(before(c, 2), mine);
+            __syncthreads();
+            hand(before(c, 1), std::integral_constant<int, 1 - odd>{}, other);
+            fetch_small(before(c, 3), other);
+            __syncthreads();
+            fetch_q(before(c, 3), other);
+            f32x4 Y[CT], dv[CT];
+            const f32x4 be = g_at(odd).four(1, q4);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) Y[j] = sums[64 * j];
+            other_grad(mf);
+            fetch_tri(before(c, 3), 2 * NS + NO, mf);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+                const Frag<NO> f = frag_of<NO>(be * Y[j], zero);
+                dv[j] = zero;
+#pragma unroll
+                for (int i = NO - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
+            }
+            store_rows<NO, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
+            ot.put(dv, lane);
+        };
+        if (nc > 0) {
+            Ahead a0, a1;
+            Frag<NS> m0[2], m1[2];
+            if constexpr (!Lds::kStaged) fetch_rows(Q, nc - 1, qr);
+            auto fetch = [&](int c, Ahead& x) __attribute__((always_inline)) { fetch_k(c, x); fetch_q(c, x); fetch_small(c, x); };
+            fetch(nc - 1, a0);
+            fetch(before(nc - 1, 1), a1);
+            fetch_tri(nc - 1, 2 * NS + NO, m0);
+            fetch_tri(before(nc - 1, 1), 2 * NS + NO, m1);
+            hand(nc - 1, std::integral_constant<int, 0>{}, a0);
+            fetch_q(before(nc - 1, 2), a0);
+            fetch_small(before(nc - 1, 2), a0);
+            __syncthreads();
+            other_grad(m0);
+            fetch_tri(before(nc - 1, 2), 2 * NS + NO, m0);
+            for (int c = nc - 1;;) {
+                chunk(c, std::integral_constant<int, 0>{}, a0, a1, m1);
+                if (--c < 0) break;
+                chunk(c, std::integral_constant<int, 1>{}, a1, a0, m0);
+                if (--c < 0) break;
+            }
+            ot.store(dV, 16 * w, len, col0, p.dv, lane);
+        }
+        T* const dvb = static_cast<T*>(a.q.dv) + ((int64_t)b * p.seqlen * p.heads + h) * p.dv;   // padding behind the sequence's end
+        const int cn = p.dv - col0 < CT * 16 ? p.dv - col0 : CT * 16;
+        for (int t = len + w; t < p.seqlen; t += 4)
+            for (int cc = lane; cc < cn; cc += 64) dvb[(int64_t)t * dv_seq + col0 + cc] = static_cast<T>(0.f);
     }
-    const int cn = p.dv - col0 < CT * 16 ? p.dv - col0 : CT * 16;
-    for (int t = len + w; t < p.seqlen; t += 4)
-        for (int cc = lane; cc < cn; cc += 64) dvb[(int64_t)t * dv_seq + col0 + cc] = static_cast<T>(0.f);
 }
 
 // ---- dq, dk, dg, dbeta of one chunk --------------------------------------------------------------------------
@@ -559,14 +661,11 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
 // ---- host ----------------------------------------------------------------------------------------------------
 template <typename T, int KP, int CT, int FIT>
 static int bwd_scan_launch(const BwdArgs& a, hipStream_t s) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int lds = 2 * NX * tile_bytes<KP>() + Exchange<NS, CT, KP>::kBytes + Exchange<NX, CT, C>::kBytes + 3 * Exchange<NS, CT, C>::kBytes
-                        + 4 * (VTile<T, CT, true>::kBytes + GateTile::kBytes);
-    static_assert(lds <= 163840, "160 KB of LDS");
+    constexpr int lds = BwdScanLds<T, KP, CT, FIT>::kBytes;
     static PerDeviceOnce once;
     if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, KP, CT, FIT>), lds)) return rc;
     const int slices = (a.l.vpad + CT * 16 - 1) / (CT * 16);
-    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, CT, FIT>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(256), lds, s, a, slices);
+    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, CT, FIT>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(512), lds, s, a, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
