@@ -352,24 +352,6 @@ __device__ __forceinline__ float ld_gate(const void* p, int64_t i, int dt) {
     if (dt == VMS_F16) return static_cast<float>(static_cast<const f16_t*>(p)[i]);
     return static_cast<float>(static_cast<const bf16_t*>(p)[i]);
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* row, int c, int n, const f32x4& v) {   // columns c .. c+3 of a row of n
-    if (c + 4 <= n) {
-        T o[4] = {static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
-        __builtin_memcpy(row + c, o, sizeof(o));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < n) row[c + e] = static_cast<T>(v[e]);
-    }
-}
-__device__ __forceinline__ void store_planes4(char* at, const f32x4& v) {   // an exact bf16 plane that went through unit_frag
-    bf16x4 o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = static_cast<bf16_t>(v[e]);
-    *reinterpret_cast<bf16x4*>(at) = o;
-}
-
 inline int allow_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
     if (bytes <= 65536) return VMS_OK;
     const hipError_t e = once.run([&] { return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
@@ -415,19 +397,6 @@ __device__ __forceinline__ void store_frag(char* base, int rows, int vpad, int r
             }
             *reinterpret_cast<vec_t<bf16_t, 4 * CT>*>(base + 2 * (((int64_t)i * rows + row0 + 16 * hh + n) * vpad + col0 + 4 * CT * p)) = o;
         }
-}
-template <typename T, int CT>
-__device__ __forceinline__ void store_cols(T* row, int c, int n, const f32x4 (&v)[CT]) {   // columns c .. c + 4 CT - 1 of a row of n
-    T o[4 * CT];
-#pragma unroll
-    for (int e = 0; e < 4 * CT; ++e) o[e] = static_cast<T>(v[e >> 2][e & 3]);
-    if (c + 4 * CT <= n) {
-        __builtin_memcpy(row + c, o, sizeof(o));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4 * CT; ++e)
-            if (c + e < n) row[c + e] = o[e];
-    }
 }
 
 // A wave's 16 tokens x 16 CT columns of an output, from accumulators [column 4 p + r of tile j][token n] through LDS (a VTile's place) to whole lines

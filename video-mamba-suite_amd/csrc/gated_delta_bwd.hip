@@ -406,6 +406,35 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     const bool has_s = tid < 4 * KP;
     const int at_p = c * C + prow;
     const bool ok_p = at_p < len;
+    // dQ (left), dK (right): a wave's 16 rows through its own part of Q's or K's tile, which nobody reads any more, to whole lines (8-byte pieces of 16 rows at
+    // once cost the memory pipe 64 accesses a store instead of 16)
+    auto store_grad = [&](const f32x4 (&x)[DT]) __attribute__((always_inline)) {
+        constexpr int PITCH = KP * (int)sizeof(T) + 16;
+        static_assert(C * PITCH <= NX * TB, "a tile's place");
+        char* const mine = (left ? Qs : Ks) + 16 * w * PITCH;
+        T* const base = left ? dqb : dkb;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const T o[4] = {static_cast<T>(x[d][0]), static_cast<T>(x[d][1]), static_cast<T>(x[d][2]), static_cast<T>(x[d][3])};
+            __builtin_memcpy(__builtin_assume_aligned(mine + n * PITCH + (16 * d + 4 * q4) * (int)sizeof(T), 8), o, sizeof(o));
+        }
+#pragma unroll
+        for (int i = 0; i < KP / 32; ++i) {
+            const int id = lane + 64 * i, row = id / (KP / 8), cc = 8 * (id % (KP / 8)), at = c * C + 16 * w + row;
+            Raw8<T> r;
+            __builtin_memcpy(&r, __builtin_assume_aligned(mine + row * PITCH + cc * (int)sizeof(T), 16), sizeof(r));
+            if (at < len) {
+                T* const to = base + token(at, len, p.reverse) * dk_seq + cc;
+                if (WHOLE) {
+                    if (cc < p.dk) __builtin_memcpy(to, &r, sizeof(r));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (cc + e < p.dk) to[e] = r.v[e];
+                }
+            }
+        }
+    };
     f32x4 total[SHARED ? DT : 1];   // dQ (left), dK (right) over the heads
     if constexpr (SHARED)
 #pragma unroll
@@ -643,19 +672,11 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
         if constexpr (SHARED) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) total[d] += A[d];
-        } else if (ok_own) {
-            T* const row = (left ? dqb : dkb) + token(at_own, len, p.reverse) * dk_seq;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) store4<T>(row, 16 * d + 4 * q4, p.dk, A[d]);
+        } else {
+            store_grad(A);
         }
     }
-    if constexpr (SHARED) {
-        if (ok_own) {
-            T* const row = (left ? dqb : dkb) + token(at_own, len, p.reverse) * dk_seq;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) store4<T>(row, 16 * d + 4 * q4, p.dk, total[d]);
-        }
-    }
+    if constexpr (SHARED) store_grad(total);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
