@@ -132,6 +132,14 @@ def test_c_entry_refuses_without_a_gpu():
     assert L.vms_gated_delta_bwd(ctypes.byref(Q), None) < 0 and b"for_backward" in L.vms_last_error()
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    """a length of 2^32 + 3 must not be taken for one of 3"""
+    t = inputs(1, 1, 1, 1, 4, 6, torch.float32, device="cpu")
+    big = {k: v.expand(1, 2**32 + 3, *v.shape[2:]) for k, v in t.items()}
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        gated_delta_rule_fn(**big)
+
+
 # ---- GPU ------------------------------------------------------------------------------------------------------------
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 
@@ -155,6 +163,15 @@ def test_head_sizes(dk, dv, dtype):
 @pytest.mark.parametrize("hk, h, b", [(1, 1, 1), (1, 5, 1), (2, 4, 3), (3, 9, 2), (8, 8, 2)])
 def test_shared_heads(hk, h, b, dtype):
     compare(inputs(b, 70, hk, h, 32, 48, dtype, seed=h))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk, dv", [(40, 72), (64, 64), (50, 70), (100, 96), (104, 90), (128, 128)])
+def test_many_heads(dk, dv, dtype):
+    """enough heads for workgroups of 32 columns, the last one partly outside; lengths of one to four chunks"""
+    lens = torch.tensor([200, 1, 129, 64, 63], dtype=torch.int32, device="cuda")
+    compare(inputs(5, 200, 8, 16, dk, dv, dtype, state=True, seed=dk), seq_lens=lens, reverse=dk % 8 == 0)
 
 
 @pytest.mark.gpu
@@ -380,6 +397,71 @@ def test_on_another_stream_and_captured():
             o = gated_delta_rule_fn(**half)
             assert torch.equal(out, o)
             assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(o, list(half.values()), dout)))
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    """two streams, two host threads: every call has its own workspace"""
+    import threading
+    sets = [inputs(2, 300, 2, 4, 64, 64, torch.bfloat16, seed=i) for i in range(2)]
+    douts = [torch.randn_like(t["v"]) for t in sets]
+
+    def run(i):
+        leaf = {k: v.clone().requires_grad_() for k, v in sets[i].items()}
+        out = gated_delta_rule_fn(**leaf)
+        return [out.detach(), *torch.autograd.grad(out, list(leaf.values()), douts[i])]
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i].append(run(i))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 5 and all(torch.equal(a, b) for g in got[i] for a, b in zip(g, want[i]))
+
+
+@pytest.mark.gpu
+def test_backward_twice_and_one_tensor_for_two():
+    t = inputs(2, 130, 2, 2, 32, 32, torch.bfloat16)
+    leaf = {k: v.clone().requires_grad_() for k, v in t.items()}
+    out = gated_delta_rule_fn(**leaf)
+    dout = torch.randn_like(out)
+    a = torch.autograd.grad(out, list(leaf.values()), dout, retain_graph=True)
+    b = torch.autograd.grad(out, list(leaf.values()), dout)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    x = t["k"].clone().requires_grad_()   # q, k and v one tensor: the gradients add up
+    parts = [t["k"].clone().requires_grad_() for _ in range(3)]
+    one, = torch.autograd.grad(gated_delta_rule_fn(x, x, x, t["g"], t["beta"]), x, dout)
+    three = torch.autograd.grad(gated_delta_rule_fn(*parts, t["g"], t["beta"]), parts, dout)
+    # autograd adds the three in bf16, in some order: one rounding (2^-8) of a sum of two, one of the whole
+    a, b, c = (p.double() for p in three)
+    two = max(x.abs().max().item() for x in (a + b, a + c, b + c))
+    top = (a + b + c).abs().max().item()
+    close(one, a + b + c, 2**-8 * (two + 2**-8 * two + top) / top, "dx")
+
+
+@pytest.mark.gpu
+def test_a_nan_stays_behind_its_chunk():
+    t = inputs(1, 200, 1, 1, 32, 32, torch.bfloat16)
+    want = gated_delta_rule_fn(**t)
+    t["v"][0, 130] = float("nan")
+    got = gated_delta_rule_fn(**t)
+    assert torch.equal(got[0, :128], want[0, :128]) and got[0, 130:].isnan().all()
+
+
+@pytest.mark.gpu
+def test_sizes_beyond_32_bits_are_refused_by_the_compiled_call():
+    t = inputs(1, 1, 1, 1, 4, 6, torch.float32)
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        gated_delta_rule_fn(**{k: v.expand(1, 2**32 + 3, *v.shape[2:]) for k, v in t.items()})
 
 
 @pytest.mark.gpu

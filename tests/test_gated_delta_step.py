@@ -42,6 +42,12 @@ def test_refusals(change, message):
         gated_delta_state_update(state, **t)
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    state, t = step_inputs(1, 1, 1, 4, 6, torch.float32, device="cpu")
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        gated_delta_state_update(state, **{k: v.expand(2**32 + 3, *v.shape[1:]) for k, v in t.items()})
+
+
 def test_states_must_stand_apart():
     from mamba_ssm.ops.gated_delta_rule import _separate_states
     s = torch.zeros(3, 2, 4, 5)

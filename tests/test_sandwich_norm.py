@@ -76,6 +76,13 @@ def test_rows_longer_than_8192_are_refused():
         sandwich_norm_fn(**t)
 
 
+def test_rows_beyond_32_bits_are_refused():
+    t = make((1, 2), torch.float32, torch.float32, device="cpu")
+    t["x"], t["residual"] = (t[k].expand(2**32 + 3, 2) for k in ("x", "residual"))
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        sandwich_norm_fn(**t)
+
+
 def test_c_entry_refuses():
     import ctypes
 

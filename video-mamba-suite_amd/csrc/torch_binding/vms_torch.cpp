@@ -996,6 +996,7 @@ void gated_delta_checks(const Tensor& q, const Tensor& k, const Tensor& v, const
     GD_CHECK(g.sizes() == v.sizes().slice(0, lead + 1) && beta.sizes() == g.sizes(), "g and beta must have the shape of v without its last axis");
     GD_CHECK(k.size(-1) >= 1 && k.size(-1) <= 128, "key heads of 1 to 128 are supported");
     GD_CHECK(v.size(-1) >= 1 && v.size(-1) <= 4096, "value heads of 1 to 4096 are supported");
+    for (const int64_t n : v.sizes()) GD_CHECK(n < (1LL << 31), "axes of less than 2^31 are supported");
     GD_CHECK(q.scalar_type() == v.scalar_type() && k.scalar_type() == v.scalar_type(), "q, k and v must have one dtype");
     GD_CHECK(is_itype(v), "fp32, fp16 or bf16 expected");
     GD_CHECK(g.scalar_type() == beta.scalar_type() && (g.scalar_type() == v.scalar_type() || g.scalar_type() == at::kFloat),

@@ -27,6 +27,7 @@ def _check_inputs(q, k, v, g, beta, lead):
     _check(g.shape == v.shape[:-1] and beta.shape == g.shape, "g and beta must have the shape of v without its last axis")
     _check(1 <= k.shape[-1] <= 128, "key heads of 1 to 128 are supported")
     _check(1 <= v.shape[-1] <= 4096, "value heads of 1 to 4096 are supported")
+    _check(max(v.shape) < 2 ** 31, "axes of less than 2^31 are supported")
     _check(q.dtype == v.dtype and k.dtype == v.dtype, "q, k and v must have one dtype")
     _check(v.dtype in (torch.float32, torch.float16, torch.bfloat16), "fp32, fp16 or bf16 expected")
     _check(g.dtype == beta.dtype and g.dtype in (v.dtype, torch.float32), "g and beta must have one dtype: fp32 or that of v")
@@ -81,7 +82,8 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
     dtype or fp32.  scale: default dk ** -0.5.  1 <= dk <= 128.
     initial_state (batch, heads, dk, dv) fp32.  reverse=True: right to left, as in selective_scan.  seq_lens (batch,) integers on the
     device: the valid tokens of each batch entry, first in memory in either direction (values are clamped to 0 .. seqlen); the rest is padding
-    that leaves the state alone, gives 0 and receives gradient 0.
+    that leaves the state alone, gives 0 and receives gradient 0.  Tokens are worked on 64 at a time: a NaN or infinity in a valid one reaches
+    the outputs of its whole group of 64 and of what follows, none of the groups before.  batch, heads <= 65535, seqlen <= 2^30.
     -> out (batch, seqlen, heads, dv), with return_final_state (out, final_state fp32).  Differentiable once in q, k, v, g, beta, initial_state."""
     fast = _compiled("gated_delta_rule", v.is_cuda and v.numel())
     if fast is not None:

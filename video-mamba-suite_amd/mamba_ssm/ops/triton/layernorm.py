@@ -194,6 +194,7 @@ def sandwich_norm_fn(x, residual, post_weight, pre_weight, post_bias=None, pre_b
         _require(t is None or (tuple(t.shape) == (N,) and t.dtype in floats), "weights and biases must be (N,) in fp32, fp16 or bf16")
     _require(post_weight is not None and pre_weight is not None, "post_weight and pre_weight are required")
     rows = x.numel() // N
+    _require(rows < 2 ** 31, "less than 2^31 rows are supported")
     rows_per_gate = 0
     if gate is not None:
         lead = tuple(gate.shape[:-1])
