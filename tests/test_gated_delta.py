@@ -429,6 +429,22 @@ def test_two_calls_at_once():
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    t = inputs(2, 70, 1, 1, 32, 32, torch.bfloat16)
+    far = dict(t)
+    for k in ("q", "k", "v"):
+        room = torch.empty(2**31 + 8 + 70 * 32, dtype=torch.bfloat16, device="cuda")
+        far[k] = room.as_strided((2, 70, 1, 32), (2**31 + 8, 32, 32, 1))
+        far[k].copy_(t[k])
+    res = []
+    for x in (t, far):
+        leaf = {k: v.detach().requires_grad_() for k, v in x.items()}
+        out = gated_delta_rule_fn(**leaf)
+        res.append([out, *torch.autograd.grad(out, list(leaf.values()), torch.ones_like(out))])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.gpu
 def test_backward_twice_and_one_tensor_for_two():
     t = inputs(2, 130, 2, 2, 32, 32, torch.bfloat16)
     leaf = {k: v.clone().requires_grad_() for k, v in t.items()}

@@ -229,6 +229,17 @@ def test_empty_rows():
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    t = make((2, 40), torch.bfloat16, torch.bfloat16)
+    want = sandwich_norm_fn(**t)
+    far = dict(t)
+    for k in ("x", "residual"):
+        far[k] = torch.empty(2**31 + 8 + 40, dtype=torch.bfloat16, device="cuda").as_strided((2, 40), (2**31 + 8, 1))
+        far[k].copy_(t[k])
+    assert all(torch.equal(a, b) for a, b in zip(want, sandwich_norm_fn(**far)))
+
+
+@pytest.mark.gpu
 def test_captured_and_same_bits():
     t = make((4, 100, 768), torch.bfloat16, torch.float32, gate="batch", gate_dtype=torch.bfloat16)
     static = {k: v.clone().requires_grad_() for k, v in t.items()}

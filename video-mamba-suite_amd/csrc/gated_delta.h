@@ -86,8 +86,7 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_sh
 
 // 8 elements of a row as they stand in memory: columns c .. c+7 of a row of n, any alignment.  WHOLE: n % 8 == 0, one 16- or 32-byte load;
 // otherwise element by element.  Never a branch: what lies outside is read from a place that exists and becomes zero in clear(), when it is
-// used.  (Behind a branch the loads of the next chunk meet the other side's values in a register copy, which waits for them at once: a chunk of
-// the walk took 5.7 us.)
+// used.  (Behind a branch the loads of the next chunk meet the other side's values in a register copy, which waits for them at once.)
 template <typename T> struct Raw8 { T v[8]; };
 template <bool WHOLE, typename T>
 __device__ __forceinline__ Raw8<T> load_raw8(const T* row, int c, int n) {
@@ -427,9 +426,9 @@ struct OTile {
     }
 };
 
-// A walk's workgroup takes 32 columns of a head, or 16 where that leaves half of the CUs without one: a chunk of 16 columns takes 0.7 .. 0.9 of the time of one of
-// 32 (its chain is the same).  (2, 2304, 8 heads, 64 x 64): 32 workgroups 65 us, 64 workgroups 50 us; (8, 8192, 8 heads, 128 x 128): 256 workgroups
-// 356 us, 512 workgroups 464 us.
+// A walk's workgroup takes 32 columns of a head, or 16 where that leaves half of the CUs without one: a chunk of 16 columns takes 0.7 .. 0.8 of the time of one of
+// 32 (its chain is the same).  (2, 2304, 8 heads, 64 x 64): 32 workgroups 54 us, 64 workgroups 38 us; (8, 8192, 8 heads, 128 x 128): 256 workgroups
+// 265 us, 512 workgroups 404 us.
 inline bool narrow(const vms_gated_delta_params& p, const Layout& l) { return (int64_t)p.batch * p.heads * (l.vpad / 32) <= device_cu_count() / 2; }
 
 int validate(const vms_gated_delta_params& p);   // gated_delta_fwd.hip

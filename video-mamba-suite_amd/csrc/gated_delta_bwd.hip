@@ -1,7 +1,7 @@
 // gated_delta_bwd.hip -- gated delta rule, backward (vms_gated_delta_bwd); algebra, precision and layouts: gated_delta.h.
 //
 // With S0, U, T, M of every chunk from the forward's workspace and dS1 = the adjoint of a chunk's last state:
-//   gd_bwd_scan  walks the chunks from the end, a wave per 16 CT columns of dS as in the forward:
+//   gd_bwd_scan  walks the chunks from the end, a workgroup per 16 CT columns of dS as in the forward:
 //                  dU = M^T dO + del K dS1;  Y = T^T dU;  dV = beta Y;  dS0 = gam_63 dS1 + Q^T (scale gam dO) - K^T (beta gam Y)
 //                and leaves dS1 and Y
 //   gd_grad      one workgroup per chunk and q / k head, no order among them:
@@ -26,7 +26,8 @@ struct BwdArgs {   // what the kernels need of vms_gated_delta_bwd_params (one k
 
 // ---- the walk over the chunks, from the end ------------------------------------------------------------------
 // Split among eight waves as the forward's walk: of the chain's four, wave w has token tile w of dU and Y and dk / 4 rows of dS; the other four load, make
-// what depends on no dS (M^T dO, the planes of dO and of scale gam dO) and store.
+// what depends on no dS (M^T dO, the planes of dO and of scale gam dO) and store.  Bound by the chain (K dS1 -> dU -> Y -> dS0): (8, 3136, 6 heads, 128 x 128) bf16
+// 2.7 us per chunk, 131 us; with all of it on four waves 164 us.
 template <typename T, int KP, int CT, int FIT>
 struct BwdScanLds {   // bytes and places in LDS
     static constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
@@ -343,7 +344,8 @@ __device__ __forceinline__ float L_of(double d) { return fast_exp2((float)(d * 1
 // Stage 1 walks v 32 columns at a time: U, Y, dO (64 rows) and S0, dS1 (KP rows) go through registers (the next block is on its way while this one is
 // multiplied) into LDS, 16-byte operands from there; the sums that need no product (Y.V, <S0, dS1>) are taken from the pieces as they pass.  Eight waves:
 // wave w has token tile w % 4 of dQ and W (w < 4: "left", what depends on the token as the later one) or of X (w >= 4: "right"), so that no product is
-// made twice and the accumulators fit.  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
+// made twice and the accumulators fit.  (8, 3136, 6 heads, 128 x 128) bf16: 153 us for 0.45 GB and 30 GFLOP of bf16 products; bound by the steps between
+// the barriers (two workgroups of eight waves fill a CU's registers).  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
 template <typename T, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
 __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO, DT = KP / 16, TB = tile_bytes<KP>();

@@ -2,8 +2,8 @@
 //
 //   gd_prep   one wave per (chunk, head): the gates, T (triangular inverse in fp32), M.
 //   gd_scan   the walk over the chunks.  The columns of S (and of V, U, O) never meet: a workgroup owns 16 CT of them for the whole
-//             sequence.  Its four waves split the chunk's 64 tokens and S's dk rows: wave w computes token tile w of K S0, U and O
-//             and dk / 4 rows of S, which stay in its accumulators.
+//             sequence.  Four of its waves walk the chain and split the chunk's 64 tokens and S's dk rows: wave w computes token tile w of
+//             K S0 and U and dk / 4 rows of S, which stay in its accumulators.  The other four load, make O and store.
 #include <type_traits>
 
 #include "gated_delta.h"
@@ -17,6 +17,7 @@ constexpr float kMinGate = -104.f;
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // ---- T, M and gates of one chunk -----------------------------------------------------------------------------
+// Bound by bytes: (8, 8192, 8 heads, 128) bf16 reads 268 MB of q and k and writes 161 MB in 87 us, 4.9 of the 5.2 TB/s of a large copy.
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
@@ -227,10 +228,15 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 }
 
 // ---- the walk over the chunks --------------------------------------------------------------------------------
-// What bounds it is the chain of one chunk (K S0 -> R -> U -> S1), not a rate: a head is 16 .. 64 tokens of work per step on one CU.  A wave with
-// a whole chunk of 16 columns to itself (no exchange, every wave reading all of K, Q, T, M from LDS) took 5.4 us per chunk at dk = 128,
-// four waves on one chunk take 1.5: three barriers, but a quarter of the products in a row and each operand of K, Q, T, M read once, straight
-// from memory into the registers of the one wave that uses it.  K alone also goes through LDS, for its transpose.
+// What bounds it is the chain of one chunk (K S0 -> R -> U -> S1), not a rate: a head is 16 .. 64 tokens of work per step on one CU.  (8, 8192, 8 heads,
+// 128 x 128) bf16, 263 us: 2.05 us per chunk, of which the matrix cores work 0.4; S0 is read by eight waves from LDS (0.35 us at 128 bytes per cycle) and
+// handed over three times.  Steps that led here, same sizes:
+//   a wave with a whole chunk of 16 columns to itself, every wave reading all of K, Q, T, M from LDS             5.4 us per chunk
+//   four waves on one chunk, K, Q, T, M straight from memory, a chunk ahead                                      2.4
+//   four waves on the chain, four on loads and outputs; lines instead of operands from memory                    2.05
+// Lines: an operand's lanes are 16 rows x 4 pieces of 16 bytes with neighbouring lanes in different rows, and the memory pipe then takes 64 accesses
+// for a load of 1 KB instead of 16 (2825 of a chunk's 5100 cycles).  Read as lines, through LDS into operands, K also stands there for its transpose.  Asked
+// for two chunks ahead (one chunk is less than a loaded memory's latency) and spread over the phases: a wave stands still while the pipe is full.
 template <typename T, int KP, int CT, int FIT>
 struct ScanLds {   // bytes and places in LDS
     static constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
