@@ -36,6 +36,25 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
     const int64_t slot = ((int64_t)b * p.heads + h) * l.chunks + c;
     char* const ws = static_cast<char*>(p.workspace);
 
+    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
+    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
+    auto rows = [&](const Rows<T>& x, int rt, int kb) __attribute__((always_inline)) {
+        const int i = c * C + 16 * rt + n;
+        return fit_load<FIT, T>(x.row(i < len ? i : len - 1), 32 * kb + 8 * q4, p.dk);
+    };
+    auto as_frag = [&](const Raw8<T>& r, int kb) __attribute__((always_inline)) { return planes_of<T>(fit_clear<FIT, T>(r, 32 * kb + 8 * q4, p.dk)); };
+    Raw8<T> kraw[4][KP / 32];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+        for (int kb = 0; kb < KP / 32; ++kb) kraw[rt][kb] = rows(K, rt, kb);
+    // q's rows of the next 16 tokens are on their way while these are multiplied, k's and the first of q before the gates: a chunk is one wave, and each
+    // memory latency it waits for shows in calls with few chunks
+    constexpr bool kEarly = KP * (int)sizeof(T) <= 256;   // (two sets of fp32 rows of 128 would spill)
+    Raw8<T> qraw[KP / 32], qnext[KP / 32];
+#pragma unroll
+    for (int kb = 0; kb < KP / 32; ++kb) qnext[kb] = rows(Q, 0, kb);
+
     {   // gates: lane = token
         const int i = c * C + lane;
         float g = 0.f, be = 0.f;
@@ -62,18 +81,6 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
     }
     __syncthreads();
 
-    const Rows<T> Q(p.q, (int64_t)b * p.q_batch_stride + (int64_t)hk * p.q_head_stride, p.q_seq_stride, len, p.reverse);
-    const Rows<T> K(p.k, (int64_t)b * p.k_batch_stride + (int64_t)hk * p.k_head_stride, p.k_seq_stride, len, p.reverse);
-    auto rows = [&](const Rows<T>& x, int rt, int kb) __attribute__((always_inline)) {
-        const int i = c * C + 16 * rt + n;
-        return fit_load<FIT, T>(x.row(i < len ? i : len - 1), 32 * kb + 8 * q4, p.dk);
-    };
-    auto as_frag = [&](const Raw8<T>& r, int kb) __attribute__((always_inline)) { return planes_of<T>(fit_clear<FIT, T>(r, 32 * kb + 8 * q4, p.dk)); };
-    Raw8<T> kraw[4][KP / 32];
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-        for (int kb = 0; kb < KP / 32; ++kb) kraw[rt][kb] = rows(K, rt, kb);
     char* const tw = ws + l.tri + slot * l.tri_slot;
     char* const mw = tw + NS * kTri;
     char* const ttw = mw + NO * kTri;   // transposes (for_backward)
@@ -90,9 +97,12 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
         f32x4 kk[4], qk[4], kq[4];   // kq: Q K^T once more, lanes along j: the transpose of M
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct) { kk[ct] = f32x4{0.f, 0.f, 0.f, 0.f}; qk[ct] = kk[ct]; kq[ct] = kk[ct]; }
-        Raw8<T> qraw[KP / 32];
 #pragma unroll
-        for (int kb = 0; kb < KP / 32; ++kb) qraw[kb] = rows(Q, rt, kb);
+        for (int kb = 0; kb < KP / 32; ++kb) {
+            if (!kEarly && rt > 0) qnext[kb] = rows(Q, rt, kb);
+            qraw[kb] = qnext[kb];
+            if (kEarly && rt < 3) qnext[kb] = rows(Q, rt + 1, kb);
+        }
 #pragma unroll
         for (int kb = 0; kb < KP / 32; ++kb) {
             const Frag<NX> qi = as_frag(qraw[kb], kb), ki = as_frag(kraw[rt][kb], kb);
