@@ -290,8 +290,13 @@ __device__ __forceinline__ Frag<N> tri_cols(const char* m, int ct, int ib, int l
     return f;
 }
 
+// L of a pair from the difference of its sums (exponents of 2, at most 0 where the pair counts): the choice is made in the exponent, as a branch around the
+// exponential and the reads of its operand costs a latency per element
+using f64x4 = vec_t<double, 4>;
+__device__ __forceinline__ float decay(bool counts, double d) { return fast_exp2((float)(counts ? d : -1e4)); }
+
 // ---- what a chunk leaves in the workspace; slot = (batch entry * heads + head) * chunks + chunk
-struct Gates { float gam[C], bet[C], del[C]; double G[C]; };
+struct Gates { float gam[C], bet[C], del[C]; double G[C]; };   // G: the sums of g in units of log 2
 struct Layout {
     int64_t tri, gates, S0, U;                      // byte offsets of the arrays in the forward's workspace
     int64_t dS, Y;                                  // ... in the backward's own

@@ -339,7 +339,6 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
-__device__ __forceinline__ float L_of(double d) { return fast_exp2((float)(d * 1.4426950408889634)); }
 
 // Stage 1 walks v 32 columns at a time: U, Y, dO (64 rows) and S0, dS1 (KP rows) go through registers (the next block is on its way while this one is
 // multiplied) into LDS, 16-byte operands from there; the sums that need no product (Y.V, <S0, dS1>) are taken from the pieces as they pass.  Eight waves:
@@ -599,14 +598,16 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
                 }
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                if (t <= w)
+                if (t <= w) {
+                    const f64x4 Gj = *reinterpret_cast<const f64x4*>(&gs->G[16 * t + 4 * q4]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int j = 16 * t + 4 * q4 + e;
-                        const float L = j <= own ? L_of(Gi - gs->G[j]) : 0.f;
+                        const float L = decay(j <= own, Gi - Gj[e]), x = L * z[t][e];
                         m[t][e] *= p.scale * L;
-                        z[t][e] = j < own ? L * z[t][e] : 0.f;
+                        z[t][e] = j < own ? x : 0.f;
                     }
+                }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 if (2 * kb <= w) {
@@ -632,14 +633,17 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             ss = fmaf(gs->gam[C - 1], ss, rowdot(Ks, A));   // + the state's own part, below
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                if (t >= w)
+                if (t >= w) {
+                    const f64x4 G4 = *reinterpret_cast<const f64x4*>(&gs->G[16 * t + 4 * q4]);
+                    const f32x4 b4 = *reinterpret_cast<const f32x4*>(&gs->bet[16 * t + 4 * q4]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = 16 * t + 4 * q4 + e;
-                        const float L = i >= own ? L_of(gs->G[i] - Gi) : 0.f;
+                        const float L = decay(i >= own, G4[e] - Gi), x = -b4[e] * L * z[t][e];
                         m[t][e] *= p.scale * L;
-                        z[t][e] = i > own ? -gs->bet[i] * L * z[t][e] : 0.f;
+                        z[t][e] = i > own ? x : 0.f;
                     }
+                }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 if (2 * kb + 1 >= w) {

@@ -21,12 +21,12 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __bui
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
-template <typename T, int KP, int FIT>
+template <typename T, int KP, int FIT, bool TRAIN>
 __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_params p, const Layout l) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
     constexpr int AR = 68;   // row pitch of As, floats
     __shared__ __attribute__((aligned(16))) float As[C * AR];
-    __shared__ double Gs[C];
+    __shared__ __attribute__((aligned(32))) double Gs[C];
     __shared__ float bs[C];
     const int lane = threadIdx.x, n = lane & 15, q4 = lane >> 4;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -70,13 +70,14 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
             const double o = __shfl_up(G, s);
             if (lane >= s) G += o;
         }
+        G *= 1.4426950408889634;   // exponents of 2 from here on
         const double last = __shfl(G, 63);
         Gs[lane] = G;
         bs[lane] = be;
         Gates* const o = reinterpret_cast<Gates*>(ws + l.gates) + slot;
-        o->gam[lane] = fast_exp2((float)(G * 1.4426950408889634));
+        o->gam[lane] = fast_exp2((float)G);
         o->bet[lane] = be;
-        o->del[lane] = fast_exp2((float)((last - G) * 1.4426950408889634));
+        o->del[lane] = fast_exp2((float)(last - G));
         o->G[lane] = G;
     }
     __syncthreads();
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
                 const Frag<NX> kj = ct == rt ? ki : as_frag(kraw[ct][kb], kb);
                 mma<NS>(kk[ct], kj, ki);
                 mma<NS>(qk[ct], kj, qi);
-                if (p.for_backward) mma<NS>(kq[ct], qi, kj);
+                if (TRAIN) mma<NS>(kq[ct], qi, kj);
             }
         }
         const int i = 16 * rt + n;
@@ -120,25 +121,30 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 #pragma unroll
         for (int ct = 0; ct <= rt; ++ct) {
             f32x4 a;
+            const f64x4 Gj = *reinterpret_cast<const f64x4*>(&Gs[16 * ct + 4 * q4]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int j = 16 * ct + 4 * q4 + r;
-                const float L = j <= i ? fast_exp2((float)((Gi - Gs[j]) * 1.4426950408889634)) : 0.f;
-                a[r] = j < i ? bi * L * kk[ct][r] : 0.f;
-                qk[ct][r] = j <= i ? p.scale * L * qk[ct][r] : 0.f;
+                const float L = decay(j <= i, Gi - Gj[r]);
+                const float x = bi * L * kk[ct][r], y = p.scale * L * qk[ct][r];
+                a[r] = j < i ? x : 0.f;
+                qk[ct][r] = j <= i ? y : 0.f;
             }
             *reinterpret_cast<f32x4*>(&As[i * AR + 16 * ct + 4 * q4]) = a;
-            if (p.for_backward) {
+            if (TRAIN) {
                 const int j = 16 * ct + n;
+                const double Gn = Gs[j];
+                const f64x4 G4 = *reinterpret_cast<const f64x4*>(&Gs[16 * rt + 4 * q4]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i2 = 16 * rt + 4 * q4 + r;
-                    kq[ct][r] = j <= i2 ? p.scale * fast_exp2((float)((Gs[i2] - Gs[j]) * 1.4426950408889634)) * kq[ct][r] : 0.f;
+                    const float x = p.scale * decay(j <= i2, G4[r] - Gn) * kq[ct][r];
+                    kq[ct][r] = j <= i2 ? x : 0.f;
                 }
                 put4(mtw + 1024 * tri_t(ct, rt >> 1) + 16 * lane + 8 * (rt & 1), kq[ct]);
             }
         }
-        if (p.for_backward && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
+        if (TRAIN && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
 #pragma unroll
         for (int kb = 0; kb <= rt / 2; ++kb) {
             const Frag<NO> f = frag_of<NO>(qk[2 * kb], qk[2 * kb + 1]);
@@ -227,7 +233,7 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 #pragma unroll
             for (int i2 = 0; i2 < NS; ++i2) *reinterpret_cast<bf16x8*>(tw + i2 * kTri + 1024 * tri(rt, kb) + 16 * lane) = f.p[i2];
         }
-    if (p.for_backward) {
+    if (TRAIN) {
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -574,21 +580,23 @@ static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStre
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-template <typename T, int KP, int FIT>
+template <typename T, int KP, int FIT, bool TRAIN>
 static int fwd_launch(const vms_gated_delta_params& p, hipStream_t s) {
     const Layout l = layout(p);
-    const dim3 grid(l.chunks, p.heads, p.batch);
-    hipLaunchKernelGGL((gd_prep_kernel<T, KP, FIT>), grid, dim3(64), 0, s, p, l);
+    hipLaunchKernelGGL((gd_prep_kernel<T, KP, FIT, TRAIN>), dim3(l.chunks, p.heads, p.batch), dim3(64), 0, s, p, l);
     VMS_LAUNCH_CHECK();
-    if (narrow(p, l)) return p.for_backward ? scan_launch<T, KP, 1, FIT, true>(p, l, s) : scan_launch<T, KP, 1, FIT, false>(p, l, s);
-    return p.for_backward ? scan_launch<T, KP, 2, FIT, true>(p, l, s) : scan_launch<T, KP, 2, FIT, false>(p, l, s);
+    return narrow(p, l) ? scan_launch<T, KP, 1, FIT, TRAIN>(p, l, s) : scan_launch<T, KP, 2, FIT, TRAIN>(p, l, s);
+}
+template <typename T, int KP, int FIT>
+static int fwd_train(const vms_gated_delta_params& p, hipStream_t s) {
+    return p.for_backward ? fwd_launch<T, KP, FIT, true>(p, s) : fwd_launch<T, KP, FIT, false>(p, s);
 }
 template <typename T, int KP>
 static int fwd_fit(const vms_gated_delta_params& p, hipStream_t s) {
     switch (fit_of(p.dk, p.dv)) {
-        case 2: return fwd_launch<T, KP, 2>(p, s);
-        case 1: return fwd_launch<T, KP, 1>(p, s);
-        default: return fwd_launch<T, KP, 0>(p, s);
+        case 2: return fwd_train<T, KP, 2>(p, s);
+        case 1: return fwd_train<T, KP, 1>(p, s);
+        default: return fwd_train<T, KP, 0>(p, s);
     }
 }
 template <typename T>
