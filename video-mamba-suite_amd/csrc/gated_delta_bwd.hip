@@ -343,8 +343,8 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
 // Stage 1 walks v 32 columns at a time: U, Y, dO (64 rows) and S0, dS1 (KP rows) go through registers (the next block is on its way while this one is
 // multiplied) into LDS, 16-byte operands from there; the sums that need no product (Y.V, <S0, dS1>) are taken from the pieces as they pass.  Eight waves:
 // wave w has token tile w % 4 of dQ and W (w < 4: "left", what depends on the token as the later one) or of X (w >= 4: "right"), so that no product is
-// made twice and the accumulators fit.  (8, 3136, 6 heads, 128 x 128) bf16: 153 us for 0.45 GB and 30 GFLOP of bf16 products; bound by the steps between
-// the barriers (two workgroups of eight waves fill a CU's registers).  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
+// made twice and the accumulators fit.  (8, 3136, 6 heads, 128 x 128) bf16: 145 us for 0.45 GB and 30 GFLOP of bf16 products; bound by the steps between
+// the barriers (a workgroup of eight waves fills a CU's registers).  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
 template <typename T, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
 __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO, DT = KP / 16, TB = tile_bytes<KP>();

@@ -17,7 +17,8 @@ constexpr float kMinGate = -104.f;
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // ---- T, M and gates of one chunk -----------------------------------------------------------------------------
-// Bound by bytes: (8, 8192, 8 heads, 128) bf16 reads 268 MB of q and k and writes 161 MB in 87 us, 4.9 of the 5.2 TB/s of a large copy.
+// Bound by bytes: (8, 8192, 8 heads, 128) bf16 reads 268 MB of q and k and writes 161 MB in 83 us, the 5.2 TB/s of a large copy; in calls with few
+// chunks by one wave's chain of steps (8 us, bf16, 64).
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
