@@ -526,7 +526,8 @@ typedef struct {
     int64_t workspace_bytes;
 } vms_gated_delta_params;
 
-/* backward.  f: the forward's block with for_backward set and its workspace (out, final_state and initial_state are not read).  dout in dtype
+/* backward.  f: the forward's block with for_backward set and its workspace (out and final_state are not read, of initial_state only whether there
+ * was one: f.initial_state or dinitial_state is set; without one the first gate's gradient is exactly 0).  dout in dtype
  * (batch, seqlen, heads, dv) with its strides; dfinal_state fp32 optional.  Written whole, contiguous: dq, dk (batch, seqlen, heads_k, dk),
  * dv (batch, seqlen, heads, dv) in dtype, dg, dbeta (batch, seqlen, heads) in gate_dtype, dinitial_state fp32 optional; zeros on padding. */
 typedef struct {

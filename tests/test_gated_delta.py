@@ -153,6 +153,18 @@ def test_lengths(l, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+def test_first_gate_without_a_state(reverse, dtype):
+    """a gate with nothing to forget has gradient 0, not two terms' roundings; with a state it has one"""
+    for l in (1, 70):
+        for state in (False, True):
+            leaf = {k: v.requires_grad_() for k, v in inputs(2, l, 1, 2, 32, 32, dtype, state=state, seed=l).items()}
+            dg, = torch.autograd.grad(gated_delta_rule_fn(**leaf, reverse=reverse).float().square().sum(), leaf["g"])
+            assert ((dg[:, l - 1 if reverse else 0] == 0) != state).all() and (l == 1 or (dg[:, 1:-1] != 0).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dk, dv", [(1, 1), (3, 5), (8, 130), (40, 72), (65, 33), (100, 100), (128, 128), (128, 17), (16, 272)])
 def test_head_sizes(dk, dv, dtype):
     compare(inputs(1, 90, 1, 2, dk, dv, dtype, state=True, seed=dk + dv))

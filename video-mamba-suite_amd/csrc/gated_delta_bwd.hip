@@ -670,6 +670,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x += part[i];
             const int at = c * C + lane;
+            if (at == 0 && !p.initial_state && !a.q.dinitial_state) x = 0.f;   // there is nothing that the first gate could forget: exact, where two equal terms would leave their roundings
             if (at < len) st_gate(a.q.dg, ((int64_t)b * p.seqlen + token(at, len, p.reverse)) * p.heads + h, p.gate_dtype, x);
         }
         if (!left)
