@@ -40,7 +40,7 @@ struct BwdScanLds {   // bytes and places in LDS
 
 template <typename T, int KP, int CT, int FIT>
 __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
+    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
     constexpr int KB = KP / 32, DW = KP / 64;
     constexpr bool WHOLE = FIT != 0;
     using Lds = BwdScanLds<T, KP, CT, FIT>;
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
         }
     };
     auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // columns 16 w + n (row blocks 0, 1; tiles 2 and 3 have no block 0)
-        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;            // first: NS + NO T, 2 NS + NO M (their transposes)
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;            // first: plane 2 NS for T, 3 NS for M (their transposes)
         f[0] = tri_cols<NS>(at, w, w >= 2 ? 1 : 0, lane);
         f[1] = tri_cols<NS>(at, w, 1, lane);
     };
@@ -178,13 +178,13 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             for (int d = 0; d < DW; ++d)
 #pragma unroll
                 for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
-            fetch_tri(before(c, 2), NS + NO, tf);
+            fetch_tri(before(c, 2), 2 * NS, tf);
         };
         if (nc > 0) {
             Frag<NS> t0[2], t1[2];
             if constexpr (!Lds::kStaged) fetch_rows(K, nc - 1, kr);
-            fetch_tri(nc - 1, NS + NO, t0);
-            fetch_tri(before(nc - 1, 1), NS + NO, t1);
+            fetch_tri(nc - 1, 2 * NS, t0);
+            fetch_tri(before(nc - 1, 1), 2 * NS, t1);
             __syncthreads();   // dO of the last chunk is there, for the other side
             for (int c = nc - 1;;) {
                 chunk(c, std::integral_constant<int, 0>{}, t0);
@@ -272,10 +272,10 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                 fetch_rows(Q, before(c, 1), qr);
             }
             if (w < KB) {
-                Frag<NO> sf[CT];
+                Frag<NS> sf[CT];
 #pragma unroll
-                for (int j = 0; j < CT; ++j) sf[j] = Sx.template get<NO>(j, n, 32 * w + 8 * q4);
-                store_frag<NO, CT, false>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
+                for (int j = 0; j < CT; ++j) sf[j] = Sx.get(j, n, 32 * w + 8 * q4);
+                store_frag<NS, CT, false>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
             }
             fetch_k(before(c, 2), mine);
             __syncthreads();
@@ -288,15 +288,15 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
 #pragma unroll
             for (int j = 0; j < CT; ++j) Y[j] = sums[64 * j];
             other_grad(mf);
-            fetch_tri(before(c, 3), 2 * NS + NO, mf);
+            fetch_tri(before(c, 3), 3 * NS, mf);
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
-                const Frag<NO> f = frag_of<NO>(be * Y[j], zero);
+                const Frag<NS> f = frag_of<NS>(be * Y[j], zero);
                 dv[j] = zero;
 #pragma unroll
-                for (int i = NO - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
+                for (int i = NS - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
             }
-            store_rows<NO, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
+            store_rows<NS, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
             ot.put(dv, lane);
         };
         if (nc > 0) {
@@ -306,14 +306,14 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             auto fetch = [&](int c, Ahead& x) __attribute__((always_inline)) { fetch_k(c, x); fetch_q(c, x); fetch_small(c, x); };
             fetch(nc - 1, a0);
             fetch(before(nc - 1, 1), a1);
-            fetch_tri(nc - 1, 2 * NS + NO, m0);
-            fetch_tri(before(nc - 1, 1), 2 * NS + NO, m1);
+            fetch_tri(nc - 1, 3 * NS, m0);
+            fetch_tri(before(nc - 1, 1), 3 * NS, m1);
             hand(nc - 1, std::integral_constant<int, 0>{}, a0);
             fetch_q(before(nc - 1, 2), a0);
             fetch_small(before(nc - 1, 2), a0);
             __syncthreads();
             other_grad(m0);
-            fetch_tri(before(nc - 1, 2), 2 * NS + NO, m0);
+            fetch_tri(before(nc - 1, 2), 3 * NS, m0);
             for (int c = nc - 1;;) {
                 chunk(c, std::integral_constant<int, 0>{}, a0, a1, m1);
                 if (--c < 0) break;
@@ -347,7 +347,7 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
 // the barriers (a workgroup of eight waves fills a CU's registers).  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
 template <typename T, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
 __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO, DT = KP / 16, TB = tile_bytes<KP>();
+    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, DT = KP / 16, TB = tile_bytes<KP>();
     constexpr int PK = C * KP / 8 / 512;   // 8-element pieces of a q / k tile per thread
     constexpr int ROW = 80;                 // bytes of 32 columns in LDS: 16 rows fall on all banks
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -361,10 +361,10 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     char* const Qs = Ks + NX * TB;
     f32x4* const Wx = reinterpret_cast<f32x4*>(Qs + NX * TB);   // beta W, from the left wave to the right one
     char* const Us = big;          // stage 1
-    char* const Ys = Us + NO * C * ROW;
-    char* const Os = Ys + NO * C * ROW;
+    char* const Ys = Us + NS * C * ROW;
+    char* const Os = Ys + NS * C * ROW;
     char* const Ss = Os + NX * C * ROW;
-    char* const Ds = Ss + NO * KP * ROW;
+    char* const Ds = Ss + NS * KP * ROW;
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
@@ -450,12 +450,12 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
         const Rows<T> V(p.v, (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride, p.v_seq_stride, len, p.reverse);
         const Rows<T> dO(a.q.dout, (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride, a.q.dout_seq_stride, len, p.reverse);
         const T* const brow = (left ? dO : V).row(ok_p ? at_p : len - 1);
-        Frag<NO> ap, sp, dp;
+        Frag<NS> ap, sp, dp;
         Raw8<T> bp;
         auto fetch = [&](int vk) __attribute__((always_inline)) {
             const int cc = 32 * vk + pcol;
 #pragma unroll
-            for (int i = 0; i < NO; ++i) {
+            for (int i = 0; i < NS; ++i) {
                 ap.p[i] = *reinterpret_cast<const bf16x8*>(Aw + 2 * (((int64_t)i * C + prow) * l.vpad + cc));
                 sp.p[i] = *reinterpret_cast<const bf16x8*>(Sw + 2 * (((int64_t)i * KP + srow) * l.vpad + cc));
                 dp.p[i] = *reinterpret_cast<const bf16x8*>(Dw + 2 * (((int64_t)i * KP + srow) * l.vpad + cc));
@@ -463,10 +463,10 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             bp = load_raw8<WHOLE, T>(brow, cc, p.dv);
         };
         float yv = 0.f, ss = 0.f;   // this thread's part of Y.V (its token), of <S0, dS1>
-        auto value = [&](const Frag<NO>& f, int e) __attribute__((always_inline)) {
+        auto value = [&](const Frag<NS>& f, int e) __attribute__((always_inline)) {
             float x = 0.f;
 #pragma unroll
-            for (int i = NO - 1; i >= 0; --i) x += static_cast<float>(f.p[i][e]);
+            for (int i = NS - 1; i >= 0; --i) x += static_cast<float>(f.p[i][e]);
             return x;
         };
         auto hand = [&](int vk) __attribute__((always_inline)) {
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             char* const at = (left ? Us : Ys) + prow * ROW + 2 * pcol;
             char* const as = Ss + srow * ROW + 2 * pcol;
 #pragma unroll
-            for (int i = 0; i < NO; ++i) {
+            for (int i = 0; i < NS; ++i) {
                 *reinterpret_cast<bf16x8*>(at + i * C * ROW) = ap.p[i];
                 if (has_s) {
                     *reinterpret_cast<bf16x8*>(as + i * KP * ROW) = sp.p[i];
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             for (int i = 0; i < decltype(planes)::value; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + (i * rows + row) * ROW + 16 * q4);
             return f;
         };
-        constexpr std::integral_constant<int, NO> no{};
+        constexpr std::integral_constant<int, NS> ns{};
         constexpr std::integral_constant<int, NX> nx{};
         // 64 x 64 products [j][i]: rows = another tile's tokens, columns (lanes) = this wave's.  left: m = dO_i.U_j, z = Y_i.U_j with this wave's tokens as i
         // (tiles j <= w); right: with this wave's tokens as j (tiles i >= w).  A: left dO S0^T -> dQ, right U dS1^T -> X;  B: left Y S0^T -> W
@@ -511,31 +511,31 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
         for (int d = 0; d < DT; ++d) { A[d] = zero; B[d] = zero; }
         auto multiply = [&]() __attribute__((always_inline)) {
             if (left) {
-                const Frag<NO> yi = from(Ys, C, own, no);
+                const Frag<NS> yi = from(Ys, C, own, ns);
                 const Frag<NX> oi = from(Os, C, own, nx);
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
                     if (t <= w) {
-                        const Frag<NO> uj = from(Us, C, 16 * t + n, no);
-                        mma<NO>(m[t], uj, oi);
-                        mma<NO>(z[t], uj, yi);
+                        const Frag<NS> uj = from(Us, C, 16 * t + n, ns);
+                        mma<NS>(m[t], uj, oi);
+                        mma<NS>(z[t], uj, yi);
                     }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const Frag<NO> s0 = from(Ss, KP, 16 * d + n, no);
-                    mma<NO>(A[d], s0, oi);
-                    mma<NO>(B[d], s0, yi);
+                    const Frag<NS> s0 = from(Ss, KP, 16 * d + n, ns);
+                    mma<NS>(A[d], s0, oi);
+                    mma<NS>(B[d], s0, yi);
                 }
             } else {
-                const Frag<NO> ui = from(Us, C, own, no);
+                const Frag<NS> ui = from(Us, C, own, ns);
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
                     if (t >= w) {
-                        mma<NO>(m[t], from(Os, C, 16 * t + n, nx), ui);
-                        mma<NO>(z[t], from(Ys, C, 16 * t + n, no), ui);
+                        mma<NS>(m[t], from(Os, C, 16 * t + n, nx), ui);
+                        mma<NS>(z[t], from(Ys, C, 16 * t + n, ns), ui);
                     }
 #pragma unroll
-                for (int d = 0; d < DT; ++d) mma<NO>(A[d], from(Ds, KP, 16 * d + n, no), ui);
+                for (int d = 0; d < DT; ++d) mma<NS>(A[d], from(Ds, KP, 16 * d + n, ns), ui);
             }
         };
         const int blocks = l.vpad / 32;
@@ -703,8 +703,8 @@ static int bwd_scan_fit(const BwdArgs& a, int fit, hipStream_t s) {
 }
 template <typename T, int KP, bool WHOLE, bool SHARED>
 static int grad_launch(const BwdArgs& a, hipStream_t s) {
-    constexpr int NX = Prec<T>::NX, NO = Prec<T>::NO;
-    constexpr int one = (2 * NO + NX) * C * 80 + 2 * NO * KP * 80, two = 2 * NX * tile_bytes<KP>() + C * KP * 4;
+    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    constexpr int one = (2 * NS + NX) * C * 80 + 2 * NS * KP * 80, two = 2 * NX * tile_bytes<KP>() + C * KP * 4;
     constexpr int lds = (int)sizeof(Gates) + (3 * C + 8) * 4 + (one > two ? one : two);
     static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;

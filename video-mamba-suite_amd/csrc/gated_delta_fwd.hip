@@ -24,7 +24,7 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __bui
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
 template <typename T, int KP, int FIT, bool TRAIN>
 __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_params p, const Layout l) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
+    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
     constexpr int AR = 68;   // row pitch of As, floats
     __shared__ __attribute__((aligned(16))) float As[C * AR];
     __shared__ __attribute__((aligned(32))) double Gs[C];
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 
     char* const tw = ws + l.tri + slot * l.tri_slot;
     char* const mw = tw + NS * kTri;
-    char* const ttw = mw + NO * kTri;   // transposes (for_backward)
+    char* const ttw = mw + NS * kTri;   // transposes (for_backward)
     char* const mtw = ttw + NS * kTri;
     auto put4 = [&](char* at, const f32x4& v) __attribute__((always_inline)) {   // half an operand, NS planes
         float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
@@ -148,9 +148,9 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
         if (TRAIN && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
 #pragma unroll
         for (int kb = 0; kb <= rt / 2; ++kb) {
-            const Frag<NO> f = frag_of<NO>(qk[2 * kb], qk[2 * kb + 1]);
+            const Frag<NS> f = frag_of<NS>(qk[2 * kb], qk[2 * kb + 1]);
 #pragma unroll
-            for (int i2 = 0; i2 < NO; ++i2)
+            for (int i2 = 0; i2 < NS; ++i2)
                 *reinterpret_cast<bf16x8*>(mw + i2 * kTri + 1024 * tri(rt, kb) + 16 * lane) = f.p[i2];
         }
     }
@@ -268,7 +268,7 @@ struct ScanLds {   // bytes and places in LDS
 
 template <typename T, int KP, int CT, int FIT, bool TRAIN>
 __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, NO = Prec<T>::NO;
+    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
     constexpr int KB = KP / 32, DW = KP / 64;   // 32-column blocks of k; 16-row tiles of S per wave
     constexpr bool WHOLE = FIT != 0;
     using Lds = ScanLds<T, KP, CT, FIT>;
@@ -440,10 +440,10 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
             VTile<T, CT, WHOLE> v;
             GateTile g;
         };
-        auto fetch_m = [&](int c, Frag<NO> (&m)[2]) __attribute__((always_inline)) {   // rows 16 w + n of M
+        auto fetch_m = [&](int c, Frag<NS> (&m)[2]) __attribute__((always_inline)) {   // rows 16 w + n of M
             const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + NS * kTri;
-            m[0] = tri_rows<NO>(at, w, 0, lane);
-            m[1] = tri_rows<NO>(at, w, w >= 2 ? 1 : 0, lane);
+            m[0] = tri_rows<NS>(at, w, 0, lane);
+            m[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
         };
         auto fetch_q = [&](int c, Ahead& a) __attribute__((always_inline)) {
             if constexpr (Lds::kStaged) fetch_lines(Q, c, a.q);
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
         };
         const OTile<T, CT, WHOLE> ot{v_at(2)};
         Raw8<T> qr[KB];
-        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NO> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
+        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NS> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
             constexpr int odd = decltype(odd_c)::value;
             const int64_t slot = slot0 + c;
             __syncthreads();
@@ -488,14 +488,14 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
                 else x = fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk);
                 const Frag<NX> qf = planes_of<T>(x);
 #pragma unroll
-                for (int j = 0; j < CT; ++j) mma<NO>(O[j], Sx.template get<NO>(j, n, 32 * kb + 8 * q4), qf);
+                for (int j = 0; j < CT; ++j) mma<NS>(O[j], Sx.get(j, n, 32 * kb + 8 * q4), qf);
             }
             if constexpr (TRAIN) {
                 if (w < KB) {   // S0, 32 rows per wave
-                    Frag<NO> sf[CT];
+                    Frag<NS> sf[CT];
 #pragma unroll
-                    for (int j = 0; j < CT; ++j) sf[j] = Sx.template get<NO>(j, n, 32 * w + 8 * q4);
-                    store_frag<NO, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
+                    for (int j = 0; j < CT; ++j) sf[j] = Sx.get(j, n, 32 * w + 8 * q4);
+                    store_frag<NS, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
                 }
             }
             if constexpr (!Lds::kStaged) fetch_rows(Q, c + 1 < nc ? c + 1 : c, qr);
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
             fetch_q(next, other);
 #pragma unroll
             for (int j = 0; j < CT; ++j) O[j] *= sg;
-            // O += M U (two planes of U keep the error of O at what M's one leaves)
+            // O += M U
             Frag<NS> uf[CT];
 #pragma unroll
             for (int j = 0; j < CT; ++j) uf[j] = Ux.get(j, n, 8 * q4);
@@ -522,11 +522,11 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
             }
             fetch_m(c + 2 < nc ? c + 2 : nc - 1, mf);
             ot.put(O, lane);
-            if constexpr (TRAIN) store_frag<NO, CT, true>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, w & 1, col0, uf, n, q4);
+            if constexpr (TRAIN) store_frag<NS, CT, true>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, w & 1, col0, uf, n, q4);
         };
         if (nc > 0) {
             Ahead a0, a1;
-            Frag<NO> m0[2], m1[2];
+            Frag<NS> m0[2], m1[2];
             if constexpr (!Lds::kStaged) fetch_rows(Q, 0, qr);
             auto fetch = [&](int c, Ahead& a) __attribute__((always_inline)) { fetch_k(c, a); fetch_v(c, a); fetch_q(c, a); };
             fetch(0, a0);

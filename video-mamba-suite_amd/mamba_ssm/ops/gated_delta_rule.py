@@ -84,6 +84,8 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
     device: the valid tokens of each batch entry, first in memory in either direction (values are clamped to 0 .. seqlen); the rest is padding
     that leaves the state alone, gives 0 and receives gradient 0.  Tokens are worked on 64 at a time: a NaN or infinity in a valid one reaches
     the outputs of its whole group of 64 and of what follows, none of the groups before.  batch, heads <= 65535, seqlen <= 2^30.
+    What is computed on the way is carried to 2^-16 for fp16 and bf16 q, k, v, and to 2^-24 for fp32: final states and the gradients of fp32 gates
+    beside 16-bit q, k, v are fp32 numbers of that accuracy.
     -> out (batch, seqlen, heads, dv), with return_final_state (out, final_state fp32).  Differentiable once in q, k, v, g, beta, initial_state."""
     fast = _compiled("gated_delta_rule", v.is_cuda and v.numel())
     if fast is not None:
