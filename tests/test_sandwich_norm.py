@@ -104,6 +104,23 @@ def test_c_entry_refuses():
     assert L.vms_sandwich_norm_fwd(ctypes.byref(P), None) < 0 and b"stats" in L.vms_last_error()
 
 
+def test_an_empty_batch_with_a_gate_per_entry_is_no_division_by_zero():
+    t = make((0, 5, 32), torch.float32, torch.float32, gate="batch", device="cpu")
+    with pytest.raises(RuntimeError, match="GPU"):
+        sandwich_norm_fn(**t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 5, 32), (3, 0, 32)])
+@pytest.mark.parametrize("gate", ["none", "channel", "ones", "batch", "token"])
+def test_empty_rows_with_every_gate(gate, shape):
+    t = {k: v.requires_grad_() for k, v in make(shape, torch.bfloat16, torch.float32, gate=gate).items()}
+    y, s = sandwich_norm_fn(**t)
+    assert y.shape == s.shape == shape and s.dtype == torch.float32
+    for k, g in zip(t, torch.autograd.grad(y.float().sum() + s.sum(), list(t.values()))):
+        assert g.shape == t[k].shape and (g == 0).all(), k
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rms", [False, True])

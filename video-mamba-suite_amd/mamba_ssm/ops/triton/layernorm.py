@@ -205,7 +205,7 @@ def sandwich_norm_fn(x, residual, post_weight, pre_weight, post_bias=None, pre_b
             rows_per_gate = rows
         else:
             _require(lead[0] == x.shape[0] and all(n == 1 for n in lead[1:]), "gate must be (N,), (batch, 1, ..., 1, N) or of the shape of x")
-            rows_per_gate = rows // x.shape[0]
+            rows_per_gate = rows // max(x.shape[0], 1)   # (an empty batch has none)
     tensors = [t for t in (residual, post_weight, pre_weight, post_bias, pre_bias, gate) if t is not None]
     _require(all(t.device == x.device for t in tensors), "all tensors must be on one device")
     _require(x.is_cuda, "tensors must be on a GPU (no CPU path in this library)")
