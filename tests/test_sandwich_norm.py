@@ -3,6 +3,8 @@
 Tolerances, relative to the largest value compared: the arithmetic is fp32 over rows of up to 8192 (sums by lane, wave and team, i.e. chains of
 under 64 additions: 64 * 2^-24 = 4e-6 per statistic, two statistics and their gradients in a row: 2e-5); sums over rows chain up to
 rows / 1024 + 80 additions, under 256 here: 2e-5 as well; one rounding to a 16-bit result: 2^-8 bf16, 2^-11 fp16."""
+import os
+
 import pytest
 import torch
 
@@ -102,6 +104,22 @@ def test_c_entry_refuses():
     P.rows_per_gate = 2
     P.stats = 260
     assert L.vms_sandwich_norm_fwd(ctypes.byref(P), None) < 0 and b"stats" in L.vms_last_error()
+
+
+def test_c_workspace_size_of_bad_gate_rows():
+    """0 for a block that the launch refuses, no division by zero (in a process of its own: that ended it)"""
+    import subprocess
+    import sys
+    code = ("import ctypes, vms_hip\n"
+            "L, P = vms_hip.lib(), vms_hip.SandwichNormParams()\n"
+            "P.rows, P.cols, P.gate = 4, 16, 256\n"
+            "got = []\n"
+            "for n in (0, 1, 2, 3, 4, 8, 2**40):\n"
+            "    P.rows_per_gate = n\n"
+            "    got.append(L.vms_sandwich_norm_bwd_workspace_bytes(ctypes.byref(P)) > 0)\n"
+            "print(got)")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": os.pathsep.join(sys.path)})
+    assert r.returncode == 0 and r.stdout.strip() == "[False, True, True, False, True, False, False]", (r.returncode, r.stdout, r.stderr)
 
 
 def test_an_empty_batch_with_a_gate_per_entry_is_no_division_by_zero():

@@ -482,7 +482,8 @@ extern "C" int vms_sandwich_norm_fwd(const vms_sandwich_norm_params* pp, void* s
     return rc;
 }
 extern "C" int64_t vms_sandwich_norm_bwd_workspace_bytes(const vms_sandwich_norm_params* pp) {
-    if (!pp || pp->rows <= 0 || pp->cols <= 0 || pp->cols > 8192 || (pp->gate && pp->rows_per_gate < 1)) return 0;
+    if (!pp || pp->rows <= 0 || pp->cols <= 0 || pp->cols > 8192 || (pp->gate && (pp->rows_per_gate < 1 || pp->rows % pp->rows_per_gate != 0)))
+        return 0;
     return (int64_t)sn::plan_of(*pp).partials * 4 * pp->cols * 4;
 }
 extern "C" int vms_sandwich_norm_bwd(const vms_sandwich_norm_bwd_params* qq, void* stream) {
