@@ -132,6 +132,23 @@ def test_c_entry_refuses_without_a_gpu():
     assert L.vms_gated_delta_bwd(ctypes.byref(Q), None) < 0 and b"for_backward" in L.vms_last_error()
 
 
+def test_a_library_without_an_entry_is_refused_when_it_is_loaded(tmp_path, monkeypatch):
+    """built before the entry was added, with the version of now: an ImportError that says what to do, not an AttributeError later"""
+    import shutil
+    import subprocess
+
+    import vms_hip
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    (tmp_path / "old.c").write_text("\n".join(f"int {n}(void) {{ return {vms_hip.ABI_VERSION}; }}" for n in vms_hip.EXPORTS if "gated_delta" not in n))
+    subprocess.check_call([cc, "-shared", "-fPIC", "-o", str(tmp_path / "old.so"), str(tmp_path / "old.c")])
+    monkeypatch.setattr(vms_hip, "LIB_PATH", str(tmp_path / "old.so"))
+    monkeypatch.setattr(vms_hip, "_lib", None)
+    with pytest.raises(ImportError, match="vms_gated_delta_fwd.*rebuild"):
+        vms_hip.lib()
+
+
 def test_sizes_beyond_32_bits_are_refused():
     """a length of 2^32 + 3 must not be taken for one of 3"""
     t = inputs(1, 1, 1, 1, 4, 6, torch.float32, device="cpu")

@@ -403,6 +403,9 @@ def lib():
                 f"{LIB_PATH} not found: build the HIP library first "
                 "(python -c 'import __graft_entry__ as g; g.build()' or make -C video-mamba-suite_amd/csrc)")
         L = ctypes.CDLL(LIB_PATH)
+        missing = [fn for fn in EXPORTS if not hasattr(L, fn)]
+        if missing:   # built before these were added: the version counts changes to what was there, not additions
+            raise ImportError(f"{LIB_PATH} lacks {', '.join(missing)}: rebuild it")
         L.vms_last_error.restype = ctypes.c_char_p
         L.vms_last_kernel.restype = ctypes.c_char_p
         if L.vms_abi_version() != ABI_VERSION:
