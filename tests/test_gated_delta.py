@@ -132,6 +132,25 @@ def test_c_entry_refuses_without_a_gpu():
     assert L.vms_gated_delta_bwd(ctypes.byref(Q), None) < 0 and b"for_backward" in L.vms_last_error()
 
 
+@pytest.mark.parametrize("dtype, for_backward, dv, most", [("VMS_BF16", 0, 32, 2**23), ("VMS_BF16", 1, 64, 2**22), ("VMS_F32", 0, 1, 2**23), ("VMS_F32", 1, 1, 2**22)])
+def test_c_entry_refuses_launches_of_2_to_the_32_threads(dtype, for_backward, dv, most):
+    """before any launch, and not one head earlier"""
+    import ctypes
+
+    import vms_hip
+    L = vms_hip.lib()
+    P = vms_hip.GatedDeltaParams()
+    P.seqlen = P.heads_k = 1
+    P.dk, P.dv, P.for_backward, P.q_seq_stride = 8, dv, for_backward, 2**40
+    P.dtype = P.gate_dtype = getattr(vms_hip, dtype)
+    P.q = P.k = P.v = P.g = P.beta = P.out = P.workspace = 256
+    P.workspace_bytes = 2**62
+    P.heads = 2048
+    for batch, message in ((most // 2048, b"too large"), (most // 2048 - 1, b"strides")):   # (the next check, so that nothing is launched)
+        P.batch = batch
+        assert L.vms_gated_delta_fwd(ctypes.byref(P), None) < 0 and message in L.vms_last_error(), L.vms_last_error()
+
+
 def test_a_library_without_an_entry_is_refused_when_it_is_loaded(tmp_path, monkeypatch):
     """built before the entry was added, with the version of now: an ImportError that says what to do, not an AttributeError later"""
     import shutil

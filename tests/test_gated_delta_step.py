@@ -71,6 +71,18 @@ def test_c_entry_refuses():
     assert L.vms_gated_delta_state_update(ctypes.byref(P), None) < 0 and b"required" in L.vms_last_error()
 
 
+def test_c_entry_refuses_launches_of_2_to_the_32_threads():
+    import ctypes
+
+    import vms_hip
+    L = vms_hip.lib()
+    P = vms_hip.GatedDeltaStepParams()
+    P.heads, P.heads_k, P.dk, P.dv = 2**8, 1, 4, 40   # two workgroups of 256 threads per head
+    for batch, message in ((2**15, b"too large"), (2**15 - 1, b"required")):
+        P.batch = batch
+        assert L.vms_gated_delta_state_update(ctypes.byref(P), None) < 0 and message in L.vms_last_error(), L.vms_last_error()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("b, hk, h, dk, dv", [(1, 1, 1, 1, 1), (3, 2, 4, 5, 7), (2, 1, 1, 32, 33), (1, 8, 8, 128, 128), (2, 2, 6, 40, 72),

@@ -561,7 +561,9 @@ int validate(const vms_gated_delta_params& p) {
     VMS_CHECK(p.dk >= 1 && p.dk <= 128, "key heads of 1 .. 128");
     VMS_CHECK(p.dv >= 1 && p.dv <= 4096, "value heads of 1 .. 4096");
     VMS_CHECK(p.heads <= 65535 && p.batch <= 65535 && p.seqlen <= (1 << 30), "problem too large");
-    VMS_CHECK((int64_t)p.batch * p.heads * ((p.dv + 15) / 16) < (1LL << 31), "problem too large");
+    // the walks' launches of 512 threads have to stay below 2^32 threads: 32 columns per workgroup, 16 in the fp32 backward (fewer workgroups take 16 only where they are few)
+    const int least = p.for_backward && p.dtype == VMS_F32 ? 16 : 32;
+    VMS_CHECK((int64_t)p.batch * p.heads * (ceil_to(p.dv, 32) / least) < (1LL << 32) / 512, "problem too large");
     VMS_CHECK(p.q && p.k && p.v && p.g && p.beta, "q, k, v, g, beta are required");
     for (const int64_t n : {p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.out_seq_stride})
         VMS_CHECK(n > -(1LL << 31) && n < (1LL << 31), "strides along the sequence of less than 2^31 elements");

@@ -129,7 +129,7 @@ extern "C" int vms_gated_delta_state_update(const vms_gated_delta_step_params* p
     VMS_CHECK(p.batch > 0 && p.heads > 0 && p.heads_k > 0, "empty problem");
     VMS_CHECK(p.heads % p.heads_k == 0, "heads must be a multiple of heads_k");
     VMS_CHECK(p.dk >= 1 && p.dk <= 128 && p.dv >= 1 && p.dv <= 4096, "key heads of 1 .. 128, value heads of 1 .. 4096");
-    VMS_CHECK((int64_t)p.batch * p.heads * ((p.dv + gds::kCols - 1) / gds::kCols) < (1LL << 31), "problem too large");
+    VMS_CHECK((int64_t)p.batch * p.heads * ((p.dv + gds::kCols - 1) / gds::kCols) < (1LL << 32) / 256, "problem too large");   // (threads of a launch)
     VMS_CHECK(p.state && p.q && p.k && p.v && p.g && p.beta && p.out, "state, q, k, v, g, beta, out are required");
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (p.state_dtype == VMS_F32) gds::launch<float>(p, s);

@@ -83,7 +83,8 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
     initial_state (batch, heads, dk, dv) fp32.  reverse=True: right to left, as in selective_scan.  seq_lens (batch,) integers on the
     device: the valid tokens of each batch entry, first in memory in either direction (values are clamped to 0 .. seqlen); the rest is padding
     that leaves the state alone, gives 0 and receives gradient 0.  Tokens are worked on 64 at a time: a NaN or infinity in a valid one reaches
-    the outputs of its whole group of 64 and of what follows, none of the groups before.  batch, heads <= 65535, seqlen <= 2^30.
+    the outputs of its whole group of 64 and of what follows, none of the groups before.  batch, heads <= 65535, seqlen <= 2^30,
+    batch * heads * ceil(dv / 32) < 2^23 (half of it for training in fp32).
     What is computed on the way is carried to 2^-16 for fp16 and bf16 q, k, v, and to 2^-24 for fp32: final states and the gradients of fp32 gates
     beside 16-bit q, k, v are fp32 numbers of that accuracy.
     -> out (batch, seqlen, heads, dv), with return_final_state (out, final_state fp32).  Differentiable once in q, k, v, g, beta, initial_state."""
@@ -154,7 +155,7 @@ def _separate_states(state):
 def gated_delta_state_update(state, q, k, v, g, beta, scale=None):
     """One token.  state (batch, heads, dk, dv) [in/out], fp32, fp16 or bf16, each (dk, dv) contiguous; q, k (batch, heads_k, dk), v (batch, heads, dv),
     one dtype; g, beta (batch, heads), that dtype or fp32; scale: default dk ** -0.5 -> out (batch, heads, dv).  The arithmetic is fp32; a
-    16-bit state is rounded as it is stored, out is computed before that rounding.  Not differentiable."""
+    16-bit state is rounded as it is stored, out is computed before that rounding.  Not differentiable.  batch * heads * ceil(dv / 32) < 2^24."""
     fast = _compiled("gated_delta_state_update", v.is_cuda)
     if fast is not None:
         return fast(state, q, k, v, g, beta, scale)
