@@ -187,3 +187,23 @@ def test_compiled_and_ctypes_steps_are_one(monkeypatch):
             with pytest.raises(RuntimeError, match="gated_delta_rule"):
                 gated_delta_state_update(bad, **t)
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compiled", [True, False])
+def test_state_of_an_inference_mode(compiled, monkeypatch):
+    """a prompt worked under inference_mode, steps outside of it: the state of such a call counts no versions and is updated like any other"""
+    import vms_hip
+    if not compiled:
+        monkeypatch.setattr(vms_hip, "_ext", None)
+    state, t = step_inputs(2, 1, 2, 16, 20, torch.bfloat16)
+    want_state = state.clone()
+    with torch.inference_mode():
+        inner = state.clone()
+    for _ in range(2):
+        want = gated_delta_state_update(want_state, **t)
+        with torch.no_grad():
+            got = gated_delta_state_update(inner, **t)
+        assert torch.equal(got, want) and torch.equal(inner, want_state)
+    with torch.inference_mode():
+        assert torch.equal(gated_delta_state_update(inner, **t), gated_delta_state_update(want_state, **t))

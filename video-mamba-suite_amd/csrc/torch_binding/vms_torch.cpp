@@ -1136,7 +1136,7 @@ Tensor gated_delta_state_update(const Tensor& state, const Tensor& q_, const Ten
     p.g_batch_stride = g.stride(0); p.g_head_stride = g.stride(1);
     p.beta_batch_stride = beta.stride(0); p.beta_head_stride = beta.stride(1);
     call("vms_gated_delta_state_update", vms_gated_delta_state_update, p, v);
-    state.unsafeGetTensorImpl()->bump_version();
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();   // (those count no versions)
     return out;
 }
 
