@@ -399,6 +399,26 @@ def test_nothing_to_walk_over():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b, l, h", [(2, 0, 2), (0, 4, 2), (2, 4, 0)])
+def test_gradients_of_nothing(b, l, h):
+    """no token, no batch entry, no head: zeros of every leaf's shape, and the state's own gradient passes through"""
+    for state in (False, True):
+        leaf = {k: v.requires_grad_() for k, v in inputs(b, l, 2, h, 8, 8, torch.bfloat16, state=state).items()}
+        out, s = gated_delta_rule_fn(**leaf, return_final_state=True)
+        assert out.shape == (b, l, h, 8) and out.dtype == torch.bfloat16 and s.shape == (b, h, 8, 8) and s.dtype == torch.float32
+        for heads in ((out, s), (out,), (s,)):
+            grads = torch.autograd.grad(heads, list(leaf.values()), [torch.ones_like(x) for x in heads], retain_graph=True)
+            for n, g in zip(leaf, grads):
+                want = 1 if n == "initial_state" and any(x is s for x in heads) else 0
+                assert g.shape == leaf[n].shape and (g == want).all(), n
+    if l == 0:   # whatever the state holds
+        t = inputs(b, l, 2, h, 8, 8, torch.bfloat16, state=True)
+        t["initial_state"][0] = float("nan")
+        t["initial_state"][1] = float("inf")
+        assert torch.equal(gated_delta_rule_fn(**t, return_final_state=True)[1].nan_to_num(5.0), t["initial_state"].nan_to_num(5.0))
+
+
+@pytest.mark.gpu
 def test_only_some_gradients():
     """a gradient that arrives through the final state alone; leaves that want none"""
     t = inputs(1, 70, 1, 1, 16, 16, torch.float32)

@@ -106,10 +106,11 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
         # clamped before the narrowing: a 64-bit length must not wrap
         seq_lens = seq_lens.clamp(0, seqlen).to(torch.int32).contiguous() if seq_lens.dtype == torch.int64 else seq_lens.contiguous()
     scale = dk ** -0.5 if scale is None else float(scale)
-    if v.numel() == 0:   # nothing to walk over: the state passes through
-        out = v * 0
-        s = torch.zeros((batch, heads, dk, dv), dtype=torch.float32, device=v.device) if initial_state is None else initial_state.clone()
-        return (out, s) if return_final_state else out
+    if v.numel() == 0:   # nothing to walk over: the state passes through, the other gradients are 0
+        zero = 0 * sum(t.float().sum() for t in (q, k, v, g, beta))   # (a number where the state is not empty: then these are)
+        s = torch.zeros((batch, heads, dk, dv), dtype=torch.float32, device=v.device) if initial_state is None else initial_state
+        out = v + (zero + 0 * s.sum()).to(v.dtype)
+        return (out, s + zero) if return_final_state else out
     out, final = GatedDeltaRuleFn.apply(q, k, v, g, beta, initial_state, scale, reverse, seq_lens, return_final_state)
     return (out, final) if return_final_state else out
 
