@@ -369,11 +369,10 @@ inline int allow_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
     return VMS_OK;
 }
 // CT accumulator tiles (rows row0 + 4 p + r, column col0 + col_of(j, n)) into NS planes of (rows, vpad): through unit_frag, so that a lane
-// stores 4 CT consecutive columns of one row.  vpad and col0 are multiples of 16 CT or of 32: a slice is inside or outside whole, or CT = 1
+// stores 4 CT consecutive columns of one row.  vpad is a multiple of 32, so that the 16 CT columns of a slice are always inside
 template <int NS, int CT>
 __device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int row0, int col0, const f32x4 (&v)[CT], int n, int p) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    if (col0 >= vpad) return;
     Frag<NS> f[CT];
 #pragma unroll
     for (int j = 0; j < CT; ++j) f[j] = frag_of<NS>(v[j], zero);
@@ -393,7 +392,6 @@ __device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int r
 template <int NS, int CT, bool PAIRED>
 __device__ __forceinline__ void store_frag(char* base, int rows, int vpad, int row0, int half, int col0, const Frag<NS> (&f)[CT], int n, int p) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    if (col0 >= vpad) return;
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
