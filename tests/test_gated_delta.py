@@ -291,6 +291,43 @@ def test_strides(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hk, dk, dv", [(2, 40, 56), (1, 64, 64), (2, 33, 17)])
+def test_gradients_of_strided_calls(hk, dk, dv, dtype):
+    """slices of one projection, heads before tokens, a strided last axis and a gradient laid out otherwise: the bits of the contiguous call"""
+    t = inputs(2, 100, hk, 2, dk, dv, dtype, seed=dk)
+    dout = torch.randn(t["v"].shape, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(dtype)
+
+    def run(make, dout):
+        leaf = {n: make(x).detach().requires_grad_() for n, x in t.items()}
+        return torch.autograd.grad(gated_delta_rule_fn(**leaf), list(leaf.values()), dout)
+    want = run(lambda x: x, dout)
+    heads_first = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    tokens_first = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    strided = lambda x: torch.stack([x, x], -1)[..., 0]  # noqa: E731
+    slices = lambda x: torch.cat([x[..., :1], x, x], -1)[..., 1:x.shape[-1] + 1]  # noqa: E731
+    for turn in (heads_first, tokens_first, strided, slices):
+        for d in (dout, turn(dout)):
+            assert turn(dout).stride() != dout.stride()
+            for n, a, b in zip(t, run(turn, d), want):
+                assert torch.equal(a, b), (turn, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_expanded_leaves(dtype):
+    """one batch entry seen three times, an expanded gradient: the leaves get the sum of three equal gradients.  autograd adds them in the leaf's type: two more
+    roundings of up to three times the size"""
+    t = inputs(1, 100, 2, 2, 40, 56, dtype)
+    leaf = {n: x.clone().requires_grad_() for n, x in t.items()}
+    gated_delta_rule_fn(**{n: x.expand(3, *x.shape[1:]) for n, x in leaf.items()}).sum().backward()
+    wide = {n: x.double().requires_grad_() for n, x in t.items()}
+    gated_delta_rule_ref(**{n: x.expand(3, *x.shape[1:]) for n, x in wide.items()}).sum().backward()
+    for n in t:
+        close(leaf[n].grad, wide[n].grad, TOL[dtype] + 2 * torch.finfo(dtype).eps / 2, "d" + n)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_fp32_gates(dtype):
     compare(inputs(2, 150, 1, 2, 64, 64, dtype, gate_dtype=torch.float32))

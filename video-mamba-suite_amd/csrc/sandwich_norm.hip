@@ -328,8 +328,8 @@ __global__ __launch_bounds__(TS < 128 ? 256 : TS, TS == 1024 ? 4 : 3) void sandw
 }
 
 // ---- the partial rows' sums.  A workgroup owns 64 columns (16 groups of 4) of one of the four arrays, 64 row lanes (with 16, one load at a time: 47 us
-// for 1536 rows of 1024); blockIdx.z < 4: dw1, db1 (with the
-// gate of each partial row's group where `weigh`), dw2, db2;  blockIdx.z >= 4: dgate of gate row z - 4 from its `parts` partial rows of P1 and P0
+// for 1536 rows of 1024); blockIdx.y < 4: dw1, db1 (with the
+// gate of each partial row's group where `weigh`), dw2, db2;  blockIdx.y >= 4: dgate of gate row y - 4 from its `parts` partial rows of P1 and P0
 __global__ __launch_bounds__(1024) void sandwich_finish_kernel(const vms_sandwich_norm_bwd_params q, const Plan plan, const int weigh) {
     __shared__ float red[2][64][65];
     const vms_sandwich_norm_params& p = q.f;
