@@ -168,6 +168,13 @@ def test_group_sizes(b, l, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b, l, cols", [(1100, 90, 16), (2100, 90, 8), (300, 50, 700), (4800, 2, 3), (70, 4, 3000)])
+def test_group_counts_on_both_sides_of_the_plan(b, l, cols):
+    """more groups than workgroups, shared and walked whole; few wide short ones"""
+    compare(make((b, l, cols), torch.bfloat16, torch.float32, gate="batch", gate_dtype=torch.bfloat16))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("weight_dtype", [torch.float16, torch.bfloat16])
 def test_weight_types_and_no_residual(weight_dtype):
     compare(make((2, 30, 96), torch.bfloat16, None, gate="channel", weight_dtype=weight_dtype))

@@ -182,7 +182,15 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void sandwich_fwd_kernel(const
 }
 
 // Which rows a workgroup walks.  groups = gate rows that collect sums (1 without a gate, or with one of a row per token, whose gradient is
-// written row by row).  Few groups: `parts` workgroups share each (whole = 0).  More groups than workgroups: a team walks whole groups (whole = 1).
+// written row by row).  `parts` workgroups share each (whole = 0), or a team walks whole groups (whole = 1).  A team's rows follow one another (about 2 us each), which
+// many teams hide; shared groups leave a partial row each, which the finish reads.  Both sides, backward of one call, us (shared / whole; bf16, fp32 stream, biases):
+//   groups          64 columns, 16 rows   64 columns, 196   384 columns, 4   384 columns, 64   768 columns, 16   1536 columns, 64   3000 columns, 4
+//   128                  18 / 31              59 / 383          12 / 14           43 / 142          49 / 43           79 / 184           45 / 25
+//   512                  35 / 32             142 / 403          21 / 16           79 / 144          63 / 53          327 / 273          129 / 52
+//   1024                 42 / 34             257 / 404          37 / 20          168 / 208          95 / 78          640 / 594          237 / 117
+//   2048                 81 / 51             519 / 568          67 / 25          279 / 260         232 / 162              -             478 / 209
+// The rule sets a team's chain against what all groups cost together, rows and partial rows.  Over 6 widths, 2 to 784 rows and 128 to 16384 groups it is within a quarter
+// of the better side, but at 128 groups of 768 columns and 4 rows, and of 3000 columns and 16 rows (a third).
 struct Plan { int groups, parts, whole, partials; int64_t rpg; };
 constexpr int kMostWgs = 1024;   // 4 per CU
 // lanes of a row in the backward: 8 columns each
@@ -192,14 +200,14 @@ static Plan plan_of(const vms_sandwich_norm_params& p) {
     l.rpg = p.gate && p.rows_per_gate > 1 ? p.rows_per_gate : p.rows;
     l.groups = (int)(p.rows / l.rpg);
     const int ts = team_of(p.cols), teams = ts == 64 ? 4 : 1, most_wgs = ts == 128 ? 3 * kMostWgs / 2 : kMostWgs;   // (as many as are resident)
-    l.whole = l.groups > most_wgs / 2;
+    l.whole = l.groups > 1 && l.groups * (l.rpg * (270 + p.cols) + 16000 + 14 * p.cols) > 1300000 * l.rpg;   // (shared: fewer than 4800)
     if (l.whole) {
         const int want = (l.groups + teams - 1) / teams;
         l.parts = 1;
         l.partials = want < most_wgs ? want : most_wgs;
     } else {
         const int64_t most = (l.rpg + teams - 1) / teams;
-        l.parts = most_wgs / l.groups;
+        l.parts = l.groups < most_wgs ? most_wgs / l.groups : 1;
         if (l.parts > most) l.parts = (int)most;
         l.partials = l.groups * l.parts;
     }
