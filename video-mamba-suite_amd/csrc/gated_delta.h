@@ -56,6 +56,18 @@ __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB
             if (i < NA && s - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], acc, 0, 0, 0);
 }
 
+// Results of products in a block that not every wave enters, at the end of the block: a matrix instruction's result may be touched 8 wait states after it at the earliest,
+// and the compiler's count of them misses ways through short conditional blocks (tools/isa_hazards.py --mfma).  The empty statements hold the results
+// here, in the order of these statements; behind the last one the waits are over.
+__device__ __forceinline__ void settle(f32x4& x) { asm volatile("s_nop 7" : "+v"(x)); }
+template <int N, typename... Rest>
+__device__ __forceinline__ void settle(f32x4 (&x)[N], Rest&... rest) {
+#pragma unroll
+    for (int i = 0; i < (sizeof...(rest) ? N : N - 1); ++i) asm volatile("" : "+v"(x[i]));
+    if constexpr (sizeof...(rest) > 0) settle(rest...);
+    else settle(x[N - 1]);
+}
+
 // x0, x1 -> their bf16 values (round to nearest) in one register; what is left of them
 __device__ __forceinline__ unsigned take_bf16(float& x0, float& x1, bool last) {
     using bf16x2 = vec_t<bf16_t, 2>;

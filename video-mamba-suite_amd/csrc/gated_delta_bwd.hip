@@ -142,9 +142,11 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                 Y[j] = zero;
                 mma<NS>(Y[j], tf[1], Ux.get(j, n, 32 + 8 * q4));
             }
-            if (w < 2)
+            if (w < 2) {
 #pragma unroll
                 for (int j = 0; j < CT; ++j) mma<NS>(Y[j], tf[0], Ux.get(j, n, 8 * q4));
+                settle(Y);
+            }
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
                 sums[64 * j] = Y[j];
@@ -254,7 +256,10 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             for (int j = 0; j < CT; ++j) {
                 f32x4 e = zero;
                 mma<NS>(e, mf[1], Ox.get(j, n, 32 + 8 * q4));
-                if (w < 2) mma<NS>(e, mf[0], Ox.get(j, n, 8 * q4));
+                if (w < 2) {
+                    mma<NS>(e, mf[0], Ox.get(j, n, 8 * q4));
+                    settle(e);
+                }
                 sums[64 * j] = e;
             }
         };
@@ -519,6 +524,8 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
                         const Frag<NS> uj = from(Us, C, 16 * t + n, ns);
                         mma<NS>(m[t], uj, oi);
                         mma<NS>(z[t], uj, yi);
+                        asm volatile("" : "+v"(m[t]));
+                        settle(z[t]);
                     }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
@@ -526,6 +533,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
                     mma<NS>(A[d], s0, oi);
                     mma<NS>(B[d], s0, yi);
                 }
+                settle(A, B);
             } else {
                 const Frag<NS> ui = from(Us, C, own, ns);
 #pragma unroll
@@ -533,9 +541,12 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
                     if (t >= w) {
                         mma<NS>(m[t], from(Os, C, 16 * t + n, nx), ui);
                         mma<NS>(z[t], from(Ys, C, 16 * t + n, ns), ui);
+                        asm volatile("" : "+v"(m[t]));
+                        settle(z[t]);
                     }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) mma<NS>(A[d], from(Ds, KP, 16 * d + n, ns), ui);
+                settle(A);
             }
         };
         const int blocks = l.vpad / 32;
@@ -618,6 +629,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
                         mma<NS>(A[d], kc, fm);
                         mma<NS>(B[d], kc, fz);
                     }
+                    settle(A, B);
                 }
             const float qd = quarters_sum(rowdot(Qs, A)), kw = quarters_sum(rowdot(Ks, B));
 #pragma unroll
@@ -653,6 +665,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
                         mma<NS>(A[d], tile_cols<KP, NX>(Qs, d, kb, n, q4), fm);
                         mma<NS>(A[d], tile_cols<KP, NX>(Ks, d, kb, n, q4), fz);
                     }
+                    settle(A);
                 }
             const float kx = quarters_sum(rowdot(Ks, A));
             if (q4 == 0) kxs[own] = kx;

@@ -372,9 +372,11 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
                 U[j] = zero;
                 mma<NS>(U[j], tf[0], Rx.get(j, n, 8 * q4));
             }
-            if (w >= 2)
+            if (w >= 2) {
 #pragma unroll
                 for (int j = 0; j < CT; ++j) mma<NS>(U[j], tf[1], Rx.get(j, n, 32 + 8 * q4));
+                settle(U);
+            }
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
                 const f32x4 x = U[j] * de;
@@ -519,6 +521,7 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
                 for (int j = 0; j < CT; ++j) uf[j] = Ux.get(j, n, 32 + 8 * q4);
 #pragma unroll
                 for (int j = 0; j < CT; ++j) mma<NS>(O[j], uf[j], mf[1]);
+                settle(O);
             }
             fetch_m(c + 2 < nc ? c + 2 : nc - 1, mf);
             ot.put(O, lane);
