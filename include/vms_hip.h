@@ -513,7 +513,7 @@ typedef struct {
     int32_t dtype, gate_dtype;
     int32_t reverse, for_backward;
     float scale;
-    int32_t reserved;
+    int32_t fp32_states;              /* 1: fp32 accuracy beside 16-bit q, k, v (fp32 ones have it always); the same in the backward */
     const void *q, *k, *v, *g, *beta;
     const float *initial_state;
     const int32_t *seq_lens;

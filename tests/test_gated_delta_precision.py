@@ -17,7 +17,8 @@ import math
 import pytest
 import torch
 
-from test_gated_delta import DTYPES, both, close, compare, inputs
+from mamba_ssm.ops.gated_delta_rule import gated_delta_rule_fn, gated_delta_rule_ref
+from test_gated_delta import DTYPES, TOL, both, close, compare, inputs
 
 PLANES = {torch.float32: math.sqrt(192) * 2**-24, torch.float16: 2**-16, torch.bfloat16: 2**-16}
 
@@ -89,3 +90,77 @@ def test_many_chunks(l, reverse, dtype):
     t = inputs(1, l, 1, 2, 64, 48, dtype, state=True, seed=l)
     t["g"] = t["g"] * 0.01
     compare(t, reverse=reverse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("b, l, hk, h, dk, dv", [(1, 200, 2, 2, 64, 64), (1, 300, 1, 2, 128, 128), (2, 130, 1, 1, 40, 72), (1, 150, 2, 2, 100, 33), (40, 70, 4, 4, 64, 32),
+                                                 (20, 129, 8, 8, 128, 128), (20, 66, 4, 8, 96, 100), (70, 65, 2, 2, 50, 50)])
+def test_fp32_states_of_16_bit_inputs(b, l, hk, h, dk, dv, dtype):
+    """calls with a state in or out carry what they compute to 2^-24: the state, its gradient and those of fp32 gates are off, in the norm, by what fp32 sums leave.
+    A rounding is 2^-24 / sqrt(3) on average: sqrt(64 + 128) of them in a row of sums, four products in a row, each with three residuals of that size:
+    (sqrt(192) + 4 * 3) 2^-24 / sqrt(3) = 9e-7; twice that for what the matrix cores' order of adding costs.  (Two planes leave 4e-6.)"""
+    t = inputs(b, l, hk, h, dk, dv, dtype, state=True, gate_dtype=torch.float32, seed=dk + dv)
+    r = torch.Generator(device="cuda").manual_seed(3)
+    dout = torch.randn(t["v"].shape, generator=r, device="cuda").to(dtype)
+    dfinal = 0.3 * torch.randn(b, h, dk, dv, generator=r, device="cuda")
+    (o, f, g), (o2, f2, g2) = both(t, dout, dfinal, reverse=b > 1)
+    for n, got, want in (("final", f, f2), *((n, g[n], g2[n]) for n in ("initial_state", "g", "beta"))):
+        off = ((got.double() - want).norm() / want.norm()).item()
+        assert got.dtype == torch.float32 and off <= 1.8e-6, (n, off)
+    with torch.no_grad():
+        for kw in ({}, {"initial_state": t["initial_state"]}):
+            x = {n: v for n, v in t.items() if n != "initial_state"} | kw
+            _, got = gated_delta_rule_fn(**x, return_final_state=True, reverse=b > 1)
+            _, want = gated_delta_rule_ref(**{n: v.double() for n, v in x.items()}, return_final_state=True, reverse=b > 1)
+            assert ((got.double() - want).norm() / want.norm()).item() <= 1.8e-6
+
+
+def stateless(t, dout, **kw):
+    """(out, gradients) of the kernels and in 64 bits, no state in or out: 16-bit inputs are carried in two planes"""
+    res = []
+    for fn, cast in ((gated_delta_rule_fn, lambda x: x.detach().clone()), (gated_delta_rule_ref, lambda x: x.detach().double())):
+        leaf = {k: cast(v).requires_grad_() for k, v in t.items()}
+        out = fn(**leaf, **kw)
+        res.append((out, dict(zip(leaf, torch.autograd.grad(out, list(leaf.values()), dout.to(out.dtype))))))
+    return res
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, gate_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("hk, d, cos, beta, decay", [(2, 64, 0.9, 0.95, 0.02), (1, 64, 0.99, 1.0, 0.02), (1, 128, 0.99, 1.0, 0.002)])
+def test_correlated_keys_without_states(hk, d, cos, beta, decay, dtype, gate_dtype):
+    l, h = 512, 2
+    t = inputs(1, l, hk, h, d, d, torch.float32, seed=d + 1)
+    r = torch.Generator(device="cuda").manual_seed(2)
+    common = torch.randn(hk, d, generator=r, device="cuda")
+    common /= common.norm(dim=-1, keepdim=True)
+    for n in ("q", "k"):
+        x = math.sqrt(1 - cos) * t[n] + math.sqrt(cos) * common
+        t[n] = (x / x.norm(dim=-1, keepdim=True)).to(dtype)
+    t["v"] = t["v"].to(dtype)
+    t["g"] = (-decay * torch.rand(1, l, h, generator=r, device="cuda")).to(gate_dtype)
+    t["beta"] = torch.full_like(t["g"], beta)
+    dout = torch.randn(t["v"].shape, generator=r, device="cuda").to(dtype)
+    (o, g), (o2, g2) = stateless(t, dout)
+    norm_close(o, o2, dtype, "out")
+    for n in g:
+        norm_close(g[n], g2[n], dtype, "d" + n, gate_terms({**t, "initial_state": torch.zeros(1, h, d, d, device="cuda")}, g2) if n == "g" else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b, l, hk, h, dk, dv", [(2, 1, 2, 2, 64, 64), (1, 150, 2, 2, 100, 33), (1, 150, 2, 2, 96, 40), (2, 200, 1, 3, 128, 128), (1, 130, 2, 2, 50, 70),
+                                                 (2, 77, 1, 2, 100, 50), (20, 129, 8, 8, 128, 128), (40, 70, 4, 4, 64, 32), (20, 66, 4, 8, 96, 100), (70, 65, 2, 2, 50, 50)])
+def test_training_without_states(b, l, hk, h, dk, dv, dtype):
+    """every form of the kernels that keeps two planes (few and many heads, 64 and 128 wide, whole and odd sizes, shared heads), ragged, both directions"""
+    t = inputs(b, l, hk, h, dk, dv, dtype, gate_dtype=torch.float32, seed=dk + dv)
+    r = torch.Generator(device="cuda").manual_seed(4)
+    dout = torch.randn(t["v"].shape, generator=r, device="cuda").to(dtype)
+    lens = torch.randint(0, l + 1, (b,), generator=r, device="cuda") if b > 2 else None
+    (o, g), (o2, g2) = stateless(t, dout, reverse=b > 1, seq_lens=lens)
+    close(o, o2, TOL[dtype], "out")
+    for n in g:
+        close(g[n], g2[n], TOL[dtype] if dtype == torch.float32 or n in "qkv" else 24 * 2**-16, "d" + n)
+    again = stateless(t, dout, reverse=b > 1, seq_lens=lens)[0]
+    assert torch.equal(again[0], o) and all(torch.equal(again[1][n], g[n]) for n in g)

@@ -10,18 +10,20 @@
 // over the chunks is four products per chunk.
 //
 // Precision.  Everything runs on the bf16 matrix cores with fp32 accumulators.  An operand is the sum of 1 .. 3 bf16 planes
-// (8 bits of the significand each), so that
-//   inputs are exact:                    bf16 1 plane, fp16 2, fp32 3                                         (NX)
-//   whatever is computed is carried with 2 planes, 3 for fp32 inputs: an operand is off by at most 2^-16 of itself (2^-24); accumulators,
-//     the state among them, are fp32                                                                          (NS)
-// 2 planes also where a result is bf16: outputs and gradients are differences of larger terms where keys share a direction, and one plane (2^-8) of M, U
-// or Y then shows 5 to 20 times as large as the result's own rounding (1.7e-3).  Relative error in the norm before that rounding, the algebra above in 64
-// bits with these operands rounded, 512 tokens, bf16, 64 x 64, keys of cosine 0.99 and beta 1 (independent keys, random beta):
-//   one plane of M, S0, U, dS1, Y    out 9.1e-3 (1.7e-3), dq 7.5e-3 (1.7e-3), dg 3.8e-2 (1.9e-3)
-//   two                              out 3.0e-5 (5.2e-6), dq 1.8e-5 (4.5e-6), dg 5.8e-4 (5.4e-6)
-//   three throughout                 out 3.0e-7 (5.8e-8), dq 2.5e-7 (6.3e-8), dg 7.1e-6 (1.6e-7)
-// What two cost: (8, 8192, 8 heads, 128 x 128) 309 -> 353 us, training at (8, 3136, 6 heads, 128 x 128) 416 -> 613 us.  Three would cost 477 and 969 us, and
-// the walks of fp16 with 128-wide keys 172 and 162 KB of the 160 KB of LDS: who wants fp32 states and fp32 gates' gradients to all their bits passes q, k and v in fp32.
+// (8 bits of the significand each: off by at most 2^-8, 2^-16, 2^-24 of itself), so that
+//   inputs are exact:                                                          bf16 1 plane, fp16 2, fp32 3                     (NX)
+//   the state's recurrence in the forward (T, R, U, S as operands):            3, since final states are fp32 whatever the inputs are  (NS)
+//   what enters 16-bit outputs alone (M, U and S0 as their operands):          2, 3 for fp32                                    (NO)
+//   what the backward computes and reads of the forward (S0, U, dS1, Y, ...):  3 for fp32 inputs and where a state comes in or goes out: its gradient and
+//     those of fp32 gates are fp32 then; else 2                                                                                  (NB)
+// Not 1 for bf16 anywhere: outputs and gradients are differences of larger terms where keys share a direction, and a plane's 2^-8 in M, U
+// or Y shows 5 to 20 times as large as the result's own rounding (1.7e-3).  Relative error in the norm before that rounding, the algebra above in 64
+// bits with its operands rounded, 512 tokens, bf16, 64 x 64, keys of cosine 0.99 and beta 1 (independent keys, random beta):
+//   one plane of M, S0, U, dS1, Y, else two   out 9.1e-3 (1.7e-3), dq 7.5e-3 (1.7e-3), dg 3.8e-2 (1.9e-3), final state 2.3e-5 (3.7e-6)
+//   two throughout                            out 3.0e-5 (5.2e-6), dq 1.8e-5 (4.5e-6), dg 5.8e-4 (5.4e-6), final state 2.3e-5 (3.7e-6)
+//   three throughout                          out 3.0e-7 (5.8e-8), dq 2.5e-7 (6.3e-8), dg 7.1e-6 (1.6e-7), final state 3.4e-7 (5.4e-8)
+// Calls of bf16, us: (8, 8192, 8 heads, 128 x 128) 309, 353, 477 (428 with the planes above); training at (8, 3136, 6 heads, 128 x 128) 416, 613, 969
+// (640; with an initial state 909).
 #pragma once
 #include "vms_common.h"
 
@@ -36,9 +38,10 @@ using f32x4 = vec_t<float, 4>;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 template <typename T> struct Prec;
-template <> struct Prec<bf16_t> { static constexpr int NX = 1, NS = 2; };
-template <> struct Prec<f16_t> { static constexpr int NX = 2, NS = 2; };
-template <> struct Prec<float> { static constexpr int NX = 3, NS = 3; };
+constexpr int NS = 3;   // (NB is a parameter of the kernels: planes_kept)
+template <> struct Prec<bf16_t> { static constexpr int NX = 1, NO = 2; };
+template <> struct Prec<f16_t> { static constexpr int NX = 2, NO = 2; };
+template <> struct Prec<float> { static constexpr int NX = 3, NO = 3; };
 
 // An operand of v_mfma_f32_16x16x32_bf16: lane = 16 p + n holds row (A) / column (B) n and 8 of the 32 contracted indices.
 // Two index orders are in use (any order is right as long as both operands share it):
@@ -279,10 +282,11 @@ struct Exchange {
             *reinterpret_cast<vec_t<unsigned, 2>*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at) = u;
         }
     }
-    __device__ __forceinline__ Frag<N> get(int j, int n, int at) const {
-        Frag<N> f;
+    template <int M = N>   // the first M planes
+    __device__ __forceinline__ Frag<M> get(int j, int n, int at) const {
+        Frag<M> f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at);
+        for (int i = 0; i < M; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + i * kPlane + (16 * j + n) * kRow + 2 * at);
         return f;
     }
 };
@@ -324,15 +328,17 @@ struct Layout {
 };
 __host__ __device__ __forceinline__ int ceil_to(int a, int b) { return (a + b - 1) / b * b; }
 __host__ __device__ __forceinline__ int pad_k(int dk) { return dk <= 64 ? 64 : 128; }
+// NB: the planes of what the backward computes and is handed
+inline int planes_kept(const vms_gated_delta_params& p) { return p.dtype == VMS_F32 || p.fp32_states ? 3 : 2; }
 __host__ inline Layout layout(const vms_gated_delta_params& p) {
     Layout l{};
-    const int ns = p.dtype == VMS_F32 ? 3 : 2;   // Prec<T>::NS
+    const int no = p.dtype == VMS_F32 ? 3 : 2, nb = p.for_backward ? planes_kept(p) : 0;   // Prec<T>::NO, the kernels' NB
     l.chunks = (p.seqlen + C - 1) / C;
     l.vpad = ceil_to(p.dv, 32);
     const int64_t slots = (int64_t)p.batch * p.heads * l.chunks;
-    l.tri_slot = (int64_t)(p.for_backward ? 4 : 2) * ns * kTri;   // planes of T, M and, for the backward, their transposes
-    l.s_slot = (int64_t)ns * pad_k(p.dk) * l.vpad * 2;
-    l.u_slot = (int64_t)ns * C * l.vpad * 2;
+    l.tri_slot = (int64_t)(NS + no + 2 * nb) * kTri;   // planes of T, M and, for the backward, their transposes
+    l.s_slot = (int64_t)nb * pad_k(p.dk) * l.vpad * 2;
+    l.u_slot = (int64_t)nb * C * l.vpad * 2;
     int64_t at = 0;
     auto take = [&](int64_t n) { int64_t o = at; at += (n + 255) / 256 * 256; return o; };
     l.tri = take(slots * l.tri_slot);
@@ -380,16 +386,16 @@ inline int allow_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
     if (e != hipSuccess) { set_error("hipFuncSetAttribute: %s", hipGetErrorString(e)); return VMS_ERR_LAUNCH; }
     return VMS_OK;
 }
-// CT accumulator tiles (rows row0 + 4 p + r, column col0 + col_of(j, n)) into NS planes of (rows, vpad): through unit_frag, so that a lane
+// CT accumulator tiles (rows row0 + 4 p + r, column col0 + col_of(j, n)) into N planes of (rows, vpad): through unit_frag, so that a lane
 // stores 4 CT consecutive columns of one row.  vpad is a multiple of 32, so that the 16 CT columns of a slice are always inside
-template <int NS, int CT>
+template <int N, int CT>
 __device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int row0, int col0, const f32x4 (&v)[CT], int n, int p) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    Frag<NS> f[CT];
+    Frag<N> f[CT];
 #pragma unroll
-    for (int j = 0; j < CT; ++j) f[j] = frag_of<NS>(v[j], zero);
+    for (int j = 0; j < CT; ++j) f[j] = frag_of<N>(v[j], zero);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
+    for (int i = 0; i < N; ++i) {
         vec_t<bf16_t, 4 * CT> o;
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
@@ -400,12 +406,12 @@ __device__ __forceinline__ void store_rows(char* base, int rows, int vpad, int r
         *reinterpret_cast<vec_t<bf16_t, 4 * CT>*>(base + 2 * (((int64_t)i * rows + row0 + n) * vpad + col0 + 4 * CT * p)) = o;
     }
 }
-// The same from operands (lane: column col_of(j, n), 32 rows): rows row0 .. of NS planes.  PAIRED: the 16 rows of one half, else both halves
-template <int NS, int CT, bool PAIRED>
-__device__ __forceinline__ void store_frag(char* base, int rows, int vpad, int row0, int half, int col0, const Frag<NS> (&f)[CT], int n, int p) {
+// The same from operands (lane: column col_of(j, n), 32 rows): rows row0 .. of N planes.  PAIRED: the 16 rows of one half, else both halves
+template <int N, int CT, bool PAIRED>
+__device__ __forceinline__ void store_frag(char* base, int rows, int vpad, int row0, int half, int col0, const Frag<N> (&f)[CT], int n, int p) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int hh = 0; hh < (PAIRED ? 1 : 2); ++hh) {
             vec_t<bf16_t, 4 * CT> o;
@@ -451,6 +457,9 @@ struct OTile {
 // 32 (its chain is the same).  (2, 2304, 8 heads, 64 x 64): 32 workgroups 54 us, 64 workgroups 38 us; (8, 8192, 8 heads, 128 x 128): 256 workgroups
 // 265 us, 512 workgroups 404 us.
 inline bool narrow(const vms_gated_delta_params& p, const Layout& l) { return (int64_t)p.batch * p.heads * (l.vpad / 32) <= device_cu_count() / 2; }
+
+// The most columns that the backward's walk takes: the planes of fp32, and three of fp16 beside 128-wide keys, leave LDS for one column tile
+constexpr int bwd_columns(int dtype, int planes, int kp) { return dtype == VMS_F32 || (dtype == VMS_F16 && planes == 3 && kp == 128) ? 16 : 32; }
 
 int validate(const vms_gated_delta_params& p);   // gated_delta_fwd.hip
 

@@ -28,27 +28,27 @@ struct BwdArgs {   // what the kernels need of vms_gated_delta_bwd_params (one k
 // Split among eight waves as the forward's walk: of the chain's four, wave w has token tile w of dU and Y and dk / 4 rows of dS; the other four load, make
 // what depends on no dS (M^T dO, the planes of dO and of scale gam dO) and store.  Bound by the chain (K dS1 -> dU -> Y -> dS0): (8, 3136, 6 heads, 128 x 128) bf16
 // 2.7 us per chunk, 131 us; with all of it on four waves 164 us.
-template <typename T, int KP, int CT, int FIT>
+template <typename T, int NB, int KP, int CT, int FIT>
 struct BwdScanLds {   // bytes and places in LDS
-    static constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    static constexpr int NX = Prec<T>::NX;
     static constexpr int kK = NX * tile_bytes<KP>(), kPiece = VTile<T, CT, FIT != 0>::kBytes, kSum = 4 * CT * 1024;
-    static constexpr int S = 0, O = S + Exchange<NS, CT, KP>::kBytes, G = O + Exchange<NX, CT, C>::kBytes, U = G + Exchange<NS, CT, C>::kBytes,
-                         Y = U + Exchange<NS, CT, C>::kBytes, E = Y + Exchange<NS, CT, C>::kBytes, V = E + kSum, B = V + 4 * kPiece, K = B + 2 * 4 * GateTile::kBytes;
+    static constexpr int S = 0, O = S + Exchange<NB, CT, KP>::kBytes, G = O + Exchange<NX, CT, C>::kBytes, U = G + Exchange<NB, CT, C>::kBytes,
+                         Y = U + Exchange<NB, CT, C>::kBytes, E = Y + Exchange<NB, CT, C>::kBytes, V = E + kSum, B = V + 4 * kPiece, K = B + 2 * 4 * GateTile::kBytes;
     static constexpr bool kStaged = K + 4 * kK <= 163840;   // two tiles each of K and Q; else one each, and K straight into the chain's registers
     static constexpr int Q = K + (kStaged ? 2 : 1) * kK, kBytes = Q + (kStaged ? 2 : 1) * kK;
 };
 
-template <typename T, int KP, int CT, int FIT>
+template <typename T, int NB, int KP, int CT, int FIT>
 __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, const int slices) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    constexpr int NX = Prec<T>::NX, kT = NS + Prec<T>::NO, kM = kT + NB;   // planes of a chunk's slot before the transposes of T, of M
     constexpr int KB = KP / 32, DW = KP / 64;
     constexpr bool WHOLE = FIT != 0;
-    using Lds = BwdScanLds<T, KP, CT, FIT>;
+    using Lds = BwdScanLds<T, NB, KP, CT, FIT>;
     static_assert(Lds::kBytes <= 163840, "160 KB of LDS");
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const Exchange<NS, CT, KP> Sx{lds + Lds::S};
+    const Exchange<NB, CT, KP> Sx{lds + Lds::S};
     const Exchange<NX, CT, C> Ox{lds + Lds::O};                                        // dO
-    const Exchange<NS, CT, C> Gx{lds + Lds::G}, Ux{lds + Lds::U}, Yx{lds + Lds::Y};   // scale gam dO, dU, -beta gam Y
+    const Exchange<NB, CT, C> Gx{lds + Lds::G}, Ux{lds + Lds::U}, Yx{lds + Lds::Y};   // scale gam dO, dU, -beta gam Y
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
@@ -83,10 +83,10 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             r[i] = fit_load<FIT, T>(x.row(at < len ? at : len - 1), piece_col(i), p.dk);
         }
     };
-    auto fetch_tri = [&](int c, int first, Frag<NS> (&f)[2]) __attribute__((always_inline)) {   // columns 16 w + n (row blocks 0, 1; tiles 2 and 3 have no block 0)
-        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;            // first: plane 2 NS for T, 3 NS for M (their transposes)
-        f[0] = tri_cols<NS>(at, w, w >= 2 ? 1 : 0, lane);
-        f[1] = tri_cols<NS>(at, w, 1, lane);
+    auto fetch_tri = [&](int c, int first, Frag<NB> (&f)[2]) __attribute__((always_inline)) {   // columns 16 w + n (row blocks 0, 1; tiles 2 and 3 have no block 0)
+        const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + first * kTri;            // first: kT, kM
+        f[0] = tri_cols<NB>(at, w, w >= 2 ? 1 : 0, lane);
+        f[1] = tri_cols<NB>(at, w, 1, lane);
     };
     auto before = [&](int c, int by) __attribute__((always_inline)) { return c > by ? c - by : 0; };
     // Both sides below meet at three barriers per chunk: dS and M^T dO are there; dU is there; Y is there
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                 Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
             }
         Raw8<T> kr[KB];
-        auto chunk = [&](int c, auto odd_c, Frag<NS> (&tf)[2]) __attribute__((always_inline)) {
+        auto chunk = [&](int c, auto odd_c, Frag<NB> (&tf)[2]) __attribute__((always_inline)) {
             constexpr int odd = decltype(odd_c)::value;
             char* const Ks = k_tile(odd);
             const char* const Qs = q_tile(odd);
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                     tile_put<KP, NX>(Ks, 16 * w + n, 32 * kb + 8 * q4, kf);
                 }
 #pragma unroll
-                for (int j = 0; j < CT; ++j) mma<NS>(dU[j], kf, Sx.get(j, n, 32 * kb + 8 * q4));
+                for (int j = 0; j < CT; ++j) mma<NB>(dU[j], kf, Sx.get(j, n, 32 * kb + 8 * q4));
             }
             if constexpr (!Lds::kStaged) fetch_rows(K, before(c, 1), kr);
             const f32x4 ga = gt.four(0, q4), be = gt.four(1, q4), de = gt.four(2, q4);
@@ -140,11 +140,11 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
                 Y[j] = zero;
-                mma<NS>(Y[j], tf[1], Ux.get(j, n, 32 + 8 * q4));
+                mma<NB>(Y[j], tf[1], Ux.get(j, n, 32 + 8 * q4));
             }
             if (w < 2) {
 #pragma unroll
-                for (int j = 0; j < CT; ++j) mma<NS>(Y[j], tf[0], Ux.get(j, n, 8 * q4));
+                for (int j = 0; j < CT; ++j) mma<NB>(Y[j], tf[0], Ux.get(j, n, 8 * q4));
                 settle(Y);
             }
 #pragma unroll
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                 for (int j = 0; j < CT; ++j) dS[d][j] *= glast;
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
-                Frag<NS> gf[CT], yf[CT];
+                Frag<NB> gf[CT], yf[CT];
 #pragma unroll
                 for (int j = 0; j < CT; ++j) { gf[j] = Gx.get(j, n, 32 * tb + 8 * q4); yf[j] = Yx.get(j, n, 32 * tb + 8 * q4); }
 #pragma unroll
@@ -171,8 +171,8 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                     const Frag<NX> qc = tile_cols<KP, NX>(Qs, DW * w + d, tb, n, q4), kc = tile_cols<KP, NX>(Ks, DW * w + d, tb, n, q4);
 #pragma unroll
                     for (int j = 0; j < CT; ++j) {
-                        mma<NS>(dS[d][j], qc, gf[j]);
-                        mma<NS>(dS[d][j], kc, yf[j]);
+                        mma<NB>(dS[d][j], qc, gf[j]);
+                        mma<NB>(dS[d][j], kc, yf[j]);
                     }
                 }
             }
@@ -180,13 +180,13 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
             for (int d = 0; d < DW; ++d)
 #pragma unroll
                 for (int j = 0; j < CT; ++j) Sx.put(j, n, 16 * (DW * w + d) + 4 * q4, dS[d][j]);
-            fetch_tri(before(c, 2), 2 * NS, tf);
+            fetch_tri(before(c, 2), kT, tf);
         };
         if (nc > 0) {
-            Frag<NS> t0[2], t1[2];
+            Frag<NB> t0[2], t1[2];
             if constexpr (!Lds::kStaged) fetch_rows(K, nc - 1, kr);
-            fetch_tri(nc - 1, 2 * NS, t0);
-            fetch_tri(before(nc - 1, 1), 2 * NS, t1);
+            fetch_tri(nc - 1, kT, t0);
+            fetch_tri(before(nc - 1, 1), kT, t1);
             __syncthreads();   // dO of the last chunk is there, for the other side
             for (int c = nc - 1;;) {
                 chunk(c, std::integral_constant<int, 0>{}, t0);
@@ -251,20 +251,20 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                 for (int r = 0; r < 4; ++r) scaled[j][r] = p.scale * ga[r] * g[r];
             }
         };
-        auto other_grad = [&](const Frag<NS> (&mf)[2]) __attribute__((always_inline)) {   // M^T dO
+        auto other_grad = [&](const Frag<NB> (&mf)[2]) __attribute__((always_inline)) {   // M^T dO
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
                 f32x4 e = zero;
-                mma<NS>(e, mf[1], Ox.get(j, n, 32 + 8 * q4));
+                mma<NB>(e, mf[1], Ox.get(j, n, 32 + 8 * q4));
                 if (w < 2) {
-                    mma<NS>(e, mf[0], Ox.get(j, n, 8 * q4));
+                    mma<NB>(e, mf[0], Ox.get(j, n, 8 * q4));
                     settle(e);
                 }
                 sums[64 * j] = e;
             }
         };
         Raw8<T> qr[KB];
-        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NS> (&mf)[2]) __attribute__((always_inline)) {   // other, mf: of chunk c - 1
+        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NB> (&mf)[2]) __attribute__((always_inline)) {   // other, mf: of chunk c - 1
             constexpr int odd = decltype(odd_c)::value;
             const int64_t slot = slot0 + c;
             __syncthreads();
@@ -277,10 +277,10 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
                 fetch_rows(Q, before(c, 1), qr);
             }
             if (w < KB) {
-                Frag<NS> sf[CT];
+                Frag<NB> sf[CT];
 #pragma unroll
                 for (int j = 0; j < CT; ++j) sf[j] = Sx.get(j, n, 32 * w + 8 * q4);
-                store_frag<NS, CT, false>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
+                store_frag<NB, CT, false>(wb + l.dS + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
             }
             fetch_k(before(c, 2), mine);
             __syncthreads();
@@ -293,32 +293,32 @@ __global__ __launch_bounds__(512, 1) void gd_bwd_scan_kernel(const BwdArgs a, co
 #pragma unroll
             for (int j = 0; j < CT; ++j) Y[j] = sums[64 * j];
             other_grad(mf);
-            fetch_tri(before(c, 3), 3 * NS, mf);
+            fetch_tri(before(c, 3), kM, mf);
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
-                const Frag<NS> f = frag_of<NS>(be * Y[j], zero);
+                const Frag<NB> f = frag_of<NB>(be * Y[j], zero);
                 dv[j] = zero;
 #pragma unroll
-                for (int i = NS - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
+                for (int i = NB - 1; i >= 0; --i) dv[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], unit_frag(0, n, q4), dv[j], 0, 0, 0);
             }
-            store_rows<NS, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
+            store_rows<NB, CT>(wb + l.Y + slot * l.u_slot, C, l.vpad, 16 * w, col0, Y, n, q4);
             ot.put(dv, lane);
         };
         if (nc > 0) {
             Ahead a0, a1;
-            Frag<NS> m0[2], m1[2];
+            Frag<NB> m0[2], m1[2];
             if constexpr (!Lds::kStaged) fetch_rows(Q, nc - 1, qr);
             auto fetch = [&](int c, Ahead& x) __attribute__((always_inline)) { fetch_k(c, x); fetch_q(c, x); fetch_small(c, x); };
             fetch(nc - 1, a0);
             fetch(before(nc - 1, 1), a1);
-            fetch_tri(nc - 1, 3 * NS, m0);
-            fetch_tri(before(nc - 1, 1), 3 * NS, m1);
+            fetch_tri(nc - 1, kM, m0);
+            fetch_tri(before(nc - 1, 1), kM, m1);
             hand(nc - 1, std::integral_constant<int, 0>{}, a0);
             fetch_q(before(nc - 1, 2), a0);
             fetch_small(before(nc - 1, 2), a0);
             __syncthreads();
             other_grad(m0);
-            fetch_tri(before(nc - 1, 2), 3 * NS, m0);
+            fetch_tri(before(nc - 1, 2), kM, m0);
             for (int c = nc - 1;;) {
                 chunk(c, std::integral_constant<int, 0>{}, a0, a1, m1);
                 if (--c < 0) break;
@@ -350,9 +350,9 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
 // wave w has token tile w % 4 of dQ and W (w < 4: "left", what depends on the token as the later one) or of X (w >= 4: "right"), so that no product is
 // made twice and the accumulators fit.  (8, 3136, 6 heads, 128 x 128) bf16: 145 us for 0.45 GB and 30 GFLOP of bf16 products; bound by the steps between
 // the barriers (a workgroup of eight waves fills a CU's registers).  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
-template <typename T, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
+template <typename T, int NB, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
 __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS, DT = KP / 16, TB = tile_bytes<KP>();
+    constexpr int NX = Prec<T>::NX, DT = KP / 16, TB = tile_bytes<KP>();
     constexpr int PK = C * KP / 8 / 512;   // 8-element pieces of a q / k tile per thread
     constexpr int ROW = 80;                 // bytes of 32 columns in LDS: 16 rows fall on all banks
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -366,10 +366,10 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     char* const Qs = Ks + NX * TB;
     f32x4* const Wx = reinterpret_cast<f32x4*>(Qs + NX * TB);   // beta W, from the left wave to the right one
     char* const Us = big;          // stage 1
-    char* const Ys = Us + NS * C * ROW;
-    char* const Os = Ys + NS * C * ROW;
+    char* const Ys = Us + NB * C * ROW;
+    char* const Os = Ys + NB * C * ROW;
     char* const Ss = Os + NX * C * ROW;
-    char* const Ds = Ss + NS * KP * ROW;
+    char* const Ds = Ss + NB * KP * ROW;
 
     const vms_gated_delta_params& p = a.q.f;
     const Layout& l = a.l;
@@ -455,12 +455,12 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
         const Rows<T> V(p.v, (int64_t)b * p.v_batch_stride + (int64_t)h * p.v_head_stride, p.v_seq_stride, len, p.reverse);
         const Rows<T> dO(a.q.dout, (int64_t)b * a.q.dout_batch_stride + (int64_t)h * a.q.dout_head_stride, a.q.dout_seq_stride, len, p.reverse);
         const T* const brow = (left ? dO : V).row(ok_p ? at_p : len - 1);
-        Frag<NS> ap, sp, dp;
+        Frag<NB> ap, sp, dp;
         Raw8<T> bp;
         auto fetch = [&](int vk) __attribute__((always_inline)) {
             const int cc = 32 * vk + pcol;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
+            for (int i = 0; i < NB; ++i) {
                 ap.p[i] = *reinterpret_cast<const bf16x8*>(Aw + 2 * (((int64_t)i * C + prow) * l.vpad + cc));
                 sp.p[i] = *reinterpret_cast<const bf16x8*>(Sw + 2 * (((int64_t)i * KP + srow) * l.vpad + cc));
                 dp.p[i] = *reinterpret_cast<const bf16x8*>(Dw + 2 * (((int64_t)i * KP + srow) * l.vpad + cc));
@@ -468,10 +468,10 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             bp = load_raw8<WHOLE, T>(brow, cc, p.dv);
         };
         float yv = 0.f, ss = 0.f;   // this thread's part of Y.V (its token), of <S0, dS1>
-        auto value = [&](const Frag<NS>& f, int e) __attribute__((always_inline)) {
+        auto value = [&](const Frag<NB>& f, int e) __attribute__((always_inline)) {
             float x = 0.f;
 #pragma unroll
-            for (int i = NS - 1; i >= 0; --i) x += static_cast<float>(f.p[i][e]);
+            for (int i = NB - 1; i >= 0; --i) x += static_cast<float>(f.p[i][e]);
             return x;
         };
         auto hand = [&](int vk) __attribute__((always_inline)) {
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             char* const at = (left ? Us : Ys) + prow * ROW + 2 * pcol;
             char* const as = Ss + srow * ROW + 2 * pcol;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
+            for (int i = 0; i < NB; ++i) {
                 *reinterpret_cast<bf16x8*>(at + i * C * ROW) = ap.p[i];
                 if (has_s) {
                     *reinterpret_cast<bf16x8*>(as + i * KP * ROW) = sp.p[i];
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
             for (int i = 0; i < decltype(planes)::value; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(base + (i * rows + row) * ROW + 16 * q4);
             return f;
         };
-        constexpr std::integral_constant<int, NS> ns{};
+        constexpr std::integral_constant<int, NB> nb{};
         constexpr std::integral_constant<int, NX> nx{};
         // 64 x 64 products [j][i]: rows = another tile's tokens, columns (lanes) = this wave's.  left: m = dO_i.U_j, z = Y_i.U_j with this wave's tokens as i
         // (tiles j <= w); right: with this wave's tokens as j (tiles i >= w).  A: left dO S0^T -> dQ, right U dS1^T -> X;  B: left Y S0^T -> W
@@ -516,36 +516,36 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
         for (int d = 0; d < DT; ++d) { A[d] = zero; B[d] = zero; }
         auto multiply = [&]() __attribute__((always_inline)) {
             if (left) {
-                const Frag<NS> yi = from(Ys, C, own, ns);
+                const Frag<NB> yi = from(Ys, C, own, nb);
                 const Frag<NX> oi = from(Os, C, own, nx);
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
                     if (t <= w) {
-                        const Frag<NS> uj = from(Us, C, 16 * t + n, ns);
-                        mma<NS>(m[t], uj, oi);
-                        mma<NS>(z[t], uj, yi);
+                        const Frag<NB> uj = from(Us, C, 16 * t + n, nb);
+                        mma<NB>(m[t], uj, oi);
+                        mma<NB>(z[t], uj, yi);
                         asm volatile("" : "+v"(m[t]));
                         settle(z[t]);
                     }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const Frag<NS> s0 = from(Ss, KP, 16 * d + n, ns);
-                    mma<NS>(A[d], s0, oi);
-                    mma<NS>(B[d], s0, yi);
+                    const Frag<NB> s0 = from(Ss, KP, 16 * d + n, nb);
+                    mma<NB>(A[d], s0, oi);
+                    mma<NB>(B[d], s0, yi);
                 }
                 settle(A, B);
             } else {
-                const Frag<NS> ui = from(Us, C, own, ns);
+                const Frag<NB> ui = from(Us, C, own, nb);
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
                     if (t >= w) {
-                        mma<NS>(m[t], from(Os, C, 16 * t + n, nx), ui);
-                        mma<NS>(z[t], from(Ys, C, 16 * t + n, ns), ui);
+                        mma<NB>(m[t], from(Os, C, 16 * t + n, nx), ui);
+                        mma<NB>(z[t], from(Ys, C, 16 * t + n, nb), ui);
                         asm volatile("" : "+v"(m[t]));
                         settle(z[t]);
                     }
 #pragma unroll
-                for (int d = 0; d < DT; ++d) mma<NS>(A[d], from(Ds, KP, 16 * d + n, ns), ui);
+                for (int d = 0; d < DT; ++d) mma<NB>(A[d], from(Ds, KP, 16 * d + n, nb), ui);
                 settle(A);
             }
         };
@@ -622,12 +622,12 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 if (2 * kb <= w) {
-                    const Frag<NS> fm = frag_of<NS>(m[2 * kb], m[2 * kb + 1]), fz = frag_of<NS>(z[2 * kb], z[2 * kb + 1]);
+                    const Frag<NB> fm = frag_of<NB>(m[2 * kb], m[2 * kb + 1]), fz = frag_of<NB>(z[2 * kb], z[2 * kb + 1]);
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
                         const Frag<NX> kc = tile_cols<KP, NX>(Ks, d, kb, n, q4);
-                        mma<NS>(A[d], kc, fm);
-                        mma<NS>(B[d], kc, fz);
+                        mma<NB>(A[d], kc, fm);
+                        mma<NB>(B[d], kc, fz);
                     }
                     settle(A, B);
                 }
@@ -659,11 +659,11 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 if (2 * kb + 1 >= w) {
-                    const Frag<NS> fm = frag_of<NS>(m[2 * kb], m[2 * kb + 1]), fz = frag_of<NS>(z[2 * kb], z[2 * kb + 1]);
+                    const Frag<NB> fm = frag_of<NB>(m[2 * kb], m[2 * kb + 1]), fz = frag_of<NB>(z[2 * kb], z[2 * kb + 1]);
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        mma<NS>(A[d], tile_cols<KP, NX>(Qs, d, kb, n, q4), fm);
-                        mma<NS>(A[d], tile_cols<KP, NX>(Ks, d, kb, n, q4), fz);
+                        mma<NB>(A[d], tile_cols<KP, NX>(Qs, d, kb, n, q4), fm);
+                        mma<NB>(A[d], tile_cols<KP, NX>(Ks, d, kb, n, q4), fz);
                     }
                     settle(A);
                 }
@@ -700,47 +700,49 @@ __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
-template <typename T, int KP, int CT, int FIT>
+template <typename T, int NB, int KP, int CT, int FIT>
 static int bwd_scan_launch(const BwdArgs& a, hipStream_t s) {
-    constexpr int lds = BwdScanLds<T, KP, CT, FIT>::kBytes;
+    constexpr int lds = BwdScanLds<T, NB, KP, CT, FIT>::kBytes;
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, KP, CT, FIT>), lds)) return rc;
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_bwd_scan_kernel<T, NB, KP, CT, FIT>), lds)) return rc;
     const int slices = (a.l.vpad + CT * 16 - 1) / (CT * 16);
-    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, KP, CT, FIT>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(512), lds, s, a, slices);
+    hipLaunchKernelGGL((gd_bwd_scan_kernel<T, NB, KP, CT, FIT>), dim3(a.q.f.batch * a.q.f.heads * slices), dim3(512), lds, s, a, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-template <typename T, int KP, int CT>
+template <typename T, int NB, int KP, int CT>
 static int bwd_scan_fit(const BwdArgs& a, int fit, hipStream_t s) {
-    return fit == 2 ? bwd_scan_launch<T, KP, CT, 2>(a, s) : fit == 1 ? bwd_scan_launch<T, KP, CT, 1>(a, s) : bwd_scan_launch<T, KP, CT, 0>(a, s);
+    return fit == 2 ? bwd_scan_launch<T, NB, KP, CT, 2>(a, s) : fit == 1 ? bwd_scan_launch<T, NB, KP, CT, 1>(a, s) : bwd_scan_launch<T, NB, KP, CT, 0>(a, s);
 }
-template <typename T, int KP, bool WHOLE, bool SHARED>
+template <typename T, int NB, int KP, bool WHOLE, bool SHARED>
 static int grad_launch(const BwdArgs& a, hipStream_t s) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    constexpr int one = (2 * NS + NX) * C * 80 + 2 * NS * KP * 80, two = 2 * NX * tile_bytes<KP>() + C * KP * 4;
+    constexpr int NX = Prec<T>::NX;
+    constexpr int one = (2 * NB + NX) * C * 80 + 2 * NB * KP * 80, two = 2 * NX * tile_bytes<KP>() + C * KP * 4;
     constexpr int lds = (int)sizeof(Gates) + (3 * C + 8) * 4 + (one > two ? one : two);
     static_assert(lds <= 163840, "160 KB of LDS");
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_grad_kernel<T, KP, WHOLE, SHARED>), lds)) return rc;
-    hipLaunchKernelGGL((gd_grad_kernel<T, KP, WHOLE, SHARED>), dim3(a.l.chunks, a.q.f.heads_k, a.q.f.batch), dim3(512), lds, s, a);
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_grad_kernel<T, NB, KP, WHOLE, SHARED>), lds)) return rc;
+    hipLaunchKernelGGL((gd_grad_kernel<T, NB, KP, WHOLE, SHARED>), dim3(a.l.chunks, a.q.f.heads_k, a.q.f.batch), dim3(512), lds, s, a);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-template <typename T, int KP>
+template <typename T, int NB, int KP>
 static int bwd_launch(const BwdArgs& a, hipStream_t s) {
     const int fit = fit_of(a.q.f.dk, a.q.f.dv);
     int rc;
-    if constexpr (sizeof(T) == 4)   // (fp32: the six planes of K and Q leave LDS for one column tile)
-        rc = bwd_scan_fit<T, KP, 1>(a, fit, s);
+    if constexpr (bwd_columns(sizeof(T) == 4 ? VMS_F32 : std::is_same_v<T, f16_t> ? VMS_F16 : VMS_BF16, NB, KP) == 16)
+        rc = bwd_scan_fit<T, NB, KP, 1>(a, fit, s);
     else
-        rc = narrow(a.q.f, a.l) ? bwd_scan_fit<T, KP, 1>(a, fit, s) : bwd_scan_fit<T, KP, 2>(a, fit, s);
+        rc = narrow(a.q.f, a.l) ? bwd_scan_fit<T, NB, KP, 1>(a, fit, s) : bwd_scan_fit<T, NB, KP, 2>(a, fit, s);
     if (rc) return rc;
-    if (a.q.f.heads == a.q.f.heads_k) return fit ? grad_launch<T, KP, true, false>(a, s) : grad_launch<T, KP, false, false>(a, s);
-    return fit ? grad_launch<T, KP, true, true>(a, s) : grad_launch<T, KP, false, true>(a, s);
+    if (a.q.f.heads == a.q.f.heads_k) return fit ? grad_launch<T, NB, KP, true, false>(a, s) : grad_launch<T, NB, KP, false, false>(a, s);
+    return fit ? grad_launch<T, NB, KP, true, true>(a, s) : grad_launch<T, NB, KP, false, true>(a, s);
 }
 template <typename T>
 static int bwd_type(const BwdArgs& a, hipStream_t s) {
-    return pad_k(a.q.f.dk) == 64 ? bwd_launch<T, 64>(a, s) : bwd_launch<T, 128>(a, s);
+    if constexpr (sizeof(T) == 2)
+        if (planes_kept(a.q.f) == 2) return pad_k(a.q.f.dk) == 64 ? bwd_launch<T, 2, 64>(a, s) : bwd_launch<T, 2, 128>(a, s);
+    return pad_k(a.q.f.dk) == 64 ? bwd_launch<T, 3, 64>(a, s) : bwd_launch<T, 3, 128>(a, s);
 }
 
 }  // namespace gd

@@ -22,9 +22,9 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __bui
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
-template <typename T, int KP, int FIT, bool TRAIN>
+template <typename T, int KP, int FIT, int NB>
 __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_params p, const Layout l) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    constexpr int NX = Prec<T>::NX, NO = Prec<T>::NO;
     constexpr int AR = 68;   // row pitch of As, floats
     __shared__ __attribute__((aligned(16))) float As[C * AR];
     __shared__ __attribute__((aligned(32))) double Gs[C];
@@ -85,14 +85,14 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 
     char* const tw = ws + l.tri + slot * l.tri_slot;
     char* const mw = tw + NS * kTri;
-    char* const ttw = mw + NS * kTri;   // transposes (for_backward)
-    char* const mtw = ttw + NS * kTri;
-    auto put4 = [&](char* at, const f32x4& v) __attribute__((always_inline)) {   // half an operand, NS planes
+    char* const ttw = mw + NO * kTri;   // transposes (for_backward)
+    char* const mtw = ttw + NB * kTri;
+    auto put4 = [&](char* at, const f32x4& v) __attribute__((always_inline)) {   // half an operand, NB planes
         float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
-        Frag<NS> f;
-        split<NS>(x, f);
+        Frag<NB ? NB : 1> f;
+        split<NB ? NB : 1>(x, f);
 #pragma unroll
-        for (int i2 = 0; i2 < NS; ++i2) *reinterpret_cast<bf16x4*>(at + i2 * kTri) = __builtin_shufflevector(f.p[i2], f.p[i2], 0, 1, 2, 3);
+        for (int i2 = 0; i2 < NB; ++i2) *reinterpret_cast<bf16x4*>(at + i2 * kTri) = __builtin_shufflevector(f.p[i2], f.p[i2], 0, 1, 2, 3);
     };
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
@@ -112,8 +112,8 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
             for (int ct = 0; ct <= rt; ++ct) {   // [j][i]: lane i, 4 consecutive j
                 const Frag<NX> kj = ct == rt ? ki : as_frag(kraw[ct][kb], kb);
                 mma<NS>(kk[ct], kj, ki);
-                mma<NS>(qk[ct], kj, qi);
-                if (TRAIN) mma<NS>(kq[ct], qi, kj);
+                mma<NO>(qk[ct], kj, qi);
+                if constexpr (NB > 0) mma<NB>(kq[ct], qi, kj);
             }
         }
         const int i = 16 * rt + n;
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
                 qk[ct][r] = j <= i ? y : 0.f;
             }
             *reinterpret_cast<f32x4*>(&As[i * AR + 16 * ct + 4 * q4]) = a;
-            if (TRAIN) {
+            if constexpr (NB > 0) {
                 const int j = 16 * ct + n;
                 const double Gn = Gs[j];
                 const f64x4 G4 = *reinterpret_cast<const f64x4*>(&Gs[16 * rt + 4 * q4]);
@@ -145,12 +145,12 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
                 put4(mtw + 1024 * tri_t(ct, rt >> 1) + 16 * lane + 8 * (rt & 1), kq[ct]);
             }
         }
-        if (TRAIN && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
+        if (NB > 0 && (rt & 1) == 0) put4(mtw + 1024 * tri_t(rt + 1, rt >> 1) + 16 * lane, f32x4{0.f, 0.f, 0.f, 0.f});   // above the diagonal
 #pragma unroll
         for (int kb = 0; kb <= rt / 2; ++kb) {
-            const Frag<NS> f = frag_of<NS>(qk[2 * kb], qk[2 * kb + 1]);
+            const Frag<NO> f = frag_of<NO>(qk[2 * kb], qk[2 * kb + 1]);
 #pragma unroll
-            for (int i2 = 0; i2 < NS; ++i2)
+            for (int i2 = 0; i2 < NO; ++i2)
                 *reinterpret_cast<bf16x8*>(mw + i2 * kTri + 1024 * tri(rt, kb) + 16 * lane) = f.p[i2];
         }
     }
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 #pragma unroll
             for (int i2 = 0; i2 < NS; ++i2) *reinterpret_cast<bf16x8*>(tw + i2 * kTri + 1024 * tri(rt, kb) + 16 * lane) = f.p[i2];
         }
-    if (TRAIN) {
+    if constexpr (NB > 0) {
 #pragma unroll
         for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -254,27 +254,29 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 // Lines: an operand's lanes are 16 rows x 4 pieces of 16 bytes with neighbouring lanes in different rows, and the memory pipe then takes 64 accesses
 // for a load of 1 KB instead of 16 (2825 of a chunk's 5100 cycles).  Read as lines, through LDS into operands, K also stands there for its transpose.  Asked
 // for two chunks ahead (one chunk is less than a loaded memory's latency) and spread over the phases: a wave stands still while the pipe is full.
-template <typename T, int KP, int CT, int FIT>
+template <typename T, int KP, int CT, int FIT, int NB>
 struct ScanLds {   // bytes and places in LDS
-    static constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
-    static constexpr bool kStaged = !(sizeof(T) == 4 && KP == 128);   // K and Q come through LDS; two tiles of three planes do not fit
-    static constexpr int kK = NX * tile_bytes<KP>(), kPiece = VTile<T, CT, FIT != 0>::kBytes;
-    static constexpr int kQRow = KP * (int)sizeof(T) + 16, kQ = kStaged ? 16 * kQRow : 0;   // per wave
-    static constexpr int S = (kStaged ? 2 : 1) * kK, R = S + Exchange<NS, CT, KP>::kBytes, U = R + Exchange<NS, CT, C>::kBytes, D = U + Exchange<NS, CT, C>::kBytes,
+    static constexpr int NX = Prec<T>::NX, NU = NB > Prec<T>::NO ? NB : Prec<T>::NO;   // planes of U: what M U and the backward need
+    static constexpr int kK = NX * tile_bytes<KP>(), kPiece = VTile<T, CT, FIT != 0>::kBytes, kQRow = KP * (int)sizeof(T) + 16;
+    static constexpr int kRest = Exchange<NS, CT, KP>::kBytes + 2 * Exchange<NS, CT, C>::kBytes + Exchange<NU, CT, C>::kBytes + 3 * 4 * kPiece + 2 * 4 * GateTile::kBytes;
+    static constexpr bool kStaged = 2 * kK + kRest + 4 * 16 * kQRow <= 163840;   // K and Q come through LDS; with many planes two tiles do not fit
+    static constexpr int kQ = kStaged ? 16 * kQRow : 0;   // per wave
+    static constexpr int S = (kStaged ? 2 : 1) * kK, R = S + Exchange<NS, CT, KP>::kBytes, U = R + Exchange<NS, CT, C>::kBytes, D = U + Exchange<NU, CT, C>::kBytes,
                          V = D + Exchange<NS, CT, C>::kBytes,           // V, O: one and one per wave and buffer
                          G = V + 3 * 4 * kPiece, Q = G + 2 * 4 * GateTile::kBytes, kBytes = Q + 4 * kQ;
     static_assert(kBytes <= 163840, "160 KB of LDS");
 };
 
-template <typename T, int KP, int CT, int FIT, bool TRAIN>
+template <typename T, int KP, int CT, int FIT, int NB>
 __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_params p, const Layout l, const int slices) {
-    constexpr int NX = Prec<T>::NX, NS = Prec<T>::NS;
+    constexpr int NX = Prec<T>::NX, NO = Prec<T>::NO;
     constexpr int KB = KP / 32, DW = KP / 64;   // 32-column blocks of k; 16-row tiles of S per wave
     constexpr bool WHOLE = FIT != 0;
-    using Lds = ScanLds<T, KP, CT, FIT>;
+    using Lds = ScanLds<T, KP, CT, FIT, NB>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const Exchange<NS, CT, KP> Sx{lds + Lds::S};
-    const Exchange<NS, CT, C> Rx{lds + Lds::R}, Ux{lds + Lds::U}, Dx{lds + Lds::D};   // R, U, del U
+    const Exchange<NS, CT, C> Rx{lds + Lds::R}, Dx{lds + Lds::D};   // R, del U
+    const Exchange<Lds::NU, CT, C> Ux{lds + Lds::U};
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
@@ -442,10 +444,10 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
             VTile<T, CT, WHOLE> v;
             GateTile g;
         };
-        auto fetch_m = [&](int c, Frag<NS> (&m)[2]) __attribute__((always_inline)) {   // rows 16 w + n of M
+        auto fetch_m = [&](int c, Frag<NO> (&m)[2]) __attribute__((always_inline)) {   // rows 16 w + n of M
             const char* const at = ws + l.tri + (slot0 + c) * l.tri_slot + NS * kTri;
-            m[0] = tri_rows<NS>(at, w, 0, lane);
-            m[1] = tri_rows<NS>(at, w, w >= 2 ? 1 : 0, lane);
+            m[0] = tri_rows<NO>(at, w, 0, lane);
+            m[1] = tri_rows<NO>(at, w, w >= 2 ? 1 : 0, lane);
         };
         auto fetch_q = [&](int c, Ahead& a) __attribute__((always_inline)) {
             if constexpr (Lds::kStaged) fetch_lines(Q, c, a.q);
@@ -474,7 +476,7 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
         };
         const OTile<T, CT, WHOLE> ot{v_at(2)};
         Raw8<T> qr[KB];
-        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NS> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
+        auto chunk = [&](int c, auto odd_c, Ahead& mine, Ahead& other, Frag<NO> (&mf)[2]) __attribute__((always_inline)) {   // other: of chunk c + 1
             constexpr int odd = decltype(odd_c)::value;
             const int64_t slot = slot0 + c;
             __syncthreads();
@@ -490,14 +492,14 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
                 else x = fit_clear<FIT, T>(qr[kb], 32 * kb + 8 * q4, p.dk);
                 const Frag<NX> qf = planes_of<T>(x);
 #pragma unroll
-                for (int j = 0; j < CT; ++j) mma<NS>(O[j], Sx.get(j, n, 32 * kb + 8 * q4), qf);
+                for (int j = 0; j < CT; ++j) mma<NO>(O[j], Sx.template get<NO>(j, n, 32 * kb + 8 * q4), qf);
             }
-            if constexpr (TRAIN) {
+            if constexpr (NB > 0) {
                 if (w < KB) {   // S0, 32 rows per wave
-                    Frag<NS> sf[CT];
+                    Frag<NB> sf[CT];
 #pragma unroll
-                    for (int j = 0; j < CT; ++j) sf[j] = Sx.get(j, n, 32 * w + 8 * q4);
-                    store_frag<NS, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
+                    for (int j = 0; j < CT; ++j) sf[j] = Sx.template get<NB>(j, n, 32 * w + 8 * q4);
+                    store_frag<NB, CT, false>(ws + l.S0 + slot * l.s_slot, KP, l.vpad, 32 * w, 0, col0, sf, n, q4);
                 }
             }
             if constexpr (!Lds::kStaged) fetch_rows(Q, c + 1 < nc ? c + 1 : c, qr);
@@ -511,25 +513,25 @@ __global__ __launch_bounds__(512, 1) void gd_scan_kernel(const vms_gated_delta_p
 #pragma unroll
             for (int j = 0; j < CT; ++j) O[j] *= sg;
             // O += M U
-            Frag<NS> uf[CT];
+            Frag<Lds::NU> uf[CT];
 #pragma unroll
             for (int j = 0; j < CT; ++j) uf[j] = Ux.get(j, n, 8 * q4);
 #pragma unroll
-            for (int j = 0; j < CT; ++j) mma<NS>(O[j], uf[j], mf[0]);
+            for (int j = 0; j < CT; ++j) mma<NO>(O[j], uf[j], mf[0]);
             if (w >= 2) {
 #pragma unroll
                 for (int j = 0; j < CT; ++j) uf[j] = Ux.get(j, n, 32 + 8 * q4);
 #pragma unroll
-                for (int j = 0; j < CT; ++j) mma<NS>(O[j], uf[j], mf[1]);
+                for (int j = 0; j < CT; ++j) mma<NO>(O[j], uf[j], mf[1]);
                 settle(O);
             }
             fetch_m(c + 2 < nc ? c + 2 : nc - 1, mf);
             ot.put(O, lane);
-            if constexpr (TRAIN) store_frag<NS, CT, true>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, w & 1, col0, uf, n, q4);
+            if constexpr (NB > 0) store_frag<NB, CT, true>(ws + l.U + slot * l.u_slot, C, l.vpad, 16 * w, w & 1, col0, uf, n, q4);
         };
         if (nc > 0) {
             Ahead a0, a1;
-            Frag<NS> m0[2], m1[2];
+            Frag<NO> m0[2], m1[2];
             if constexpr (!Lds::kStaged) fetch_rows(Q, 0, qr);
             auto fetch = [&](int c, Ahead& a) __attribute__((always_inline)) { fetch_k(c, a); fetch_v(c, a); fetch_q(c, a); };
             fetch(0, a0);
@@ -564,8 +566,8 @@ int validate(const vms_gated_delta_params& p) {
     VMS_CHECK(p.dk >= 1 && p.dk <= 128, "key heads of 1 .. 128");
     VMS_CHECK(p.dv >= 1 && p.dv <= 4096, "value heads of 1 .. 4096");
     VMS_CHECK(p.heads <= 65535 && p.batch <= 65535 && p.seqlen <= (1 << 30), "problem too large");
-    // the walks' launches of 512 threads have to stay below 2^32 threads: 32 columns per workgroup, 16 in the fp32 backward (fewer workgroups take 16 only where they are few)
-    const int least = p.for_backward && p.dtype == VMS_F32 ? 16 : 32;
+    // the walks' launches of 512 threads have to stay below 2^32 threads (fewer columns than these only where workgroups are few)
+    const int least = p.for_backward ? bwd_columns(p.dtype, planes_kept(p), pad_k(p.dk)) : 32;
     VMS_CHECK((int64_t)p.batch * p.heads * (ceil_to(p.dv, 32) / least) < (1LL << 32) / 512, "problem too large");
     VMS_CHECK(p.q && p.k && p.v && p.g && p.beta, "q, k, v, g, beta are required");
     for (const int64_t n : {p.q_seq_stride, p.k_seq_stride, p.v_seq_stride, p.out_seq_stride})
@@ -576,26 +578,29 @@ int validate(const vms_gated_delta_params& p) {
     return VMS_OK;
 }
 
-template <typename T, int KP, int CT, int FIT, bool TRAIN>
+template <typename T, int KP, int CT, int FIT, int NB>
 static int scan_launch(const vms_gated_delta_params& p, const Layout& l, hipStream_t s) {
-    constexpr int lds = ScanLds<T, KP, CT, FIT>::kBytes;
+    constexpr int lds = ScanLds<T, KP, CT, FIT, NB>::kBytes;
     static PerDeviceOnce once;
-    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, CT, FIT, TRAIN>), lds)) return rc;
+    if (int rc = allow_lds(once, reinterpret_cast<const void*>(&gd_scan_kernel<T, KP, CT, FIT, NB>), lds)) return rc;
     const int slices = (l.vpad + CT * 16 - 1) / (CT * 16);
-    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, FIT, TRAIN>), dim3(p.batch * p.heads * slices), dim3(512), lds, s, p, l, slices);
+    hipLaunchKernelGGL((gd_scan_kernel<T, KP, CT, FIT, NB>), dim3(p.batch * p.heads * slices), dim3(512), lds, s, p, l, slices);
     VMS_LAUNCH_CHECK();
     return VMS_OK;
 }
-template <typename T, int KP, int FIT, bool TRAIN>
+template <typename T, int KP, int FIT, int NB>
 static int fwd_launch(const vms_gated_delta_params& p, hipStream_t s) {
     const Layout l = layout(p);
-    hipLaunchKernelGGL((gd_prep_kernel<T, KP, FIT, TRAIN>), dim3(l.chunks, p.heads, p.batch), dim3(64), 0, s, p, l);
+    hipLaunchKernelGGL((gd_prep_kernel<T, KP, FIT, NB>), dim3(l.chunks, p.heads, p.batch), dim3(64), 0, s, p, l);
     VMS_LAUNCH_CHECK();
-    return narrow(p, l) ? scan_launch<T, KP, 1, FIT, TRAIN>(p, l, s) : scan_launch<T, KP, 2, FIT, TRAIN>(p, l, s);
+    return narrow(p, l) ? scan_launch<T, KP, 1, FIT, NB>(p, l, s) : scan_launch<T, KP, 2, FIT, NB>(p, l, s);
 }
 template <typename T, int KP, int FIT>
 static int fwd_train(const vms_gated_delta_params& p, hipStream_t s) {
-    return p.for_backward ? fwd_launch<T, KP, FIT, true>(p, s) : fwd_launch<T, KP, FIT, false>(p, s);
+        if (!p.for_backward) return fwd_launch<T, KP, FIT, 0>(p, s);
+    if constexpr (sizeof(T) == 2)
+        if (planes_kept(p) == 2) return fwd_launch<T, KP, FIT, 2>(p, s);
+    return fwd_launch<T, KP, FIT, 3>(p, s);
 }
 template <typename T, int KP>
 static int fwd_fit(const vms_gated_delta_params& p, hipStream_t s) {

@@ -1005,11 +1005,11 @@ void gated_delta_checks(const Tensor& q, const Tensor& k, const Tensor& v, const
 }
 
 void gated_delta_fill(vms_gated_delta_params& p, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale,
-                      const Tensor& seq_lens, bool reverse, bool for_backward) {
+                      const Tensor& seq_lens, bool reverse, bool for_backward, bool fp32_states) {
     p.batch = v.size(0); p.seqlen = v.size(1); p.heads = v.size(2); p.dv = v.size(3);
     p.heads_k = k.size(2); p.dk = k.size(3);
     p.dtype = dtype_code(v); p.gate_dtype = dtype_code(g);
-    p.reverse = reverse; p.for_backward = for_backward; p.scale = (float)scale;
+    p.reverse = reverse; p.for_backward = for_backward; p.scale = (float)scale; p.fp32_states = fp32_states;
     p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.g = g.data_ptr(); p.beta = beta.data_ptr();
     p.seq_lens = seq_lens.defined() ? static_cast<const int32_t*>(seq_lens.data_ptr()) : nullptr;
     p.q_batch_stride = q.stride(0); p.q_seq_stride = q.stride(1); p.q_head_stride = q.stride(2);
@@ -1031,7 +1031,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
         Tensor fin = want_final ? at::empty({v.size(0), v.size(2), k.size(3), v.size(3)}, f32) : Tensor();
         const Tensor s0 = initial_state.has_value() ? initial_state->contiguous() : Tensor();
         vms_gated_delta_params p{};
-        gated_delta_fill(p, q, k, v, g, beta, scale, seq_lens, reverse, for_backward);
+        gated_delta_fill(p, q, k, v, g, beta, scale, seq_lens, reverse, for_backward, want_final || initial_state.has_value());
         p.initial_state = s0.defined() ? s0.data_ptr<float>() : nullptr;
         p.final_state = fin.defined() ? fin.data_ptr<float>() : nullptr;
         p.out = out.data_ptr();
@@ -1044,6 +1044,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
             ctx->saved_data["scale"] = scale;
             ctx->saved_data["reverse"] = reverse;
             ctx->saved_data["state"] = initial_state.has_value();
+            ctx->saved_data["states"] = want_final || initial_state.has_value();
             ctx->set_materialize_grads(false);
         }
         return want_final ? variable_list{out, fin} : variable_list{out};
@@ -1058,7 +1059,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
             const Tensor dout = grads[0].defined() ? unit_last(grads[0].to(v.scalar_type())) : at::zeros(v.sizes(), v.options());
             const Tensor dfin = grads.size() > 1 && grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : Tensor();
             vms_gated_delta_bwd_params b{};
-            gated_delta_fill(b.f, q, k, v, g, beta, ctx->saved_data["scale"].toDouble(), seq_lens, ctx->saved_data["reverse"].toBool(), true);
+            gated_delta_fill(b.f, q, k, v, g, beta, ctx->saved_data["scale"].toDouble(), seq_lens, ctx->saved_data["reverse"].toBool(), true, ctx->saved_data["states"].toBool());
             b.f.workspace = ws.data_ptr(); b.f.workspace_bytes = ws.numel();
             r[0] = at::empty(q.sizes(), q.options());
             r[1] = at::empty(k.sizes(), k.options());

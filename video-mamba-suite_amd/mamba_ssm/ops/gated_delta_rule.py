@@ -58,7 +58,7 @@ class GatedDeltaRuleFn(torch.autograd.Function):
         ws = _k.gated_delta_fwd(q, k, v, g, beta, scale, s0, seq_lens, reverse, out, final, for_backward)
         if for_backward:
             ctx.save_for_backward(q, k, v, g, beta, seq_lens, ws)
-            ctx.meta = (scale, reverse, initial_state is not None)
+            ctx.meta = (scale, reverse, initial_state is not None, initial_state is not None or return_final_state)
             ctx.set_materialize_grads(False)
         return out, final
 
@@ -66,13 +66,13 @@ class GatedDeltaRuleFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
         q, k, v, g, beta, seq_lens, ws = ctx.saved_tensors
-        scale, reverse, has_state = ctx.meta
+        scale, reverse, has_state, states = ctx.meta
         dout = torch.zeros_like(v) if dout is None else _unit_last(dout.to(v.dtype))
         dfinal = dfinal.float().contiguous() if dfinal is not None else None
         new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
         dq, dk, dv, dg, dbeta = new(q), new(k), new(v), new(g), new(beta)
         ds = torch.empty((v.shape[0], v.shape[2], k.shape[-1], v.shape[-1]), dtype=torch.float32, device=v.device) if has_state else None
-        _k.gated_delta_bwd(q, k, v, g, beta, scale, seq_lens, reverse, ws, dout, dfinal, dq, dk, dv, dg, dbeta, ds)
+        _k.gated_delta_bwd(q, k, v, g, beta, scale, seq_lens, reverse, states, ws, dout, dfinal, dq, dk, dv, dg, dbeta, ds)
         return dq, dk, dv, dg, dbeta, ds, None, None, None, None
 
 
@@ -85,8 +85,8 @@ def gated_delta_rule_fn(q, k, v, g, beta, scale=None, initial_state=None, return
     that leaves the state alone, gives 0 and receives gradient 0.  Tokens are worked on 64 at a time: a NaN or infinity in a valid one reaches
     the outputs of its whole group of 64 and of what follows, none of the groups before.  batch, heads <= 65535, seqlen <= 2^30,
     batch * heads * ceil(dv / 32) < 2^23 (half of it for training in fp32).
-    What is computed on the way is carried to 2^-16 for fp16 and bf16 q, k, v, and to 2^-24 for fp32: final states and the gradients of fp32 gates
-    beside 16-bit q, k, v are fp32 numbers of that accuracy.
+    States are as exact as fp32 sums are, whatever q, k and v are; so are all gradients with an initial or a final state, or with fp32 q, k, v.  Without
+    either, fp16 and bf16 gradients are carried to 2^-16 on the way, and so are fp32 gates' beside them.
     -> out (batch, seqlen, heads, dv), with return_final_state (out, final_state fp32).  Differentiable once in q, k, v, g, beta, initial_state."""
     fast = _compiled("gated_delta_rule", v.is_cuda and v.numel())
     if fast is not None:

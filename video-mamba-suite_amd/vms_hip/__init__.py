@@ -116,7 +116,7 @@ class StateUpdateParams(ctypes.Structure):
 class GatedDeltaParams(ctypes.Structure):
     _fields_ = (
         [(n, _i32) for n in ("batch", "seqlen", "heads", "heads_k", "dk", "dv", "dtype", "gate_dtype", "reverse", "for_backward")]
-        + [("scale", ctypes.c_float), ("reserved", _i32)]
+        + [("scale", ctypes.c_float), ("fp32_states", _i32)]
         + [(n, _vp) for n in ("q", "k", "v", "g", "beta", "initial_state", "seq_lens", "out", "final_state")]
         + [(f"{t}_{d}_stride", _i64) for t in ("q", "k", "v", "out", "g", "beta") for d in ("batch", "seq", "head")]
         + [("workspace", _vp), ("workspace_bytes", _i64)]
@@ -1058,11 +1058,11 @@ def state_update(state, x, dt, A, B, C, D, z, dt_bias, out, dt_softplus):
 
 
 # ---- gated delta rule (csrc/gated_delta_fwd.hip, gated_delta_bwd.hip) ----------------------------------------
-def _fill_gated_delta(P, q, k, v, g, beta, scale, seq_lens, reverse, for_backward):
+def _fill_gated_delta(P, q, k, v, g, beta, scale, seq_lens, reverse, for_backward, fp32_states):
     P.batch, P.seqlen, P.heads, P.dv = v.shape
     P.heads_k, P.dk = k.shape[2:]
     P.dtype, P.gate_dtype = dtype_code(v), dtype_code(g)
-    P.reverse, P.for_backward, P.scale = int(bool(reverse)), int(bool(for_backward)), float(scale)
+    P.reverse, P.for_backward, P.scale, P.fp32_states = int(bool(reverse)), int(bool(for_backward)), float(scale), int(bool(fp32_states))
     P.q, P.k, P.v, P.g, P.beta, P.seq_lens = _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(seq_lens)
     P.q_batch_stride, P.q_seq_stride, P.q_head_stride = q.stride()[:3]
     P.k_batch_stride, P.k_seq_stride, P.k_head_stride = k.stride()[:3]
@@ -1075,7 +1075,7 @@ def gated_delta_fwd(q, k, v, g, beta, scale, initial_state, seq_lens, reverse, o
     """q, k, v, out: unit last stride; initial_state / final_state: contiguous fp32.  -> the workspace, which gated_delta_bwd of the same
     call reads (for_backward)"""
     P = GatedDeltaParams()
-    _fill_gated_delta(P, q, k, v, g, beta, scale, seq_lens, reverse, for_backward)
+    _fill_gated_delta(P, q, k, v, g, beta, scale, seq_lens, reverse, for_backward, initial_state is not None or final_state is not None)
     P.initial_state, P.final_state, P.out = _ptr(initial_state), _ptr(final_state), _ptr(out)
     P.out_batch_stride, P.out_seq_stride, P.out_head_stride = out.stride()[:3]
     ws = torch.empty(lib().vms_gated_delta_workspace_bytes(ctypes.byref(P)), dtype=torch.uint8, device=v.device)
@@ -1084,10 +1084,10 @@ def gated_delta_fwd(q, k, v, g, beta, scale, initial_state, seq_lens, reverse, o
     return ws
 
 
-def gated_delta_bwd(q, k, v, g, beta, scale, seq_lens, reverse, ws, dout, dfinal_state, dq, dk, dv, dg, dbeta, dinitial_state):
-    """dq .. dbeta, dinitial_state: contiguous, written whole"""
+def gated_delta_bwd(q, k, v, g, beta, scale, seq_lens, reverse, states, ws, dout, dfinal_state, dq, dk, dv, dg, dbeta, dinitial_state):
+    """dq .. dbeta, dinitial_state: contiguous, written whole; states: the forward had an initial or a final state"""
     Q = GatedDeltaBwdParams()
-    _fill_gated_delta(Q.f, q, k, v, g, beta, scale, seq_lens, reverse, True)
+    _fill_gated_delta(Q.f, q, k, v, g, beta, scale, seq_lens, reverse, True, states)
     Q.f.workspace, Q.f.workspace_bytes = _ptr(ws), ws.numel()
     Q.dout, Q.dfinal_state, Q.dinitial_state = _ptr(dout), _ptr(dfinal_state), _ptr(dinitial_state)
     Q.dq, Q.dk, Q.dv, Q.dg, Q.dbeta = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dg), _ptr(dbeta)
