@@ -453,9 +453,11 @@ struct OTile {
     }
 };
 
-// A walk's workgroup takes 32 columns of a head, or 16 where that leaves half of the CUs without one: a chunk of 16 columns takes 0.7 .. 0.8 of the time of one of
-// 32 (its chain is the same).  (2, 2304, 8 heads, 64 x 64): 32 workgroups 54 us, 64 workgroups 38 us; (8, 8192, 8 heads, 128 x 128): 256 workgroups
-// 265 us, 512 workgroups 404 us.
+// A walk's workgroup takes 32 columns of a head, or 16 where that leaves half of the CUs without one: a chunk of 16 columns takes 0.65 .. 0.75 of the time of one of
+// 32 (its chain is the same).  Forward / backward walk, us, 32 against 16 columns (bf16):
+//   (2, 2304, 8 heads, 64 x 64)      32 workgroups 77 / 72      64 workgroups 56 / 50
+//   (8, 3136, 6 heads, 128 x 128)   192 workgroups 184 / 168   384 workgroups 267 / 264
+//   (8, 8192, 8 heads, 128 x 128)   256 workgroups 388         512 workgroups 492
 inline bool narrow(const vms_gated_delta_params& p, const Layout& l) { return (int64_t)p.batch * p.heads * (l.vpad / 32) <= device_cu_count() / 2; }
 
 // The most columns that the backward's walk takes: the planes of fp32, and three of fp16 beside 128-wide keys, leave LDS for one column tile

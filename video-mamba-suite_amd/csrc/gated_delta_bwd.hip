@@ -27,7 +27,7 @@ struct BwdArgs {   // what the kernels need of vms_gated_delta_bwd_params (one k
 // ---- the walk over the chunks, from the end ------------------------------------------------------------------
 // Split among eight waves as the forward's walk: of the chain's four, wave w has token tile w of dU and Y and dk / 4 rows of dS; the other four load, make
 // what depends on no dS (M^T dO, the planes of dO and of scale gam dO) and store.  Bound by the chain (K dS1 -> dU -> Y -> dS0): (8, 3136, 6 heads, 128 x 128) bf16
-// 2.7 us per chunk, 131 us; with all of it on four waves 164 us.
+// 3.4 us per chunk, 169 us, 7200 cycles of which LDS works 3100, 1170 on bank conflicts; with one plane for what is stored 131 us, all of it on four waves then 164 us.
 template <typename T, int NB, int KP, int CT, int FIT>
 struct BwdScanLds {   // bytes and places in LDS
     static constexpr int NX = Prec<T>::NX;
@@ -348,8 +348,9 @@ __device__ __forceinline__ float quarters_sum(float v) {   // over the four lane
 // Stage 1 walks v 32 columns at a time: U, Y, dO (64 rows) and S0, dS1 (KP rows) go through registers (the next block is on its way while this one is
 // multiplied) into LDS, 16-byte operands from there; the sums that need no product (Y.V, <S0, dS1>) are taken from the pieces as they pass.  Eight waves:
 // wave w has token tile w % 4 of dQ and W (w < 4: "left", what depends on the token as the later one) or of X (w >= 4: "right"), so that no product is
-// made twice and the accumulators fit.  (8, 3136, 6 heads, 128 x 128) bf16: 145 us for 0.45 GB and 30 GFLOP of bf16 products; bound by the steps between
-// the barriers (a workgroup of eight waves fills a CU's registers).  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
+// made twice and the accumulators fit.  (8, 3136, 6 heads, 128 x 128) bf16: 278 us for 0.69 GB and 70 GFLOP of bf16 products (145 us for
+// 0.45 GB and 36 GFLOP with one plane); bound by the steps between the barriers (a workgroup of eight waves fills a CU's registers) and by LDS, half of whose cycles
+// are bank conflicts.  Stage 2 multiplies the 64 x 64 results with Q and K, whose tiles take stage 1's place in LDS.
 template <typename T, int NB, int KP, bool WHOLE, bool SHARED>   // WHOLE: dk % 8 == 0 and dv % 8 == 0; SHARED: several heads per q / k head
 __global__ __launch_bounds__(512, 2) void gd_grad_kernel(const BwdArgs a) {
     constexpr int NX = Prec<T>::NX, DT = KP / 16, TB = tile_bytes<KP>();

@@ -17,8 +17,8 @@ constexpr float kMinGate = -104.f;
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // ---- T, M and gates of one chunk -----------------------------------------------------------------------------
-// Bound by bytes: (8, 8192, 8 heads, 128) bf16 reads 268 MB of q and k and writes 161 MB in 83 us, the 5.2 TB/s of a large copy; in calls with few
-// chunks by one wave's chain of steps (8 us, bf16, 64).
+// Bound by bytes: (8, 8192, 8 heads, 128) bf16 reads 268 MB of q and k and writes 262 MB in 96 us, 5.5 TB/s (a large copy: 5.2); in calls with few
+// chunks by one wave's chain of steps (10 us, bf16, 64).
 // K K^T and Q K^T (16x16x32 bf16 MFMA, operands straight from memory), L from double cumulative sums (differences of long sums keep
 // their bits), then T: the four 16 x 16 diagonal blocks by forward substitution (16 lanes each, a column per lane; a power series would
 // lose ~13 bits to the binomials of equal keys), joined by T21 = -T22 A21 T11 with fp32 MFMA.
@@ -246,11 +246,13 @@ __global__ __launch_bounds__(64, 2) void gd_prep_kernel(const vms_gated_delta_pa
 
 // ---- the walk over the chunks --------------------------------------------------------------------------------
 // What bounds it is the chain of one chunk (K S0 -> R -> U -> S1), not a rate: a head is 16 .. 64 tokens of work per step on one CU.  (8, 8192, 8 heads,
-// 128 x 128) bf16, 263 us: 2.05 us per chunk, of which the matrix cores work 0.4; S0 is read by eight waves from LDS (0.35 us at 128 bytes per cycle) and
-// handed over three times.  Steps that led here, same sizes:
-//   a wave with a whole chunk of 16 columns to itself, every wave reading all of K, Q, T, M from LDS             5.4 us per chunk
+// 128 x 128) bf16, 378 us: 2.95 us or 5800 cycles per chunk, of which the matrix cores work 1460 and LDS 3820: S0's planes are read by eight waves (three by the chain, two
+// by the others) and handed over three times, and 1680 cycles go to bank conflicts (rows of K's tile, whose pitch suits the transposing reads, 8-byte writes of the
+// exchanges, V's tile).  Steps that led here, same sizes, us per chunk:
+//   a wave with a whole chunk of 16 columns to itself, every wave reading all of K, Q, T, M from LDS             5.4
 //   four waves on one chunk, K, Q, T, M straight from memory, a chunk ahead                                      2.4
 //   four waves on the chain, four on loads and outputs; lines instead of operands from memory                    2.05
+//   three planes on the chain instead of two, two instead of one in the outputs (for their accuracy)             2.95
 // Lines: an operand's lanes are 16 rows x 4 pieces of 16 bytes with neighbouring lanes in different rows, and the memory pipe then takes 64 accesses
 // for a load of 1 KB instead of 16 (2825 of a chunk's 5100 cycles).  Read as lines, through LDS into operands, K also stands there for its transpose.  Asked
 // for two chunks ahead (one chunk is less than a loaded memory's latency) and spread over the phases: a wave stands still while the pipe is full.
