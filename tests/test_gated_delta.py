@@ -151,6 +151,24 @@ def test_c_entry_refuses_launches_of_2_to_the_32_threads(dtype, for_backward, dv
         assert L.vms_gated_delta_fwd(ctypes.byref(P), None) < 0 and message in L.vms_last_error(), L.vms_last_error()
 
 
+def test_c_messages_hold_their_condition():
+    """conditions with a % in them used to be the format of the message"""
+    import ctypes
+
+    import vms_hip
+    L = vms_hip.lib()
+    P, S, N = vms_hip.GatedDeltaParams(), vms_hip.GatedDeltaStepParams(), vms_hip.SandwichNormParams()
+    P.seqlen = P.batch = S.batch = 1
+    P.heads = S.heads = 3
+    P.heads_k = S.heads_k = 2
+    for fn, p in ((L.vms_gated_delta_fwd, P), (L.vms_gated_delta_state_update, S)):
+        assert fn(ctypes.byref(p), None) < 0
+        assert L.vms_last_error() == b"vms check failed: p.heads % p.heads_k == 0 -- heads must be a multiple of heads_k"
+    N.rows, N.cols, N.rows_per_gate = 4, 16, 3
+    N.x = N.post_weight = N.pre_weight = N.gate = 256
+    assert L.vms_sandwich_norm_fwd(ctypes.byref(N), None) < 0 and b"p.rows % p.rows_per_gate == 0 -- rows must" in L.vms_last_error()
+
+
 def test_a_library_without_an_entry_is_refused_when_it_is_loaded(tmp_path, monkeypatch):
     """built before the entry was added, with the version of now: an ImportError that says what to do, not an AttributeError later"""
     import shutil

@@ -219,6 +219,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // ---- host-side plumbing (vms_host.hip) ---------------------------------------------------------------
 void set_error(const char* fmt, ...);      // thread-local message behind vms_last_error()
+void set_check_error(const char* cond, const char* fmt, ...);   // the condition as it stands: it may hold a %
 const char* last_error();
 void set_last_kernel(const char* name);    // thread-local name behind vms_last_kernel()
 // compute units of the calling thread's current device; immutable per device, looked up once per device
@@ -249,7 +250,7 @@ inline int scan_impl_level(const vms_scan_fwd_params& p) { return p.impl == VMS_
 #define VMS_CHECK(cond, ...)                                              \
     do {                                                                  \
         if (!(cond)) {                                                    \
-            ::vms::set_error("vms check failed: " #cond " -- " __VA_ARGS__); \
+            ::vms::set_check_error(#cond, __VA_ARGS__);                   \
             return VMS_ERR_INVALID_ARG;                                   \
         }                                                                 \
     } while (0)

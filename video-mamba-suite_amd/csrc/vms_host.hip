@@ -25,6 +25,14 @@ void set_error(const char* fmt, ...) {
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
 }
+void set_check_error(const char* cond, const char* fmt, ...) {
+    const int n = snprintf(g_err, sizeof(g_err), "vms check failed: %s -- ", cond);
+    if (n < 0 || n >= (int)sizeof(g_err)) return;
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err + n, sizeof(g_err) - n, fmt, ap);
+    va_end(ap);
+}
 const char* last_error() { return g_err; }
 void set_last_kernel(const char* name) { g_kernel = name; }
 
